@@ -254,8 +254,9 @@ def _adamw_plain(s):
 def _adamw_own(s):
     from probtalk_amd import train_ops as T
     f, x = s["flat"], s["lists"]
-    norm, coef = T.grad_norm(x["grad"], s["max_norm"])
-    T.adamw_step(x["param"], x["grad"], x["m"], x["v"], x.get("scale"), coef=coef, seed=s["seed"], **s["hyper"])
+    if "list" not in s:                       # an optimizer keeps it with its moments
+        s["list"] = T.AdamWList(x["param"], x["m"], x["v"], x.get("scale"))
+    norm = s["list"].step(x["grad"], max_norm=s["max_norm"], seed=s["seed"], **s["hyper"])
     m, v = T.moment_values(f["m"], f["v"], f["scale"]) if s["bits"] == 8 else (f["m"], f["v"])
     return {"norm": norm[0], "param": f["param"], "exp_avg": m, "exp_avg_sq": v}
 
