@@ -262,6 +262,26 @@ int pt_train_clip_coef(const float* sumsq, float max_norm, float* coef, float* n
 int pt_train_adamw(float* p, const float* g, float* m, float* v, size_t n, const float* gscale, float lr, float beta1,
                    float beta2, float eps, float wd, int step, void* stream);
 int pt_train_add(const float* a, const float* b, float* out, size_t n, void* stream);
+/* The same two over a whole list of tensors (host arrays of `count` device pointers and sizes; entries of size 0 are skipped; a
+ * call reads the arrays before it returns).
+ * pt_train_grad_norm: *norm = sqrt(sum over the list of g^2), *coef = min(1, max_norm / (*norm + 1e-6)); is_bf16 (may be NULL: all
+ *   fp32) marks tensors held in bf16.  Squares are summed in fp64 in a fixed order: the same gradients give the same bits.  ws:
+ *   pt_train_grad_norm_workspace_bytes(n, count) bytes, 8-byte aligned.
+ * pt_train_adamw_multi: the update of pt_train_adamw on every tensor.  dtype of p and g: 0 fp32, 1 bf16 (parameters are then rounded
+ *   stochastically).  scales NULL: m and v are fp32.  Else m and v hold one byte a value and scales[i] points to
+ *   ceil(n[i] / 256) x 2 floats, the scales of each block of 256 values for m and v: a magnitude code c stands for scale * c below
+ *   2^M, for scale * (2^M + c mod 2^M) * 2^(c / 2^M - 1) above; m: sign in bit 7, M = 3; v: M = 4.  All zero = moments of zero.
+ *   New codes are rounded stochastically with 32 bits of hash(seed, step, position in the list) per value.
+ *   step >= 1; or step_dev: a device int32 that holds it, with dyn = 3 floats of device scratch (a captured step: the caller
+ *   advances *step_dev on the stream before each replayed step).
+ * pt_train_moment_values: the fp32 values that n codes of one tensor stand for. */
+size_t pt_train_grad_norm_workspace_bytes(const int64_t* n, int count);
+int pt_train_grad_norm(const void* const* g, const int64_t* n, const uint8_t* is_bf16, int count, float max_norm, float* norm,
+                       float* coef, void* ws, size_t ws_bytes, void* stream);
+int pt_train_adamw_multi(void* const* p, const void* const* g, void* const* m, void* const* v, float* const* scales, const int64_t* n,
+                         int count, int dtype, const float* gscale, float lr, float beta1, float beta2, float eps, float wd, int step,
+                         const int32_t* step_dev, float* dyn, uint32_t seed, void* stream);
+int pt_train_moment_values(const uint8_t* m, const uint8_t* v, const float* scales, int64_t n, float* m_out, float* v_out, void* stream);
 /* ProductQuantization.forward train branch (vqvae_modules.py:495-534): EMA cluster sizes / code sums from the assigned
  * latent rows, Laplace smoothing, dead-code re-seeding from the first K latent rows, new codebooks.  z rows [rows, ldz]
  * (G*D used columns), idx int64 [rows, G]; counts [G,K] and dw [G,K,D] are scratch; cs_hidden [G,K], dw_hidden [G,K,D],

@@ -35,6 +35,10 @@ int launch_sumsq(const float* g, size_t n, float* out, hipStream_t s);
 int launch_adamw(float* p, const float* g, float* m, float* v, size_t n, const float* gscale, float lr, float beta1, float beta2, float eps, float wd, int step, hipStream_t s);
 int launch_clip_coef(const float* sumsq, float max_norm, float* coef, float* norm_out, hipStream_t s);
 int launch_add(const float* a, const float* b, float* out, size_t n, hipStream_t s);
+int launch_adamw_multi(void* const* p, const void* const* g, void* const* m, void* const* v, float* const* scales, const int64_t* n, int count, int dtype, const float* gscale, float lr, float beta1, float beta2, float eps, float wd, int step, const int* step_dev, float* dyn, unsigned seed, hipStream_t s);
+int launch_moment_values(const unsigned char* m, const unsigned char* v, const float* scales, int64_t n, float* m_out, float* v_out, hipStream_t s);
+size_t grad_norm_workspace(const int64_t* n, int count);
+int launch_grad_norm(const void* const* g, const int64_t* n, const unsigned char* is_bf16, int count, float max_norm, float* norm, float* coef, void* ws, size_t ws_bytes, hipStream_t s);
 int launch_attention_bf16(const unsigned short* Q, int ldq, const unsigned short* K, int ldk, const unsigned short* V, int ldv, unsigned short* O, int ldo, int B, int Nq, int Nk, int H, hipStream_t s);
 int launch_maskgit_noise(unsigned long long seed, int step, int B, int N, int V, float* q, float* g, hipStream_t s);
 int launch_maskgit_bits(const unsigned* bits, int n, float* u, float* q, float* g, hipStream_t s);
@@ -524,6 +528,20 @@ int pt_train_clip_coef(const float* sumsq, float max_norm, float* coef, float* n
 int pt_train_adamw(float* p, const float* g, float* m, float* v, size_t n, const float* gscale, float lr, float beta1,
                    float beta2, float eps, float wd, int step, void* stream) {
   return launch_adamw(p, g, m, v, n, gscale, lr, beta1, beta2, eps, wd, step, (hipStream_t)stream);
+}
+int pt_train_adamw_multi(void* const* p, const void* const* g, void* const* m, void* const* v, float* const* scales, const int64_t* n,
+                         int count, int dtype, const float* gscale, float lr, float beta1, float beta2, float eps, float wd, int step,
+                         const int32_t* step_dev, float* dyn, uint32_t seed, void* stream) {
+  return launch_adamw_multi(p, g, m, v, scales, n, count, dtype, gscale, lr, beta1, beta2, eps, wd, step, step_dev, dyn, seed,
+                            (hipStream_t)stream);
+}
+int pt_train_moment_values(const uint8_t* m, const uint8_t* v, const float* scales, int64_t n, float* m_out, float* v_out, void* stream) {
+  return launch_moment_values(m, v, scales, n, m_out, v_out, (hipStream_t)stream);
+}
+size_t pt_train_grad_norm_workspace_bytes(const int64_t* n, int count) { return n && count > 0 ? grad_norm_workspace(n, count) : sizeof(double); }
+int pt_train_grad_norm(const void* const* g, const int64_t* n, const uint8_t* is_bf16, int count, float max_norm, float* norm,
+                       float* coef, void* ws, size_t ws_bytes, void* stream) {
+  return launch_grad_norm(g, n, is_bf16, count, max_norm, norm, coef, ws, ws_bytes, (hipStream_t)stream);
 }
 int pt_train_add(const float* a, const float* b, float* out, size_t n, void* stream) {
   return launch_add(a, b, out, n, (hipStream_t)stream);

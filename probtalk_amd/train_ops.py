@@ -7,6 +7,10 @@ All activations are channels-last 2-D fp32 tensors `[B*L, C]` with C a multiple 
 of the inference library.  Conv `kind`: 0 = Linear / 1x1, 1 = k3 s1 p1, 2 = k7 s1 p3, 3 = k4 s2 p1, 4 = ConvTranspose
 k4 s2 p1 (reference shapes: nets/spg/vqvae_modules.py:107-200, nets/inpainting/gated_pixelcnn_1d.py:39-83).
 """
+import array
+import contextlib
+import ctypes as C
+
 import torch
 
 from . import _lib
@@ -198,7 +202,6 @@ class Attention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, kv, q_off, k_off, v_off, B, Nq, Nk, p, seed):
-        import ctypes as C
         L = _lib.lib()
         o = _empty(B * Nq, 512)
         qb, kb = q.data_ptr() + 4 * q_off, kv.data_ptr()
@@ -214,7 +217,6 @@ class Attention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do):
-        import ctypes as C
         q, kv = ctx.saved_tensors
         q_off, k_off, v_off, B, Nq, Nk, p, seed, packed = ctx.meta
         L = _lib.lib()
@@ -524,7 +526,6 @@ class VQLosses(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, pred, gt, B, Tn, bounds, weights, vel_cols, beta):
-        import ctypes as C
         L = _lib.lib()
         nparts = len(weights)
         sums = _zeros(nparts + 2)
@@ -548,7 +549,6 @@ class MaskedL1Losses(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, pred, gt, nmask, t_nmask, B, Tn, bounds, weights, vel_cols):
-        import ctypes as C
         L = _lib.lib()
         nparts = len(weights)
         sums = _zeros(nparts + 2)
@@ -569,52 +569,223 @@ class MaskedL1Losses(torch.autograd.Function):
 # ---------------------------------------------------------------------------------------------------------------
 # optimizer side: torch.nn.utils.clip_grad_norm_ + torch.optim.AdamW semantics on HIP kernels
 # ---------------------------------------------------------------------------------------------------------------
+MOMENT_BLOCK = 256      # values of an 8-bit moment that share a scale
+
+
+def _on(device):
+    """Launches go to the current stream of the tensors' device."""
+    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _same(what, tensors, dtypes, device=None):
+    """The device of `tensors`, checked with their types and layout."""
+    for t in tensors:
+        if not torch.is_tensor(t) or not t.is_cuda:
+            raise RuntimeError(f"{what}: tensors must be on the GPU")
+        device = device or t.device
+        if t.device != device:
+            raise RuntimeError(f"{what}: tensors on {device} and {t.device}")
+        if t.dtype not in dtypes:
+            raise RuntimeError(f"{what}: {t.dtype} where {' or '.join(map(str, dtypes))} is taken")
+        if not t.is_contiguous():
+            raise RuntimeError(f"{what}: tensors must be contiguous")
+    return device
+
+
+def _addresses(tensors):
+    return array.array("Q", map(torch.Tensor.data_ptr, tensors))
+
+
+def _address(a):
+    return None if a is None else C.c_void_p(a.buffer_info()[0])
+
+
+def _grad_norm(pointers, sizes, is_bf16, max_norm, device):
+    L = _lib.lib()
+    n = len(pointers)
+    out = torch.empty(2, device=device, dtype=torch.float32)
+    ws = torch.empty(int(L.pt_train_grad_norm_workspace_bytes(_address(sizes), n)), dtype=torch.uint8, device=device)
+    check(L.pt_train_grad_norm(_address(pointers), _address(sizes), is_bf16, n, float(max_norm), ptr(out), C.c_void_p(out.data_ptr() + 4),
+                               ptr(ws), ws.numel(), stream()))
+    return out[:1], out[1:]
+
+
+def grad_norm(grads, max_norm):
+    """(norm, coef), two device tensors of one float: the norm over all of `grads` (fp32 or bf16) and the factor
+    min(1, max_norm / (norm + 1e-6)) of torch.nn.utils.clip_grad_norm_.  The sum runs in fp64 in a fixed order."""
+    grads = [g.contiguous() for g in grads]
+    device = _same("grad_norm", grads, (torch.float32, torch.bfloat16)) if grads else torch.device("cuda", torch.cuda.current_device())
+    kinds = None
+    if any(g.dtype is torch.bfloat16 for g in grads):
+        kinds = bytes(g.dtype is torch.bfloat16 for g in grads)
+    with _on(device):
+        return _grad_norm(_addresses(grads), array.array("q", [g.numel() for g in grads]), kinds, max_norm, device)
+
+
 def clip_grad_norm(params, max_norm):
     """Scales the gradients' effect by min(1, max_norm / (total_norm + 1e-6)); returns (total_norm tensor, coef tensor).
     The coefficient stays on the device and is applied inside the AdamW kernel (no extra pass over the gradients)."""
-    L = _lib.lib()
-    ss, coef, norm = _zeros(1), _empty(1), _empty(1)
-    for p in params:
-        if p.grad is not None:
-            g = p.grad.contiguous()
-            check(L.pt_train_sumsq(ptr(g), g.numel(), ptr(ss), stream()))
-    check(L.pt_train_clip_coef(ptr(ss), float(max_norm), ptr(coef), ptr(norm), stream()))
-    return norm, coef
+    return grad_norm([p.grad for p in params if p.grad is not None], max_norm)
+
+
+class AdamWList:
+    """AdamW over a fixed list of tensors, a few launches a step whatever their number.
+
+    params: fp32, or bf16 (then rounded stochastically).  exp_avgs, exp_avg_sqs: fp32 tensors of the parameters' sizes; or, with
+    `scales`, uint8 tensors of these sizes (8-bit moments) and one fp32 tensor (ceil(n / 256), 2) each: the scales of every block
+    of 256 values for the first and the second moment.  Zeros everywhere stand for moments of zero.  `moment_values` gives what
+    8-bit moments stand for.  All are updated in place; the list keeps their memory, so it does not follow a tensor whose
+    `.data` is exchanged afterwards.  Two steps of one list must not run at the same time on two streams."""
+
+    def __init__(self, params, exp_avgs, exp_avg_sqs, scales=None):
+        lists = [[t.detach() for t in x] for x in ((params, exp_avgs, exp_avg_sqs) if scales is None else
+                                                   (params, exp_avgs, exp_avg_sqs, scales))]
+        params, exp_avgs, exp_avg_sqs = lists[:3]
+        if not params or any(len(x) != len(params) for x in lists):
+            raise RuntimeError(f"AdamWList: lists of {', '.join(str(len(x)) for x in lists)} tensors")
+        self.dtype = params[0].dtype
+        self.device = _same("AdamWList", params, (torch.float32, torch.bfloat16))
+        _same("AdamWList", params, (self.dtype,))
+        _same("AdamWList", exp_avgs + exp_avg_sqs, (torch.float32 if scales is None else torch.uint8,), self.device)
+        for i, p in enumerate(params):
+            if not p.numel() == exp_avgs[i].numel() == exp_avg_sqs[i].numel():
+                raise RuntimeError(f"AdamWList: tensor {i} has {p.numel()} values, its moments {exp_avgs[i].numel()} and {exp_avg_sqs[i].numel()}")
+        if scales is not None:
+            _same("AdamWList", lists[3], (torch.float32,), self.device)
+            for p, s in zip(params, lists[3]):
+                if tuple(s.shape) != (-(-p.numel() // MOMENT_BLOCK), 2):
+                    raise RuntimeError(f"AdamWList: {p.numel()} values have scales of shape {(-(-p.numel() // MOMENT_BLOCK), 2)}, not {tuple(s.shape)}")
+        self._lists = lists                  # holds the memory behind the addresses
+        self._arrays = [_addresses(x) for x in lists] + ([None] if scales is None else [])
+        for a in self._arrays:
+            used = [x for x in a or () if x]
+            if len(set(used)) != len(used):
+                raise RuntimeError("AdamWList: the same tensor twice")
+        self.sizes = [p.numel() for p in params]
+        self._n = array.array("q", self.sizes)
+        self._elems = sum(self.sizes)
+
+    def step(self, grads, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, coef=None, max_norm=None, seed=0):
+        """One step with `grads` (of the parameters' type and sizes).  coef: device scalar that scales the gradients; max_norm
+        instead: the coefficient of this list's own gradient norm, which is then returned.  step: the count of this step, from
+        1; or a CUDA int32 tensor of one value that holds it, read when the step runs (a captured step needs that: the
+        caller adds 1 to it inside the capture).  seed: of the random bits of stochastic roundings."""
+        if len(grads) != len(self.sizes):
+            raise RuntimeError(f"AdamWList.step: {len(grads)} gradients for {len(self.sizes)} parameters")
+        if not all(map(torch.Tensor.is_contiguous, grads)):
+            grads = [g.contiguous() for g in grads]
+        if list(map(torch.Tensor.numel, grads)) != self.sizes:
+            raise RuntimeError("AdamWList.step: a gradient has another size than its parameter")
+        if set(map(torch.Tensor.get_device, grads)) != {self.device.index} or not all([g.dtype is self.dtype for g in grads]):
+            raise RuntimeError(f"AdamWList.step: gradients must be {self.dtype} on {self.device}")
+        if coef is not None and max_norm is not None:
+            raise RuntimeError("AdamWList.step: coef or max_norm, not both")
+        on_device = torch.is_tensor(step)
+        if on_device:
+            _same("AdamWList.step", [step], (torch.int32,), self.device)
+            if step.numel() != 1:
+                raise RuntimeError("AdamWList.step: step is one value")
+        elif step < 1:
+            raise RuntimeError(f"AdamWList.step: steps count from 1, got {step}")
+        if coef is not None:
+            _same("AdamWList.step", [coef], (torch.float32,), self.device)
+            if coef.numel() != 1:
+                raise RuntimeError("AdamWList.step: coef is one value")
+        norm = None
+        with _on(self.device):
+            if not on_device and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamWList.step: a captured step would repeat one step count: pass `step` as a CUDA int32 tensor")
+            g = _addresses(grads)
+            if max_norm is not None:
+                norm, coef = _grad_norm(g, self._n, bytes([1]) * len(grads) if self.dtype is torch.bfloat16 else None, max_norm, self.device)
+            dyn = torch.empty(3, device=self.device, dtype=torch.float32) if on_device else None
+            P, M, V, S = map(_address, self._arrays)
+            check(_lib.lib().pt_train_adamw_multi(P, _address(g), M, V, S, _address(self._n), len(grads),
+                                                  int(self.dtype is torch.bfloat16), ptr(coef), lr, betas[0], betas[1], eps, weight_decay,
+                                                  0 if on_device else step, ptr(step) if on_device else None, ptr(dyn), seed & 0xFFFFFFFF,
+                                                  stream()))
+        return norm
+
+
+def moment_values(exp_avg, exp_avg_sq, scale):
+    """The fp32 values that the 8-bit moments of one tensor stand for (see AdamWList)."""
+    device = _same("moment_values", [exp_avg, exp_avg_sq], (torch.uint8,))
+    _same("moment_values", [scale], (torch.float32,), device)
+    n = exp_avg.numel()
+    if exp_avg_sq.numel() != n or tuple(scale.shape) != (-(-n // MOMENT_BLOCK), 2):
+        raise RuntimeError(f"moment_values: {n} and {exp_avg_sq.numel()} codes with scales of shape {tuple(scale.shape)}")
+    m, v = (torch.empty(t.shape, device=device, dtype=torch.float32) for t in (exp_avg, exp_avg_sq))
+    with _on(device):
+        check(_lib.lib().pt_train_moment_values(ptr(exp_avg), ptr(exp_avg_sq), ptr(scale), n, ptr(m), ptr(v), stream()))
+    return m, v
 
 
 class AdamW:
-    """torch.optim.AdamW (amsgrad off) on the library's kernel; state_dict()/load_state_dict() use torch's layout."""
+    """torch.optim.AdamW (amsgrad off) on the library's kernel; state_dict()/load_state_dict() use torch's layout.
+    state_bits = 8 holds the moments in a byte each (AdamWList), with a third state tensor 'scale'; its stochastic rounding
+    draws from `seed`."""
 
-    def __init__(self, param_groups, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    def __init__(self, param_groups, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits!r}")
         self.param_groups = [dict(params=list(g["params"]), lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay)
                              for g in param_groups]
         self.state = {}
+        self.state_bits, self.seed = state_bits, int(seed)
+        self._lists = {}
 
     def zero_grad(self):
         for g in self.param_groups:
             for p in g["params"]:
                 p.grad = None
 
+    def _names(self):
+        return ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq", "scale")
+
+    def _state(self, p):
+        st = self.state.get(p)
+        if st is None:
+            if self.state_bits == 32:
+                st = {k: torch.zeros(p.shape, device=p.device, dtype=torch.float32) for k in ("exp_avg", "exp_avg_sq")}
+            else:
+                st = {k: torch.zeros(p.shape, device=p.device, dtype=torch.uint8) for k in ("exp_avg", "exp_avg_sq")}
+                st["scale"] = torch.zeros(-(-p.numel() // MOMENT_BLOCK), 2, device=p.device, dtype=torch.float32)
+            st = self.state[p] = {"step": 0} | st
+        if not p.is_cuda:
+            raise RuntimeError("AdamW.step: parameters must be on the GPU")
+        for k in self._names():                    # state restored before the module moved to the GPU
+            if st[k].device != p.device:
+                st[k] = st[k].to(p.device)
+        return st
+
+    def _list(self, ps, sts):
+        """The AdamWList of these parameters: made once, and anew where a parameter's or a moment's memory is another."""
+        key = tuple(map(id, ps))
+        held = [x for k in self._names() for x in map(torch.Tensor.data_ptr, [st[k] for st in sts])] + list(map(torch.Tensor.data_ptr, ps))
+        made = self._lists.get(key)
+        if made is None or made[1] != held:
+            if len(self._lists) >= 32:
+                self._lists.clear()
+            made = self._lists[key] = (AdamWList(ps, *([st[k] for st in sts] for k in self._names())), held, ps)
+        return made[0]
+
     def step(self, coefs=None):
         """coefs: optional {param: device scalar} of clip coefficients."""
-        L = _lib.lib()
-        for g in self.param_groups:
+        for gi, g in enumerate(self.param_groups):
+            parts = {}
             for p in g["params"]:
                 if p.grad is None:
                     continue
-                st = self.state.get(p)
-                if st is None:
-                    st = self.state[p] = {"step": 0, "exp_avg": torch.zeros_like(p), "exp_avg_sq": torch.zeros_like(p)}
-                if not p.is_cuda:
-                    raise RuntimeError("AdamW.step: parameters must be on the GPU")
-                for k in ("exp_avg", "exp_avg_sq"):        # state restored before the module moved to the GPU
-                    if st[k].device != p.device:
-                        st[k] = st[k].to(p.device)
-                st["step"] += 1
+                st = self._state(p)
                 c = None if coefs is None else coefs.get(p)
-                gr = p.grad.contiguous()
-                check(L.pt_train_adamw(ptr(p.data), ptr(gr), ptr(st["exp_avg"]), ptr(st["exp_avg_sq"]), p.numel(), ptr(c),
-                                       g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"], st["step"], stream()))
+                part = parts.setdefault((id(c), st["step"], p.dtype, p.device), (c, [], []))
+                part[1].append(p)
+                part[2].append(st)
+            for k, ((_, done, _, _), (c, ps, sts)) in enumerate(parts.items()):
+                self._list(ps, sts).step([p.grad for p in ps], done + 1, g["lr"], g["betas"], g["eps"], g["weight_decay"], coef=c,
+                                         seed=self.seed + 0x10001 * gi + 0x1000003 * k)
+                for st in sts:
+                    st["step"] = done + 1
 
     def state_dict(self):
         idx, packed, groups = {}, {}, []
@@ -625,15 +796,23 @@ class AdamW:
                 ids.append(idx[p])
             groups.append({k: v for k, v in g.items() if k != "params"} | {"params": ids})
         for p, st in self.state.items():
-            packed[idx[p]] = {"step": torch.tensor(float(st["step"])), "exp_avg": st["exp_avg"], "exp_avg_sq": st["exp_avg_sq"]}
+            packed[idx[p]] = {"step": torch.tensor(float(st["step"]))} | {k: st[k] for k in self._names()}
         return {"state": packed, "param_groups": groups}
 
     def load_state_dict(self, sd):
         flat = [p for g in self.param_groups for p in g["params"]]
         for i, st in sd.get("state", {}).items():
             p = flat[int(i)]
-            self.state[p] = {"step": int(float(st["step"])), "exp_avg": st["exp_avg"].to(p.device).float().clone(),
-                             "exp_avg_sq": st["exp_avg_sq"].to(p.device).float().clone()}
+            if self.state_bits == 8:
+                if "scale" not in st:
+                    raise RuntimeError("AdamW: a state with moments in 32 bits cannot be loaded with state_bits=8")
+                new = {k: st[k].to(p.device).clone() for k in self._names()}
+            elif "scale" in st:                    # moments saved in 8 bits: what they stand for
+                m, v = moment_values(*(st[k].to("cuda") for k in ("exp_avg", "exp_avg_sq", "scale")))
+                new = {"exp_avg": m.to(p.device), "exp_avg_sq": v.to(p.device)}
+            else:
+                new = {k: st[k].to(p.device).float().clone() for k in self._names()}
+            self.state[p] = {"step": int(float(st["step"]))} | new
         for g, sg in zip(self.param_groups, sd.get("param_groups", [])):
             for k in ("lr", "betas", "eps", "weight_decay"):
                 if k in sg:

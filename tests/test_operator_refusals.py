@@ -1,0 +1,38 @@
+"""What the operators refuse before anything reaches a GPU: wrong arguments at the C entries and tensors on the host."""
+import ctypes as C
+
+import pytest
+import torch
+
+from probtalk_amd import _lib
+from probtalk_amd import train_ops as T
+
+
+def refused(rc, word):
+    assert rc != 0 and word in _lib.lib().pt_last_error().decode()
+
+
+def test_adamw_list_refuses_host_tensors():
+    t = [torch.zeros(4)]
+    with pytest.raises(RuntimeError, match="GPU"):
+        T.AdamWList(t, t, t)
+    with pytest.raises(RuntimeError, match="GPU"):
+        T.grad_norm(t, 1.0)
+
+
+def test_c_entries_of_the_lists():
+    L = _lib.lib()
+    n, null, p = (C.c_int64 * 2)(10, 0), (C.c_void_p * 2)(None, None), (C.c_void_p * 2)(256, None)
+    out = C.c_void_p(256)
+    refused(L.pt_train_grad_norm(null, n, None, 2, 1.0, out, out, out, 64, None), "null tensor 0")
+    refused(L.pt_train_grad_norm(p, n, None, 2, 1.0, out, out, None, 64, None), "bad argument")
+    refused(L.pt_train_grad_norm(p, n, None, 2, 1.0, out, out, out, 4, None), "workspace")
+    refused(L.pt_train_grad_norm(p, n, None, 2, 1.0, out, out, C.c_void_p(260), 64, None), "workspace")
+    assert L.pt_train_grad_norm_workspace_bytes((C.c_int64 * 3)(1, 16384, 16385), 3) == 8 * 4
+    h = (None, 1e-3, 0.9, 0.99, 1e-8, 0.0)
+    refused(L.pt_train_adamw_multi(p, p, p, null, None, n, 2, 0, *h, 1, None, None, 0, None), "null tensor 0")
+    refused(L.pt_train_adamw_multi(p, p, p, p, null, n, 2, 0, *h, 1, None, None, 0, None), "null tensor 0")
+    refused(L.pt_train_adamw_multi(p, p, p, p, None, n, 2, 2, *h, 1, None, None, 0, None), "bad argument")
+    refused(L.pt_train_adamw_multi(p, p, p, p, None, n, 2, 0, *h, 0, None, None, 0, None), "step")
+    refused(L.pt_train_adamw_multi(p, p, p, p, None, n, 2, 0, *h, 0, out, None, 0, None), "scratch")
+    refused(L.pt_train_moment_values(None, out, out, 4, out, out, None), "bad argument")
