@@ -222,6 +222,22 @@ int pt_train_ln_fwd(const float* x, const float* res, const float* gamma, const 
                     void* stream);
 int pt_train_ln_bwd(const float* dy, const float* x, const float* res, const float* stats, const float* gamma, float* dx,
                     float* dgamma, float* dbeta, int rows, void* stream);
+/* The norms around a residual sum with its gate and scale, rows of `cols` (1 to 8192) values, dtype 0 fp32 | 1 bf16:
+ *   y = x + res_scale * gate[row / rows_per_clip] * u,  u = N(t) * post_w + post_b,  h = N(y) * pre_w + pre_b
+ * kind 0 LayerNorm, 1 RMSNorm.  x, t: row strides ldx, ldt; gate [rows / rows_per_clip][cols]; the rest contiguous; vectors fp32.  May
+ * be NULL: t (then y is x and not written), gate, res_scale (ones), post_w (u = t), post_b, pre_w (no h), pre_b.  stats [rows][4]
+ * (16-byte aligned, may be NULL) is what the backward call needs: mean and 1/std of t and of y.
+ * Backward: dy or dh may be NULL (zeros); any gradient but dx may be NULL.  ws: pt_train_gated_norm_workspace_bytes(rows, cols,
+ * rows_per_clip or 0 without a gate) bytes, 16-byte aligned.  Gradients are written, not added to, and do not depend on timing. */
+size_t pt_train_gated_norm_workspace_bytes(int64_t rows, int cols, int rows_per_clip);
+int pt_train_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* res_scale,
+                            const float* post_w, const float* post_b, const float* pre_w, const float* pre_b, void* y, void* h,
+                            float* stats, int64_t rows, int cols, int rows_per_clip, int kind, float eps, int dtype, void* stream);
+int pt_train_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* res_scale,
+                            const float* post_w, const float* post_b, const float* pre_w, const float* stats, const void* dy,
+                            const void* dh, void* dx, void* dt, void* dgate, float* dres_scale, float* dpost_w, float* dpost_b,
+                            float* dpre_w, float* dpre_b, void* ws, size_t ws_bytes, int64_t rows, int cols, int rows_per_clip,
+                            int kind, int dtype, void* stream);
 /* StylizationBlock_V3 'sb' modulation (PTransformer.py:134-139): h = SiLU(y*(1+scale[c]) + shift[c]), table [n_classes][1024] */
 int pt_train_modsilu_fwd(const float* y, const float* table, const int64_t* label, int n_label, int rows_per_clip, int n_classes,
                          float* h, int rows, void* stream);

@@ -69,6 +69,11 @@ def _proto(lib):
     lib.pt_train_colsum.argtypes = [vp, i, vp, i, i, i, vp, vp]
     lib.pt_train_ln_fwd.argtypes = [vp, vp, vp, vp, vp, vp, i, vp]
     lib.pt_train_ln_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i, vp]
+    i64 = C.c_int64
+    lib.pt_train_gated_norm_workspace_bytes.restype = sz
+    lib.pt_train_gated_norm_workspace_bytes.argtypes = [i64, i, i]
+    lib.pt_train_gated_norm_fwd.argtypes = [vp, i64, vp, i64] + [vp] * 9 + [i64, i, i, i, f, i, vp]
+    lib.pt_train_gated_norm_bwd.argtypes = [vp, i64, vp, i64] + [vp] * 17 + [sz, i64, i, i, i, i, vp]
     lib.pt_train_modsilu_fwd.argtypes = [vp, vp, vp, i, i, i, vp, i, vp]
     lib.pt_train_modsilu_bwd.argtypes = [vp, vp, vp, vp, i, i, i, vp, vp, i, vp]
     lib.pt_train_attention_fwd.argtypes = [vp, i, vp, i, vp, i, vp, i, i, i, i, i, f, u64, vp]
@@ -121,7 +126,8 @@ EXPORTS = [
     "pt_train_cross_entropy", "pt_train_bn_fwd", "pt_train_bn_bwd", "pt_train_act_bwd", "pt_train_gate_fwd",
     "pt_train_gate_bwd", "pt_train_embed_bwd", "pt_train_dropout", "pt_train_sumsq", "pt_train_clip_coef",
     "pt_train_adamw", "pt_train_add", "pt_train_grad_norm_workspace_bytes", "pt_train_grad_norm", "pt_train_adamw_multi",
-    "pt_train_moment_values", "pt_train_pq_ema", "pt_train_pq_ema_shared", "pt_train_vq_ema", "pt_train_vq_losses", "pt_train_masked_l1_losses", "pt_train_sqdiff", "pt_train_commit_bwd",
+    "pt_train_moment_values",
+    "pt_train_gated_norm_workspace_bytes", "pt_train_gated_norm_fwd", "pt_train_gated_norm_bwd", "pt_train_pq_ema", "pt_train_pq_ema_shared", "pt_train_vq_ema", "pt_train_vq_losses", "pt_train_masked_l1_losses", "pt_train_sqdiff", "pt_train_commit_bwd",
     "pt_set_option", "pt_get_option",
 ]
 

@@ -37,6 +37,9 @@ int launch_clip_coef(const float* sumsq, float max_norm, float* coef, float* nor
 int launch_add(const float* a, const float* b, float* out, size_t n, hipStream_t s);
 int launch_adamw_multi(void* const* p, const void* const* g, void* const* m, void* const* v, float* const* scales, const int64_t* n, int count, int dtype, const float* gscale, float lr, float beta1, float beta2, float eps, float wd, int step, const int* step_dev, float* dyn, unsigned seed, hipStream_t s);
 int launch_moment_values(const unsigned char* m, const unsigned char* v, const float* scales, int64_t n, float* m_out, float* v_out, hipStream_t s);
+size_t gated_norm_workspace(int rows, int cols, int clip);
+int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1, const float* b1, const float* w2, const float* b2, void* y, void* h, float* stats, int64_t rows, int cols, int clip, int kind, float eps, int dtype, hipStream_t s);
+int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1, const float* b1, const float* w2, const float* stats, const void* dy, const void* dh, void* dx, void* dt, void* dgate, float* da, float* dw1, float* db1, float* dw2, float* db2, void* ws, size_t ws_bytes, int64_t rows, int cols, int clip, int kind, int dtype, hipStream_t s);
 size_t grad_norm_workspace(const int64_t* n, int count);
 int launch_grad_norm(const void* const* g, const int64_t* n, const unsigned char* is_bf16, int count, float max_norm, float* norm, float* coef, void* ws, size_t ws_bytes, hipStream_t s);
 int launch_attention_bf16(const unsigned short* Q, int ldq, const unsigned short* K, int ldk, const unsigned short* V, int ldv, unsigned short* O, int ldo, int B, int Nq, int Nk, int H, hipStream_t s);
@@ -474,6 +477,23 @@ int pt_train_ln_fwd(const float* x, const float* res, const float* gamma, const 
 int pt_train_ln_bwd(const float* dy, const float* x, const float* res, const float* stats, const float* gamma, float* dx,
                     float* dgamma, float* dbeta, int rows, void* stream) {
   return launch_ln_bwd(dy, x, res, stats, gamma, dx, dgamma, dbeta, rows, (hipStream_t)stream);
+}
+size_t pt_train_gated_norm_workspace_bytes(int64_t rows, int cols, int rows_per_clip) {
+  return rows > 0x7FFFFFFF ? 0 : gated_norm_workspace((int)rows, cols, rows_per_clip);
+}
+int pt_train_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* res_scale,
+                            const float* post_w, const float* post_b, const float* pre_w, const float* pre_b, void* y, void* h,
+                            float* stats, int64_t rows, int cols, int rows_per_clip, int kind, float eps, int dtype, void* stream) {
+  return launch_gated_norm_fwd(x, ldx, t, ldt, gate, res_scale, post_w, post_b, pre_w, pre_b, y, h, stats, rows, cols, rows_per_clip,
+                               kind, eps, dtype, (hipStream_t)stream);
+}
+int pt_train_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* res_scale,
+                            const float* post_w, const float* post_b, const float* pre_w, const float* stats, const void* dy,
+                            const void* dh, void* dx, void* dt, void* dgate, float* dres_scale, float* dpost_w, float* dpost_b,
+                            float* dpre_w, float* dpre_b, void* ws, size_t ws_bytes, int64_t rows, int cols, int rows_per_clip,
+                            int kind, int dtype, void* stream) {
+  return launch_gated_norm_bwd(x, ldx, t, ldt, gate, res_scale, post_w, post_b, pre_w, stats, dy, dh, dx, dt, dgate, dres_scale, dpost_w,
+                               dpost_b, dpre_w, dpre_b, ws, ws_bytes, rows, cols, rows_per_clip, kind, dtype, (hipStream_t)stream);
 }
 int pt_train_modsilu_fwd(const float* y, const float* table, const int64_t* label, int n_label, int rows_per_clip, int n_classes,
                          float* h, int rows, void* stream) {

@@ -1,0 +1,573 @@
+// Norm of a block's output, gate, residual scale, residual sum and the norm in front of the next block, in one pass:
+//
+//   u = N(t) w1 + b1,   y = x + a g u,   h = N(y) w2 + b2          N: LayerNorm or RMSNorm over the row
+//
+// with one gate row g per clip (rows_per_clip rows share it) and one residual scale a per column.  Left out parts: t (y = x), g, a
+// (ones), w1 (u = t), w2 (no h).  Backward, with dn = dh w2 and "bar" the mean over the row (its first term only for LayerNorm):
+//
+//   D  = dy + r_y (dn - bar(dn) - y^ bar(dn y^))                    dx = D
+//   dm = D a g w1,  dt = r_t (dm - bar(dm) - t^ bar(dm t^))
+//   dw2 = sum dh y^, db2 = sum dh, dw1 = a sum g D t^, db1 = a sum g D, da = w1 sum g D t^ + b1 sum g D, dg = sum over the clip of D a u
+//
+// Bound by HBM: forward 2 rows in and 2 out, backward 4 in and 2 out.  y and the statistics' arguments are recomputed from x and t
+// (the same bytes as reading a stored y, and exact where y is held in bf16); only 4 floats a row are kept from the forward pass.
+//
+// A row is held by WPR waves, 8 values a lane; a worker (these waves) walks a run of rows, so the column vectors stay in registers
+// and the column sums of the backward pass are register adds.  A worker's rows lie in one clip, or are whole clips, so the gate's
+// gradient is a register sum too, stored once per clip (or once per worker, and added up in order by the second kernel with the
+// other column sums).  No atomics: the same inputs give the same bits.
+#include <algorithm>
+#include <cstdint>
+
+#include "pt_common.h"
+
+namespace pt {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int PER = 8;                 // values of a row per lane
+
+struct GatedArgs {
+  const void* x; const void* t; const void* gate;
+  const float* a; const float* w1; const float* b1; const float* w2; const float* b2;
+  const void* dy; const void* dh;
+  void* y; void* h; float* stats;      // stats [rows][4]: mean t, 1/std t, mean y, 1/std y
+  void* dx; void* dt; void* dgate;
+  float* part;                         // [blocks][4][cols]: sum g D t^ | sum g D | sum dh y^ | sum dh
+  float* gpart;                        // [workers][cols]: a worker's share of its clip's gate gradient, or null (whole clips)
+  size_t ldx, ldt;
+  int rows, cols, clip;                // rows per clip (of the gate)
+  int run, spc;                        // rows per worker; workers per clip, or 0: a worker takes run / clip whole clips
+  float eps;
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_sum(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+// sum over the wave, the same in every lane, without the LDS crossbar
+__device__ __forceinline__ float wave_sum(float v) {
+  v = dpp_sum<0xB1>(v);        // quad_perm [1,0,3,2]
+  v = dpp_sum<0x4E>(v);        // quad_perm [2,3,0,1]
+  v = dpp_sum<0x141>(v);       // row_half_mirror
+  v = dpp_sum<0x140>(v);       // row_mirror
+  return row_lanes_sum(v);
+}
+
+template <int WPR>
+struct RowSum {
+  float* slot;                         // LDS [2][RPB][WPR][2]
+  int flip = 0;
+  __device__ __forceinline__ void operator()(float& a, float& b) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (WPR > 1) {
+      // two slots in turn: a slot is written again only behind the barrier of the other one, which every reader has passed
+      float* s = slot + flip * 2 * (blockDim.x >> 6);
+      flip ^= 1;
+      const int wave = threadIdx.x >> 6, first = wave / WPR * WPR;
+      if ((threadIdx.x & 63) == 0) { s[2 * wave] = a; s[2 * wave + 1] = b; }
+      __syncthreads();
+      a = b = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) { a += s[2 * (first + w)]; b += s[2 * (first + w) + 1]; }
+    }
+  }
+};
+
+// columns of a lane: chunks of 16 bytes, neighbouring lanes next to each other
+template <typename T, int WPR>
+__device__ __forceinline__ int column(int i) {
+  constexpr int V = 16 / sizeof(T), L = 64 * WPR;
+  const int lane = threadIdx.x % L;
+  return (i / V * L + lane) * V + i % V;
+}
+
+__device__ __forceinline__ unsigned short to_bf16(float x) { return __builtin_bit_cast(unsigned short, (__bf16)x); }
+
+template <typename T, int WPR, bool VEC>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, int cols, float (&v)[PER]) {
+  constexpr int V = 16 / sizeof(T);
+#pragma unroll
+  for (int c = 0; c < PER / V; ++c) {
+    const int c0 = column<T, WPR>(c * V);
+    if constexpr (VEC) {
+      if constexpr (V == 4) {
+        f32x4 q = {0.f, 0.f, 0.f, 0.f};
+        if (c0 < cols) q = *reinterpret_cast<const f32x4*>(p + c0);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[c * V + j] = q[j];
+      } else {
+        u16x8 q = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (c0 < cols) q = *reinterpret_cast<const u16x8*>(p + c0);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[c * V + j] = __uint_as_float((unsigned)q[j] << 16);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if constexpr (V == 4) v[c * V + j] = c0 + j < cols ? p[c0 + j] : 0.f;
+        else v[c * V + j] = c0 + j < cols ? __uint_as_float((unsigned)p[c0 + j] << 16) : 0.f;
+      }
+    }
+  }
+}
+template <typename T, int WPR, bool VEC>
+__device__ __forceinline__ void store_row(T* __restrict__ p, int cols, const float (&v)[PER]) {
+  constexpr int V = 16 / sizeof(T);
+#pragma unroll
+  for (int c = 0; c < PER / V; ++c) {
+    const int c0 = column<T, WPR>(c * V);
+    if constexpr (VEC) {
+      if (c0 < cols) {
+        if constexpr (V == 4) {
+          const f32x4 q = {v[c * V], v[c * V + 1], v[c * V + 2], v[c * V + 3]};
+          *reinterpret_cast<f32x4*>(p + c0) = q;
+        } else {
+          u16x8 q;
+#pragma unroll
+          for (int j = 0; j < V; ++j) q[j] = to_bf16(v[c * V + j]);
+          *reinterpret_cast<u16x8*>(p + c0) = q;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c0 + j < cols) {
+          if constexpr (V == 4) p[c0 + j] = v[c * V + j];
+          else p[c0 + j] = to_bf16(v[c * V + j]);
+        }
+    }
+  }
+}
+// a column vector in fp32 at the columns of T's chunks; `fill` where there is none
+template <typename T, int WPR>
+__device__ __forceinline__ void load_cols(const float* __restrict__ p, int cols, float fill, float (&v)[PER]) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int c = column<T, WPR>(i);
+    v[i] = p ? (c < cols ? p[c] : 0.f) : fill;
+  }
+}
+
+// rows [r0, r1) of a worker; workers behind the last one get none
+__device__ __forceinline__ void worker_rows(const GatedArgs& g, int worker, int& r0, int& r1) {
+  int64_t begin = (int64_t)worker * g.run, end = begin + g.run, most = g.rows;
+  if (g.spc) {
+    const int clip = worker / g.spc, seg = worker - clip * g.spc;
+    begin = (int64_t)clip * g.clip + (int64_t)seg * g.run;
+    end = begin + g.run;
+    most = min(most, ((int64_t)clip + 1) * g.clip);
+  }
+  r0 = (int)min(begin, most);
+  r1 = (int)min(end, most);
+}
+
+// mean and 1/std of the values; what lies behind the last column is kept out of the sums
+template <typename T, int WPR, bool LAYER>
+__device__ __forceinline__ void row_stats(const float (&v)[PER], int cols, float inv_cols, float eps, RowSum<WPR>& sum, float& mean, float& rstd) {
+  mean = 0.f;
+  if constexpr (LAYER) {
+    float s = 0.f, z = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s += v[i];
+    sum(s, z);
+    mean = s * inv_cols;
+  }
+  float q = 0.f, z = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const float d = column<T, WPR>(i) < cols ? v[i] - mean : 0.f;
+    q += d * d;
+  }
+  sum(q, z);
+  rstd = 1.f / sqrtf(q * inv_cols + eps);
+}
+
+template <typename T, int WPR, bool LAYER, bool VEC>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kernel(const GatedArgs g) {
+  constexpr int L = 64 * WPR, THREADS = WPR > 4 ? L : 256, RPB = THREADS / L;
+  __shared__ float red[2 * 2 * (THREADS / 64)];
+  RowSum<WPR> sum{red};
+  int r0, r1;
+  worker_rows(g, blockIdx.x * RPB + threadIdx.x / L, r0, r1);
+  const int cols = g.cols;
+  const float inv_cols = 1.f / (float)cols;
+  const T* __restrict__ X = (const T*)g.x;
+  const T* __restrict__ Tt = (const T*)g.t;
+  float a[PER], w1[PER], b1[PER], w2[PER], b2[PER], gt[PER];
+  load_cols<T, WPR>(g.a, cols, 1.f, a);
+  load_cols<T, WPR>(g.w1, cols, 1.f, w1);
+  load_cols<T, WPR>(g.b1, cols, 0.f, b1);
+  load_cols<T, WPR>(g.w2, cols, 1.f, w2);
+  load_cols<T, WPR>(g.b2, cols, 0.f, b2);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) gt[i] = a[i];
+  float nx[PER], nt[PER];
+  if (r0 < r1) {
+    load_row<T, WPR, VEC>(X + (size_t)r0 * g.ldx, cols, nx);
+    if (Tt) load_row<T, WPR, VEC>(Tt + (size_t)r0 * g.ldt, cols, nt);
+  }
+  int left = 0;                                          // rows left of the current clip
+  for (int k = 0; k < g.run; ++k) {                      // the same count for every worker of the block: barriers inside
+    const int row = r0 + k;
+    const bool on = row < r1;
+    float x[PER], t[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { x[i] = nx[i]; t[i] = nt[i]; }
+    if (row + 1 < r1) {
+      load_row<T, WPR, VEC>(X + (size_t)(row + 1) * g.ldx, cols, nx);
+      if (Tt) load_row<T, WPR, VEC>(Tt + (size_t)(row + 1) * g.ldt, cols, nt);
+    }
+    if (g.gate && on && left == 0) {
+      const int clip = row / g.clip;
+      left = (clip + 1) * g.clip - row;
+      load_row<T, WPR, VEC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) gt[i] *= a[i];
+    }
+    --left;
+    if (!on) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) { x[i] = 0.f; t[i] = 0.f; }
+    }
+    float mt = 0.f, rt = 1.f, my = 0.f, ry = 1.f;
+    if (Tt) {
+      if (g.w1) {
+        row_stats<T, WPR, LAYER>(t, cols, inv_cols, g.eps, sum, mt, rt);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) t[i] = (t[i] - mt) * rt * w1[i] + b1[i];
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] += gt[i] * t[i];
+      if (on) store_row<T, WPR, VEC>((T*)g.y + (size_t)row * cols, cols, x);
+    }
+    if (g.w2) {
+      // from the sum in fp32, not from the stored y: one rounding less in h
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = column<T, WPR>(i) < cols ? x[i] : 0.f;
+      row_stats<T, WPR, LAYER>(x, cols, inv_cols, g.eps, sum, my, ry);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = (x[i] - my) * ry * w2[i] + b2[i];
+      if (on) store_row<T, WPR, VEC>((T*)g.h + (size_t)row * cols, cols, x);
+    }
+    if (g.stats && on && threadIdx.x % L == 0) {
+      const f32x4 s = {mt, rt, my, ry};
+      *reinterpret_cast<f32x4*>(g.stats + (size_t)row * 4) = s;
+    }
+  }
+}
+
+template <typename T, int WPR, bool LAYER, bool VEC>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_bwd_kernel(const GatedArgs g) {
+  constexpr int L = 64 * WPR, THREADS = WPR > 4 ? L : 256, RPB = THREADS / L;
+  __shared__ float red[2 * 2 * (THREADS / 64)];
+  __shared__ float join[RPB > 1 ? RPB * L * PER : 1];
+  RowSum<WPR> sum{red};
+  const int worker = blockIdx.x * RPB + threadIdx.x / L;
+  int r0, r1;
+  worker_rows(g, worker, r0, r1);
+  const int cols = g.cols;
+  const float inv_cols = 1.f / (float)cols;
+  const T* __restrict__ X = (const T*)g.x;
+  const T* __restrict__ Tt = (const T*)g.t;
+  const T* __restrict__ DY = (const T*)g.dy;
+  const T* __restrict__ DH = (const T*)g.dh;
+  // 16 waves leave 128 registers a lane: the column vectors are then read for every row (they stay in the caches) and the
+  // next row's loads do not run ahead; with both kept the kernel would spill 150 registers
+  constexpr bool WIDE = WPR == 16;
+  float a[PER], w1[PER], b1[PER], w2[PER], gt[PER];
+  auto columns = [&]() {
+    load_cols<T, WPR>(g.a, cols, 1.f, a);
+    load_cols<T, WPR>(g.w1, cols, 1.f, w1);
+    load_cols<T, WPR>(g.b1, cols, 0.f, b1);
+    load_cols<T, WPR>(g.w2, cols, 1.f, w2);
+  };
+  if constexpr (!WIDE) columns();
+  float aw[PER], ab[PER], bw[PER], bb[PER], dg[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) { gt[i] = 1.f; aw[i] = ab[i] = bw[i] = bb[i] = dg[i] = 0.f; }
+  float nx[PER], nt[PER], ny[PER], nh[PER];
+  f32x4 ns = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < PER; ++i) nx[i] = nt[i] = ny[i] = nh[i] = 0.f;
+  auto fetch = [&](int row) {
+    load_row<T, WPR, VEC>(X + (size_t)row * g.ldx, cols, nx);
+    if (Tt) load_row<T, WPR, VEC>(Tt + (size_t)row * g.ldt, cols, nt);
+    if (DY) load_row<T, WPR, VEC>(DY + (size_t)row * cols, cols, ny);
+    if (DH) load_row<T, WPR, VEC>(DH + (size_t)row * cols, cols, nh);
+    ns = *reinterpret_cast<const f32x4*>(g.stats + (size_t)row * 4);
+  };
+  if (!WIDE && r0 < r1) fetch(r0);
+  int left = 0, clip = 0;
+  for (int k = 0; k < g.run; ++k) {
+    const int row = r0 + k;
+    const bool on = row < r1;
+    if constexpr (WIDE) {
+      asm volatile("" ::: "memory");                       // keeps the reads in the loop
+      columns();
+      if (on) fetch(row);
+    }
+    float x[PER], t[PER], dy[PER], dh[PER];
+    const f32x4 st = ns;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { x[i] = nx[i]; t[i] = nt[i]; dy[i] = ny[i]; dh[i] = nh[i]; }
+    if (!WIDE && row + 1 < r1) fetch(row + 1);
+    if (!on) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = t[i] = dy[i] = dh[i] = 0.f;
+    }
+    if (g.gate && on && left == 0) {
+      clip = row / g.clip;
+      left = (clip + 1) * g.clip - row;
+      load_row<T, WPR, VEC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
+    }
+    --left;
+    float tn[PER], u[PER], yn[PER], dn[PER], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      tn[i] = g.w1 ? (t[i] - st[0]) * st[1] : t[i];
+      u[i] = tn[i] * w1[i] + b1[i];
+      const float y = x[i] + gt[i] * a[i] * u[i];
+      yn[i] = (y - st[2]) * st[3];
+      dn[i] = column<T, WPR>(i) < cols ? dh[i] * w2[i] : 0.f;
+      s1 += dn[i];
+      s2 += dn[i] * yn[i];
+    }
+    if (DH) {
+      sum(s1, s2);
+      const float m1 = LAYER ? s1 * inv_cols : 0.f, m2 = s2 * inv_cols;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        bw[i] += dh[i] * yn[i];
+        bb[i] += dh[i];
+        dy[i] += st[3] * (dn[i] - m1 - yn[i] * m2);
+      }
+    }
+    if (on) store_row<T, WPR, VEC>((T*)g.dx + (size_t)row * cols, cols, dy);
+    if (Tt) {
+      float s3 = 0.f, s4 = 0.f, dm[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float d = on && column<T, WPR>(i) < cols ? dy[i] : 0.f;
+        const float gd = gt[i] * d;
+        aw[i] += gd * tn[i];
+        ab[i] += gd;
+        dg[i] += d * a[i] * u[i];
+        dm[i] = gd * a[i] * w1[i];
+        s3 += dm[i];
+        s4 += dm[i] * tn[i];
+      }
+      if (g.w1) {
+        sum(s3, s4);
+        const float m3 = LAYER ? s3 * inv_cols : 0.f, m4 = s4 * inv_cols;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) dm[i] = st[1] * (dm[i] - m3 - tn[i] * m4);
+      }
+      if (on && g.dt) store_row<T, WPR, VEC>((T*)g.dt + (size_t)row * cols, cols, dm);
+    }
+    if (g.dgate && on && (left == 0 || row + 1 == r1)) {
+      if (g.gpart) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) if (column<T, WPR>(i) < cols) g.gpart[(size_t)worker * cols + column<T, WPR>(i)] = dg[i];
+      } else {
+        store_row<T, WPR, VEC>((T*)g.dgate + (size_t)clip * cols, cols, dg);
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) dg[i] = 0.f;
+    }
+  }
+  // this block's column sums
+  float* __restrict__ out = g.part + (size_t)blockIdx.x * 4 * cols;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = q == 0 ? aw[i] : q == 1 ? ab[i] : q == 2 ? bw[i] : bb[i];
+    if constexpr (RPB > 1) {
+      const int lane = threadIdx.x % L, who = threadIdx.x / L;
+      __syncthreads();
+      if (who)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) join[(who * PER + i) * L + lane] = v[i];
+      __syncthreads();
+      if (!who)
+#pragma unroll
+        for (int w = 1; w < RPB; ++w)
+#pragma unroll
+          for (int i = 0; i < PER; ++i) v[i] += join[(w * PER + i) * L + lane];
+      if (who) continue;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) if (column<T, WPR>(i) < cols) out[(size_t)q * cols + column<T, WPR>(i)] = v[i];
+  }
+}
+
+// Adds the blocks' column sums (grid part 1: 64 columns and one of the two norms per block, 16 waves share the blocks) and the
+// workers' shares of each clip's gate gradient (part 2: 256 columns of one clip per block).
+struct GatedFinish {
+  const float* part; const float* gpart;
+  const float* a; const float* w1; const float* b1;
+  float* da; float* dw1; float* db1; float* dw2; float* db2;
+  void* dgate;
+  int blocks, cols, spc;
+  int col_blocks, n_first;             // part 1: 2 * col_blocks blocks
+};
+template <typename T>
+__global__ __launch_bounds__(1024) void gated_norm_finish_kernel(const GatedFinish f) {
+  if ((int)blockIdx.x < f.n_first) {
+    const int which = blockIdx.x / f.col_blocks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = (blockIdx.x - which * f.col_blocks) * 64 + lane;
+    float p = 0.f, q = 0.f;
+    if (c < f.cols) {
+      const float* s = f.part + (size_t)which * 2 * f.cols + c;
+#pragma unroll 8
+      for (int b = wave; b < f.blocks; b += 16) {
+        p += s[(size_t)b * 4 * f.cols];
+        q += s[(size_t)b * 4 * f.cols + f.cols];
+      }
+    }
+    __shared__ float red[2][16][64];
+    red[0][wave][lane] = p;
+    red[1][wave][lane] = q;
+    __syncthreads();
+    if (wave || c >= f.cols) return;
+    p = q = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) { p += red[0][w][lane]; q += red[1][w][lane]; }
+    if (which) {
+      if (f.dw2) f.dw2[c] = p;
+      if (f.db2) f.db2[c] = q;
+    } else {
+      const float a = f.a ? f.a[c] : 1.f, w = f.w1 ? f.w1[c] : 1.f, b = f.b1 ? f.b1[c] : 0.f;
+      if (f.dw1) f.dw1[c] = a * p;
+      if (f.db1) f.db1[c] = a * q;
+      if (f.da) f.da[c] = w * p + b * q;
+    }
+    return;
+  }
+  const int k = blockIdx.x - f.n_first, per = (f.cols + 1023) / 1024, clip = k / per, c = (k - clip * per) * 1024 + threadIdx.x;
+  if (c >= f.cols) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int w = 0; w < f.spc; ++w) s += f.gpart[((size_t)clip * f.spc + w) * f.cols + c];
+  if constexpr (sizeof(T) == 4) ((float*)f.dgate)[(size_t)clip * f.cols + c] = s;
+  else ((unsigned short*)f.dgate)[(size_t)clip * f.cols + c] = to_bf16(s);
+}
+
+// ---------------------------------------------------------------------------
+struct GatedPlan { int wpr, rpb, run, spc, workers, blocks; };
+// Two blocks per CU, each with rows of its own to walk: enough loads in flight (a wave holds two rows' worth), and few partial sums.
+static GatedPlan gated_plan(int rows, int cols, int clip, bool gate) {
+  GatedPlan p;
+  p.wpr = cols <= 512 ? 1 : cols <= 1024 ? 2 : cols <= 2048 ? 4 : cols <= 4096 ? 8 : 16;
+  p.rpb = p.wpr >= 4 ? 1 : 4 / p.wpr;
+  const int64_t want = (int64_t)device_cus() * 2 * p.rpb;
+  const int64_t run = std::max<int64_t>(1, (rows + want - 1) / want);
+  p.spc = 0;
+  if (!gate) {
+    p.run = (int)run;
+    p.workers = (int)((rows + run - 1) / run);
+  } else if (clip <= run) {
+    p.run = (int)(run / clip * clip);
+    p.workers = (int)(((int64_t)rows + p.run - 1) / p.run);
+  } else {
+    p.spc = (int)((clip + run - 1) / run);
+    p.run = (clip + p.spc - 1) / p.spc;                    // at most `run`, and none of the spc workers is without rows
+    p.workers = (rows + clip - 1) / clip * p.spc;
+  }
+  p.blocks = (p.workers + p.rpb - 1) / p.rpb;
+  return p;
+}
+
+size_t gated_norm_workspace(int rows, int cols, int clip) {
+  if (rows < 1 || cols < 1 || cols > 8192 || clip < 0) return 0;
+  const GatedPlan p = gated_plan(rows, cols, clip ? clip : rows, clip > 0);
+  return ((size_t)p.blocks * 4 + (p.spc ? p.workers : 0)) * cols * sizeof(float);
+}
+
+template <typename T, int WPR, bool LAYER, bool VEC>
+static int run_gated(const GatedArgs& g, const GatedPlan& p, bool back, hipStream_t s) {
+  constexpr int threads = WPR > 4 ? 64 * WPR : 256;
+  if (back) PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, LAYER, VEC>), dim3(p.blocks), dim3(threads), 0, s, g);
+  else PT_LAUNCH((gated_norm_fwd_kernel<T, WPR, LAYER, VEC>), dim3(p.blocks), dim3(threads), 0, s, g);
+  return 0;
+}
+template <typename T, int WPR>
+static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, bool vec, bool back, hipStream_t s) {
+  return layer ? (vec ? run_gated<T, WPR, true, true>(g, p, back, s) : run_gated<T, WPR, true, false>(g, p, back, s))
+               : (vec ? run_gated<T, WPR, false, true>(g, p, back, s) : run_gated<T, WPR, false, false>(g, p, back, s));
+}
+template <typename T>
+static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, bool vec, bool back, hipStream_t s) {
+  switch (p.wpr) {
+    case 1: return run_gated<T, 1>(g, p, layer, vec, back, s);
+    case 2: return run_gated<T, 2>(g, p, layer, vec, back, s);
+    case 4: return run_gated<T, 4>(g, p, layer, vec, back, s);
+    case 8: return run_gated<T, 8>(g, p, layer, vec, back, s);
+    default: return run_gated<T, 16>(g, p, layer, vec, back, s);
+  }
+}
+
+static int check_gated(const char* who, const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, int64_t rows, int cols, int clip,
+                       int kind, int dtype) {
+  PT_CHECK(x && rows >= 1 && rows <= 0x7FFFFFFF && cols >= 1 && cols <= 8192, "%s: %lld rows of %d columns (1 to 8192)", who, (long long)rows, cols);
+  PT_CHECK(ldx >= cols && (!t || ldt >= cols), "%s: row strides %lld and %lld for %d columns", who, (long long)ldx, (long long)ldt, cols);
+  PT_CHECK(!gate || (t && clip >= 1 && rows % clip == 0), "%s: %lld rows in clips of %d", who, (long long)rows, clip);
+  PT_CHECK((kind == 0 || kind == 1) && (dtype == 0 || dtype == 1), "%s: kind %d, dtype %d", who, kind, dtype);
+  return 0;
+}
+static bool gated_vec(const GatedArgs& g, int dtype) {
+  const size_t v = dtype ? 8 : 4;
+  const uintptr_t p = (uintptr_t)g.x | (uintptr_t)g.t | (uintptr_t)g.gate | (uintptr_t)g.dy | (uintptr_t)g.dh | (uintptr_t)g.y | (uintptr_t)g.h |
+                      (uintptr_t)g.dx | (uintptr_t)g.dt | (uintptr_t)g.dgate;
+  return !(p & 15) && g.cols % v == 0 && g.ldx % v == 0 && (!g.t || g.ldt % v == 0);
+}
+
+int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1,
+                          const float* b1, const float* w2, const float* b2, void* y, void* h, float* stats, int64_t rows, int cols, int clip,
+                          int kind, float eps, int dtype, hipStream_t s) {
+  if (check_gated("gated_norm_fwd", x, ldx, t, ldt, gate, rows, cols, clip, kind, dtype)) return 1;
+  PT_CHECK((t || w2) && (!t || y) && (!w2 || h) && ((uintptr_t)stats & 15) == 0, "gated_norm_fwd: null or misaligned argument");
+  GatedArgs g = {};
+  g.x = x; g.t = t; g.gate = gate; g.a = a; g.w1 = w1; g.b1 = b1; g.w2 = w2; g.b2 = b2; g.y = y; g.h = h; g.stats = stats;
+  g.ldx = (size_t)ldx; g.ldt = (size_t)ldt; g.rows = (int)rows; g.cols = cols; g.clip = gate ? clip : (int)rows; g.eps = eps;
+  const GatedPlan p = gated_plan(g.rows, cols, g.clip, gate != nullptr);
+  g.run = p.run; g.spc = p.spc;
+  const bool vec = gated_vec(g, dtype);
+  return dtype ? run_gated<unsigned short>(g, p, kind == 0, vec, false, s) : run_gated<float>(g, p, kind == 0, vec, false, s);
+}
+
+int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1,
+                          const float* b1, const float* w2, const float* stats, const void* dy, const void* dh, void* dx, void* dt,
+                          void* dgate, float* da, float* dw1, float* db1, float* dw2, float* db2, void* ws, size_t ws_bytes, int64_t rows,
+                          int cols, int clip, int kind, int dtype, hipStream_t s) {
+  if (check_gated("gated_norm_bwd", x, ldx, t, ldt, gate, rows, cols, clip, kind, dtype)) return 1;
+  PT_CHECK(stats && dx && (dy || dh) && (!dh || w2) && (!dgate || gate) && (!dt || t), "gated_norm_bwd: null argument");
+  PT_CHECK(ws && ws_bytes >= gated_norm_workspace((int)rows, cols, gate ? clip : 0) && (((uintptr_t)ws | (uintptr_t)stats) & 15) == 0,
+           "gated_norm_bwd: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, gated_norm_workspace((int)rows, cols, gate ? clip : 0));
+  GatedArgs g = {};
+  g.x = x; g.t = t; g.gate = gate; g.a = a; g.w1 = w1; g.b1 = b1; g.w2 = w2; g.dy = dy; g.dh = dh; g.stats = const_cast<float*>(stats);
+  g.dx = dx; g.dt = dt; g.dgate = dgate;
+  g.ldx = (size_t)ldx; g.ldt = (size_t)ldt; g.rows = (int)rows; g.cols = cols; g.clip = gate ? clip : (int)rows;
+  const GatedPlan p = gated_plan(g.rows, cols, g.clip, gate != nullptr);
+  g.run = p.run; g.spc = p.spc;
+  g.part = (float*)ws;
+  g.gpart = p.spc && dgate ? g.part + (size_t)p.blocks * 4 * cols : nullptr;
+  const bool vec = gated_vec(g, dtype);
+  if (dtype ? run_gated<unsigned short>(g, p, kind == 0, vec, true, s) : run_gated<float>(g, p, kind == 0, vec, true, s)) return 1;
+  GatedFinish f = {};
+  f.part = g.part; f.gpart = g.gpart; f.a = a; f.w1 = w1; f.b1 = b1;
+  f.da = t ? da : nullptr; f.dw1 = t ? dw1 : nullptr; f.db1 = t ? db1 : nullptr; f.dw2 = dw2; f.db2 = db2;
+  f.dgate = dgate; f.blocks = p.blocks; f.cols = cols; f.spc = p.spc;
+  f.col_blocks = (cols + 63) / 64;
+  f.n_first = 2 * f.col_blocks;
+  const int64_t gate_blocks = g.gpart ? (int64_t)(rows / clip) * ((cols + 1023) / 1024) : 0;
+  PT_CHECK(f.n_first + gate_blocks < 0x7FFFFFFF, "gated_norm_bwd: too many clips");
+  if (dtype) PT_LAUNCH(gated_norm_finish_kernel<unsigned short>, dim3((unsigned)(f.n_first + gate_blocks)), dim3(1024), 0, s, f);
+  else PT_LAUNCH(gated_norm_finish_kernel<float>, dim3((unsigned)(f.n_first + gate_blocks)), dim3(1024), 0, s, f);
+  return 0;
+}
+
+}  // namespace pt

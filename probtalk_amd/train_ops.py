@@ -171,6 +171,96 @@ def layer_norm(x, gamma, beta, res=None):
     return LayerNormRes.apply(x, res, gamma, beta)
 
 
+def _row_stride(v):
+    return 0 if v is None else v.stride(0) if v.shape[0] > 1 else v.shape[1]
+
+
+class GatedNorm(torch.autograd.Function):
+    """y = x + res_scale * gate * N(t; post), h = N(y; pre) (see gated_norm)."""
+
+    @staticmethod
+    def forward(ctx, x, t, gate, res_scale, post_w, post_b, pre_w, pre_b, clip, kind, eps, grad):
+        rows, cols = x.shape
+        bf = int(x.dtype is torch.bfloat16)
+        y = None if t is None else torch.empty(rows, cols, device=x.device, dtype=x.dtype)
+        h = None if pre_w is None else torch.empty(rows, cols, device=x.device, dtype=x.dtype)
+        stats = torch.empty(rows, 4, device=x.device, dtype=torch.float32) if grad else None
+        with _on(x.device):
+            check(_lib.lib().pt_train_gated_norm_fwd(ptr(x), _row_stride(x), ptr(t), _row_stride(t), ptr(gate), ptr(res_scale),
+                                                     ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(y), ptr(h), ptr(stats), rows, cols,
+                                                     clip, kind, eps, bf, stream()))
+        if grad:
+            ctx.save_for_backward(x, t, gate, res_scale, post_w, post_b, pre_w, stats)
+            ctx.meta = (clip, kind, bf)
+            ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    def backward(ctx, dy, dh):
+        x, t, gate, res_scale, post_w, post_b, pre_w, stats = ctx.saved_tensors
+        clip, kind, bf = ctx.meta
+        if dy is None and dh is None:
+            return (None,) * 12
+        rows, cols = x.shape
+        need = ctx.needs_input_grad
+        dy, dh = (None if d is None else d.contiguous() for d in (dy, dh))
+        new = lambda like: torch.empty(like.shape, device=x.device, dtype=like.dtype)  # noqa: E731
+        vec = lambda i: torch.empty(cols, device=x.device, dtype=torch.float32) if need[i] else None  # noqa: E731
+        dx = new(x)
+        dt = new(t) if need[1] else None
+        dgate = new(gate) if need[2] else None
+        da, dw1, db1, dw2, db2 = vec(3), vec(4), vec(5), vec(6), vec(7)
+        L = _lib.lib()
+        with _on(x.device):
+            ws = torch.empty(int(L.pt_train_gated_norm_workspace_bytes(rows, cols, clip if gate is not None else 0)), dtype=torch.uint8, device=x.device)
+            check(L.pt_train_gated_norm_bwd(ptr(x), _row_stride(x), ptr(t), _row_stride(t), ptr(gate), ptr(res_scale), ptr(post_w),
+                                            ptr(post_b), ptr(pre_w), ptr(stats), ptr(dy), ptr(dh), ptr(dx), ptr(dt), ptr(dgate), ptr(da), ptr(dw1),
+                                            ptr(db1), ptr(dw2), ptr(db2), ptr(ws), ws.numel(), rows, cols, clip, kind, bf, stream()))
+        return dx, dt, dgate, da, dw1, db1, dw2, db2, None, None, None, None
+
+
+def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, rows_per_clip=None,
+               kind="layer", eps=1e-5):
+    """The norm of a block's output, its gate and residual scale, the residual sum and the norm in front of the next block:
+
+        y = x + res_scale * gate * u,   u = N(t) * post_weight + post_bias,   h = N(y) * pre_weight + pre_bias      -> (y, h)
+
+    x, t: rows (R, C) of fp32 or bf16, 1 <= C <= 8192, with neighbouring columns.  gate (R / rows_per_clip, C) of x's type: a row
+    for every rows_per_clip rows (by default as many as it has rows for).  Vectors of C values in fp32.  kind: 'layer' (mean and
+    variance) or 'rms'.  Left out: t (y is x itself), gate, res_scale, post_weight (u = t), pre_weight (h is None).  Statistics and
+    sums are fp32; h is taken from y before it is rounded to bf16.  To capture the backward pass into a HIP graph, make the leaves
+    inside the capture (x.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
+    if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16) or not 1 <= x.shape[1] <= 8192:
+        raise RuntimeError(f"gated_norm: rows (R, C) of fp32 or bf16 on the GPU with C up to 8192, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    if kind not in ("layer", "rms"):
+        raise ValueError(f"gated_norm: kind must be 'layer' or 'rms', got {kind!r}")
+    rows, cols = x.shape
+    if t is None and (gate is not None or res_scale is not None or post_weight is not None or pre_weight is None):
+        raise RuntimeError("gated_norm: without t there is nothing to gate, scale or norm but x: pass pre_weight alone")
+    if (post_bias is not None and post_weight is None) or (pre_bias is not None and pre_weight is None):
+        raise RuntimeError("gated_norm: a bias comes with its weight")
+    for name, v, shape, dtype in (("t", t, (rows, cols), x.dtype), ("res_scale", res_scale, (cols,), torch.float32),
+                                  ("post_weight", post_weight, (cols,), torch.float32), ("post_bias", post_bias, (cols,), torch.float32),
+                                  ("pre_weight", pre_weight, (cols,), torch.float32), ("pre_bias", pre_bias, (cols,), torch.float32)):
+        if v is not None and (tuple(v.shape) != shape or v.dtype is not dtype or v.device != x.device):
+            raise RuntimeError(f"gated_norm: {name} must be {shape} {dtype} on {x.device}, got {tuple(v.shape)} {v.dtype} on {v.device}")
+    clip = max(rows, 1)
+    if gate is not None:
+        if gate.dim() != 2 or gate.shape[1] != cols or gate.dtype is not x.dtype or gate.device != x.device:
+            raise RuntimeError(f"gated_norm: gate must be (clips, {cols}) {x.dtype} on {x.device}, got {tuple(gate.shape)} {gate.dtype} on {gate.device}")
+        clip = int(rows_per_clip) if rows_per_clip is not None else rows // max(gate.shape[0], 1)
+        if clip < 1 or gate.shape[0] * clip != rows:
+            raise RuntimeError(f"gated_norm: {rows} rows are not {gate.shape[0]} clips of {clip}")
+    if rows == 0:
+        raise RuntimeError("gated_norm: no rows")
+    near = lambda v: v if v is None or (v.stride(1) == 1 and v.stride(0) >= cols) else v.contiguous()  # noqa: E731
+    flat = lambda v: None if v is None else v.contiguous()  # noqa: E731
+    given = [near(x), near(t), flat(gate), flat(res_scale), flat(post_weight), flat(post_bias), flat(pre_weight), flat(pre_bias)]
+    grad = torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in given)
+    y, h = GatedNorm.apply(*given, clip, 0 if kind == "layer" else 1, float(eps), grad)
+    return (x if t is None else y), h
+
+
 class ModSiLU(torch.autograd.Function):
     """h = SiLU(y * (1 + scale[c]) + shift[c]) with table (n_classes, 1024) = scale | shift (PTransformer.py:134-139)."""
 

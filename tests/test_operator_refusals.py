@@ -36,3 +36,26 @@ def test_c_entries_of_the_lists():
     refused(L.pt_train_adamw_multi(p, p, p, p, None, n, 2, 0, *h, 0, None, None, 0, None), "step")
     refused(L.pt_train_adamw_multi(p, p, p, p, None, n, 2, 0, *h, 0, out, None, 0, None), "scratch")
     refused(L.pt_train_moment_values(None, out, out, 4, out, out, None), "bad argument")
+
+
+def test_gated_norm_refuses():
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        T.gated_norm(torch.zeros(2, 4), pre_weight=torch.ones(4))
+    L, p, odd, n = _lib.lib(), C.c_void_p(256), C.c_void_p(264), None
+    fwd = lambda *a: L.pt_train_gated_norm_fwd(*a, None)  # noqa: E731
+    refused(fwd(n, 4, p, 4, n, n, n, n, p, n, p, p, n, 2, 4, 2, 0, 1e-5, 0), "rows")
+    refused(fwd(p, 4, p, 4, n, n, n, n, p, n, p, p, n, 0, 4, 2, 0, 1e-5, 0), "rows")
+    refused(fwd(p, 9000, p, 9000, n, n, n, n, p, n, p, p, n, 2, 9000, 2, 0, 1e-5, 0), "columns")
+    refused(fwd(p, 3, p, 4, n, n, n, n, p, n, p, p, n, 2, 4, 2, 0, 1e-5, 0), "stride")
+    refused(fwd(p, 4, p, 4, p, n, n, n, p, n, p, p, n, 3, 4, 2, 0, 1e-5, 0), "clips")
+    refused(fwd(p, 4, p, 4, n, n, n, n, p, n, p, p, n, 2, 4, 2, 2, 1e-5, 0), "kind")
+    refused(fwd(p, 4, n, 0, n, n, n, n, n, n, n, n, n, 2, 4, 2, 0, 1e-5, 0), "null")
+    refused(fwd(p, 4, p, 4, n, n, n, n, p, n, n, p, n, 2, 4, 2, 0, 1e-5, 0), "null")
+    refused(fwd(p, 4, p, 4, n, n, n, n, p, n, p, p, odd, 2, 4, 2, 0, 1e-5, 0), "misaligned")
+    bwd = lambda st, dy, dh, dx, dgate, ws, size: L.pt_train_gated_norm_bwd(p, 4, p, 4, n, n, n, n, p, st, dy, dh, dx, p, dgate, n, n, n, n, n, ws, size, 2, 4, 2, 0, 0, None)  # noqa: E731
+    refused(bwd(n, p, p, p, n, p, 1 << 20), "null")
+    refused(bwd(p, n, n, p, n, p, 1 << 20), "null")
+    refused(bwd(p, p, p, n, n, p, 1 << 20), "null")
+    refused(bwd(p, p, p, p, p, p, 1 << 20), "null")           # a gate's gradient without a gate
+    refused(bwd(p, p, p, p, n, p, 0), "workspace")
+    refused(bwd(p, p, p, p, n, odd, 1 << 20), "workspace")
