@@ -186,6 +186,25 @@ int pt_attention_cl(const float* Q, int ldq, const float* K, int ldk, const floa
  * 544 keys and stream through it in 256-key chunks beyond (any Nk). */
 int pt_attention_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, void* O, int ldo, int B,
                       int Nq, int Nk, int H, void* stream);
+/* Attention over a window of keys and a few first ones.  q (B, Nq, H, D), k and v (B, Nk, Hk, D), dtype 0 fp32 | 1 bf16, D a multiple of 8
+ * up to 128, H a multiple of Hk (query head h uses key head h / (H / Hk)), Nk >= Nq.  strides: nine host values, of batch, row and head for
+ * q, k and v, in elements; neighbouring channels are neighbours in memory; addresses and strides are multiples of 16 bytes.
+ * Row i stands at position t = i + Nk - Nq and sees key j where j <= t + right and (j >= t - left or j < sinks) and j < lengths[b].
+ * left, right: -1 = no limit; sinks <= 128; lengths: B device int32 (NULL: Nk), taken into [0, Nk]; keys behind are not read.  A row
+ * that sees nothing gives zeros.  o, dout, dq (B, Nq, H, D) and dk, dv (B, Nk, Hk, D) are contiguous; lse [B][H][Nq] (16-byte aligned, NULL:
+ * not wanted) is what the backward call needs.  Inside lengths[b] keys and values must be finite: one that is not may reach rows
+ * within 128 positions of those that see it. */
+int pt_attention_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* strides, const int32_t* lengths, int B,
+                            int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, void* stream);
+size_t pt_attention_window_bwd_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks);
+int pt_attention_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                            const int64_t* strides, const int32_t* lengths, int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks,
+                            float scale, int dtype, void* ws, size_t ws_bytes, void* stream);
+/* The same for one token per sequence over a cache: q (B, H, D), k and v (B, N, Hk, D), strides: batch and head of q, then batch, row
+ * and head of k and v; lengths[b] tokens are in the cache, the last of them the query's own.  Only visible keys are read. */
+size_t pt_attention_window_step_workspace_bytes(int B, int N, int H, int Hk, int D, int left, int sinks);
+int pt_attention_window_step(const void* q, const void* k, const void* v, void* o, const int64_t* strides, const int32_t* lengths, int B, int N, int H,
+                             int Hk, int D, int left, int sinks, float scale, int dtype, void* ws, size_t ws_bytes, void* stream);
 /* measurement aid (bench.py roofline leg): when enabled every tap-GEMM launch is bracketed by HIP events
  * on its stream; pt_prof_read sums elapsed ms / algorithmic FLOPs / launches per kernel config
  * {0-2: fp32 tap-GEMM 128x128 / 64x128 / 64x64 tiles, 3-5: 4-wave bf16 tap-GEMM 128x128 / 64x128 / 64x64 and the conv

@@ -40,6 +40,11 @@ int launch_moment_values(const unsigned char* m, const unsigned char* v, const f
 size_t gated_norm_workspace(int rows, int cols, int clip);
 int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1, const float* b1, const float* w2, const float* b2, void* y, void* h, float* stats, int64_t rows, int cols, int clip, int kind, float eps, int dtype, hipStream_t s);
 int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1, const float* b1, const float* w2, const float* stats, const void* dy, const void* dh, void* dx, void* dt, void* dgate, float* da, float* dw1, float* db1, float* dw2, float* db2, void* ws, size_t ws_bytes, int64_t rows, int cols, int clip, int kind, int dtype, hipStream_t s);
+int launch_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* st, const int* lengths, int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, hipStream_t s);
+size_t window_bwd_workspace(int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks);
+int launch_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv, const int64_t* st, const int* lengths, int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, void* ws, size_t ws_bytes, hipStream_t s);
+size_t window_step_workspace(int B, int N, int H, int Hk, int D, int left, int sinks);
+int launch_window_step(const void* q, const void* k, const void* v, void* o, const int64_t* st, const int* lengths, int B, int N, int H, int Hk, int D, int left, int sinks, float scale, int dtype, void* ws, size_t ws_bytes, hipStream_t s);
 size_t grad_norm_workspace(const int64_t* n, int count);
 int launch_grad_norm(const void* const* g, const int64_t* n, const unsigned char* is_bf16, int count, float max_norm, float* norm, float* coef, void* ws, size_t ws_bytes, hipStream_t s);
 int launch_attention_bf16(const unsigned short* Q, int ldq, const unsigned short* K, int ldk, const unsigned short* V, int ldv, unsigned short* O, int ldo, int B, int Nq, int Nk, int H, hipStream_t s);
@@ -449,6 +454,26 @@ int pt_attention_bf16(const void* Q, int ldq, const void* K, int ldk, const void
   PT_CHECK(Q && K && V && O, "pt_attention_bf16: null argument");
   return launch_attention_bf16((const unsigned short*)Q, ldq, (const unsigned short*)K, ldk, (const unsigned short*)V, ldv,
                                (unsigned short*)O, ldo, B, Nq, Nk, H, (hipStream_t)stream);
+}
+int pt_attention_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* strides, const int32_t* lengths, int B,
+                            int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, void* stream) {
+  return launch_window_fwd(q, k, v, o, lse, strides, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale, dtype, (hipStream_t)stream);
+}
+size_t pt_attention_window_bwd_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks) {
+  return window_bwd_workspace(B, Nq, Nk, H, Hk, D, left, right, sinks);
+}
+int pt_attention_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                            const int64_t* strides, const int32_t* lengths, int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks,
+                            float scale, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  return launch_window_bwd(q, k, v, o, dout, lse, dq, dk, dv, strides, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale, dtype, ws, ws_bytes,
+                           (hipStream_t)stream);
+}
+size_t pt_attention_window_step_workspace_bytes(int B, int N, int H, int Hk, int D, int left, int sinks) {
+  return window_step_workspace(B, N, H, Hk, D, left, sinks);
+}
+int pt_attention_window_step(const void* q, const void* k, const void* v, void* o, const int64_t* strides, const int32_t* lengths, int B, int N, int H,
+                             int Hk, int D, int left, int sinks, float scale, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  return launch_window_step(q, k, v, o, strides, lengths, B, N, H, Hk, D, left, sinks, scale, dtype, ws, ws_bytes, (hipStream_t)stream);
 }
 int pt_pq_gather_cl(const void* idx, int idx_are_int64, const float* codebooks, int rows, int G, int D, int K,
                     float* out, int ldq, void* stream) {

@@ -332,6 +332,120 @@ def attention_cross(q, kv, B, Nq, Nk, p=0.0, seeds=None):
     return Attention.apply(q, kv, 0, 0, 512, B, Nq, Nk, p, seeds.next() if p > 0 else 0)
 
 
+def _strides(*tensors):
+    """Strides of all but the last dimension, as the C entries take them (a dimension of one value has none)."""
+    return array.array("q", [s if n > 1 else 0 for t in tensors for s, n in zip(t.stride()[:-1], t.shape[:-1])])
+
+
+def _has_vectors(t):
+    """Whether rows of channels can be read in 16-byte vectors."""
+    size = t.element_size()
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and
+            all(n == 1 or (s * size) % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])))
+
+
+def _vectors(t):
+    """t itself if it can be read in vectors, else a contiguous copy."""
+    if _has_vectors(t):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class WindowAttention(torch.autograd.Function):
+    """softmax over a window of keys and a few first ones (see window_attention)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, left, right, sinks, scale, grad):
+        B, Nq, H, D = q.shape
+        Nk, Hk = k.shape[1], k.shape[2]
+        o = torch.empty(B, Nq, H, D, device=q.device, dtype=q.dtype)
+        lse = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32) if grad else None
+        ctx.meta = (B, Nq, Nk, H, Hk, D, left, right, sinks, scale, int(q.dtype is torch.bfloat16))
+        with _on(q.device):
+            check(_lib.lib().pt_attention_window_fwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), _address(_strides(q, k, v)), ptr(lengths), *ctx.meta,
+                                                     stream()))
+        if grad:
+            ctx.save_for_backward(q, k, v, lengths, o, lse)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, lengths, o, lse = ctx.saved_tensors
+        L = _lib.lib()
+        do = _vectors(do.contiguous())
+        dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+        with _on(q.device):
+            ws = torch.empty(int(L.pt_attention_window_bwd_workspace_bytes(*ctx.meta[:9])), dtype=torch.uint8, device=q.device)
+            check(L.pt_attention_window_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(do), ptr(lse), ptr(dq), ptr(dk), ptr(dv), _address(_strides(q, k, v)),
+                                            ptr(lengths), *ctx.meta, ptr(ws), ws.numel(), stream()))
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+def _check_window(what, q, k, v, heads, batch, lengths, left, right, sinks, scale):
+    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != batch or k.shape[3] != q.shape[-1] or k.shape[1] < 1:
+        raise RuntimeError(f"{what}: shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} do not go together")
+    if not q.is_cuda or k.device != q.device or v.device != q.device:
+        raise RuntimeError(f"{what}: tensors must be on one GPU, got {q.device}, {k.device} and {v.device}")
+    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise RuntimeError(f"{what}: fp32 or bf16, one type for all, got {q.dtype}, {k.dtype} and {v.dtype}")
+    d = q.shape[-1]
+    if d % 8 or not 8 <= d <= 128 or k.shape[2] < 1 or heads < 1 or heads % k.shape[2]:
+        raise RuntimeError(f"{what}: {heads} query heads over {k.shape[2]} key heads of {d} channels (a multiple of 8 up to 128)")
+    if lengths is not None and (tuple(lengths.shape) != (batch,) or lengths.dtype is not torch.int32 or lengths.device != q.device or not lengths.is_contiguous()):
+        raise RuntimeError(f"{what}: lengths must be ({batch},) torch.int32 on {q.device}")
+    left, right = (-1 if n is None else int(n) for n in (left, right))
+    if left < -1 or right < -1 or not 0 <= sinks <= 128:
+        raise RuntimeError(f"{what}: a window of {left} to the left and {right} to the right with {sinks} first keys (up to 128)")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise RuntimeError(f"{what}: scale must be positive, got {scale}")
+    return min(left, 1 << 30), min(right, 1 << 30), int(sinks), scale
+
+
+def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=None):
+    """Attention of q (B, Nq, H, D) over k, v (B, Nk, Hk, D), fp32 or bf16 -> (B, Nq, H, D); H is a multiple of Hk (heads of a
+    group share a key head), D a multiple of 8 up to 128, any strides.  Row i stands at position t = i + Nk - Nq and sees key j where
+
+        j <= t + right   and   (j >= t - left or j < sinks)   and   j < lengths[b]
+
+    left, right: None for no limit (right = 0 is causal); sinks: first keys that stay visible, up to 128; lengths: int32 (B,), the
+    keys of each sequence of a padded batch (what lies behind is not read; all of them by default).  A row that sees nothing gives
+    zeros and no gradient.  Softmax and sums are fp32; scale is 1 / sqrt(D) by default.  Keys and values inside a sequence must be
+    finite.  The backward pass is free of atomics: the same inputs give the same bits.  To capture it into a HIP graph, make the
+    leaves inside the capture (q.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
+    if q.dim() != 4 or q.shape[0] < 1 or q.shape[1] < 1:
+        raise RuntimeError(f"window_attention: q is (B, Nq, H, D), got {tuple(q.shape)}")
+    args = _check_window("window_attention", q, k, v, q.shape[2], q.shape[0], lengths, left, right, sinks, scale)
+    if k.shape[1] < q.shape[1]:
+        raise RuntimeError(f"window_attention: {q.shape[1]} rows for {k.shape[1]} keys")
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return WindowAttention.apply(_vectors(q), _vectors(k), _vectors(v), lengths, *args, grad)
+
+
+def window_attention_step(q, k, v, lengths, left=None, sinks=0, scale=None):
+    """window_attention for one new token per sequence over a cache: q (B, H, D), k, v (B, N, Hk, D) with room for N tokens, of
+    which the first lengths[b] (int32) are filled and the last of these is the token's own -> (B, H, D).  Reads the visible keys
+    only, whatever else the cache holds; a sequence of length 0 gives zeros.  No gradient."""
+    if q.dim() != 3 or q.shape[0] < 1:
+        raise RuntimeError(f"window_attention_step: q is (B, H, D), got {tuple(q.shape)}")
+    if lengths is None:
+        raise RuntimeError("window_attention_step: lengths are needed")
+    left, _, sinks, scale = _check_window("window_attention_step", q, k, v, q.shape[1], q.shape[0], lengths, left, 0, sinks, scale)
+    q, k, v = q.detach(), k.detach(), v.detach()
+    if not _has_vectors(k) or not _has_vectors(v):
+        raise RuntimeError("window_attention_step: a cache's channels must be neighbours, its address and strides multiples of 16 bytes")
+    q = _vectors(q)
+    (B, H, D), (N, Hk) = q.shape, k.shape[1:3]
+    o = torch.empty(B, H, D, device=q.device, dtype=q.dtype)
+    L = _lib.lib()
+    with _on(q.device):
+        ws = torch.empty(int(L.pt_attention_window_step_workspace_bytes(B, N, H, Hk, D, left, sinks)), dtype=torch.uint8, device=q.device)
+        check(L.pt_attention_window_step(ptr(q), ptr(k), ptr(v), ptr(o), _address(_strides(q, k, v)), ptr(lengths), B, N, H, Hk, D, left, sinks, scale,
+                                         int(q.dtype is torch.bfloat16), ptr(ws), ws.numel(), stream()))
+    return o
+
+
 class CrossEntropy(torch.autograd.Function):
     """F.cross_entropy(logits [rows, V], target [rows]) with mean reduction (predictor.py:261)."""
 
@@ -687,7 +801,8 @@ def _addresses(tensors):
 
 
 def _address(a):
-    return None if a is None else C.c_void_p(a.buffer_info()[0])
+    """An array.array as a pointer argument; the argument holds the array, which may have no other reference."""
+    return None if a is None else (C.c_char * (len(a) * a.itemsize)).from_buffer(a)
 
 
 def _grad_norm(pointers, sizes, is_bf16, max_norm, device):

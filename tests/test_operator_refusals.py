@@ -59,3 +59,45 @@ def test_gated_norm_refuses():
     refused(bwd(p, p, p, p, p, p, 1 << 20), "null")           # a gate's gradient without a gate
     refused(bwd(p, p, p, p, n, p, 0), "workspace")
     refused(bwd(p, p, p, p, n, odd, 1 << 20), "workspace")
+
+
+def test_host_arrays_live_as_long_as_their_addresses():
+    """Strides and pointer lists go to the C entries as addresses of arrays that nothing else refers to."""
+    t = torch.zeros(5, 6, 7, 8)
+    held = [T._address(T._strides(t, t[:, :1], t[:1])) for _ in range(50)]
+    junk = [T._strides(t[:, ::2], t, t) for _ in range(200)]
+    for a in held:
+        assert list((C.c_int64 * 9).from_address(C.addressof(a))) == [336, 56, 8, 336, 0, 8, 0, 56, 8]
+    assert len(junk) == 200 and T._address(None) is None
+
+
+def test_window_attention_refuses():
+    t = torch.zeros(1, 4, 2, 8)
+    with pytest.raises(RuntimeError, match="on one GPU"):
+        T.window_attention(t, t, t)
+    with pytest.raises(RuntimeError, match="on one GPU"):
+        T.window_attention_step(t[:, 0], t, t, torch.ones(1, dtype=torch.int32))
+    L, p, odd, n = _lib.lib(), C.c_void_p(256), C.c_void_p(264), None
+    st = (C.c_int64 * 9)(*([64] * 9))
+    one = dict(B=1, Nq=4, Nk=4, H=2, Hk=1, D=16, left=1, right=0, sinks=0, scale=0.5, dtype=1)
+    def fwd(word, q=p, lse=p, o=p, strides=st, **kw):
+        refused(L.pt_attention_window_fwd(q, p, p, o, lse, strides, n, *(one | kw).values(), None), word)
+    fwd("null", q=n)
+    fwd("null", o=n)
+    fwd("multiples", q=odd)
+    fwd("multiples", strides=(C.c_int64 * 9)(*([64] * 8 + [60])))
+    for kw, word in ((dict(B=0), "rows"), (dict(Nq=0), "rows"), (dict(Nq=5), "rows"), (dict(Nk=1 << 29), "rows"), (dict(B=70000), "rows"), (dict(H=3, Hk=2), "heads"),
+                     (dict(Hk=0), "heads"), (dict(D=12), "dimension"), (dict(D=136), "dimension"), (dict(left=-2), "window"), (dict(sinks=129), "window"),
+                     (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(dtype=2), "dtype")):
+        fwd(word, **kw)
+    ws = L.pt_attention_window_bwd_workspace_bytes(1, 700, 700, 2, 1, 64, 50, 0, 5)
+    assert ws > 2 * 700 * 4 and L.pt_attention_window_bwd_workspace_bytes(1, 700, 700, 2, 1, 64, 50, 0, 0) == 5632
+    big = (one | dict(Nq=700, Nk=700, D=64, left=50, sinks=5)).values()
+    refused(L.pt_attention_window_bwd(p, p, p, p, p, p, p, p, p, st, n, *big, p, ws - 1, None), "workspace")
+    refused(L.pt_attention_window_bwd(p, p, p, p, p, n, p, p, p, st, n, *big, p, ws, None), "null")
+    refused(L.pt_attention_window_bwd(p, p, p, p, odd, p, p, p, p, st, n, *big, p, ws, None), "multiples")
+    step = dict(B=1, N=4, H=2, Hk=1, D=16, left=1, sinks=0, scale=0.5, dtype=1)
+    refused(L.pt_attention_window_step(p, p, p, p, st, n, *step.values(), p, 1 << 20, None), "null")
+    refused(L.pt_attention_window_step(p, p, p, p, st, p, *(step | dict(N=0)).values(), p, 1 << 20, None), "keys")
+    refused(L.pt_attention_window_step(p, p, p, p, st, p, *step.values(), p, 0, None), "workspace")
+    refused(L.pt_attention_window_step(p, odd, p, p, st, p, *step.values(), p, 1 << 20, None), "multiples")
