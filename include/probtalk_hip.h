@@ -188,7 +188,8 @@ int pt_attention_bf16(const void* Q, int ldq, const void* K, int ldk, const void
                       int Nq, int Nk, int H, void* stream);
 /* Attention over a window of keys and a few first ones.  q (B, Nq, H, D), k and v (B, Nk, Hk, D), dtype 0 fp32 | 1 bf16, D a multiple of 8
  * up to 128, H a multiple of Hk (query head h uses key head h / (H / Hk)), Nk >= Nq.  strides: nine host values, of batch, row and head for
- * q, k and v, in elements; neighbouring channels are neighbours in memory; addresses and strides are multiples of 16 bytes.
+ * q, k and v, in elements; neighbouring channels are neighbours in memory; addresses and strides are multiples of 16 bytes,
+ * rows at most 2^20 values apart.
  * Row i stands at position t = i + Nk - Nq and sees key j where j <= t + right and (j >= t - left or j < sinks) and j < lengths[b].
  * left, right: -1 = no limit; sinks <= 128; lengths: B device int32 (NULL: Nk), taken into [0, Nk]; keys behind are not read.  A row
  * that sees nothing gives zeros.  o, dout, dq (B, Nq, H, D) and dk, dv (B, Nk, Hk, D) are contiguous; lse [B][H][Nq] (16-byte aligned, NULL:

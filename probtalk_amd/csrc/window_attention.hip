@@ -17,7 +17,8 @@
 // kernel S = Q K^T then dV^T += dO^T P: probabilities never leave the registers, softmax statistics are one value per lane.
 // The first operand of those second products is the transpose of a tile that lies row by row in LDS: bf16 reads it with the
 // transposing ds_read_b64_tr_b16, fp32 with single words.  LDS rows hold 16-byte chunks in an order that is free of bank conflicts
-// for both kinds of reads: chunk ^= bit-reversed low bits of the row.
+// for both kinds of reads (Tile::swz).  Tiles come by
+// LDS-DMA into two buffers: a tile is under way while the one before is worked on.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -34,7 +35,8 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef const __attribute__((address_space(1))) void* glb_ptr_t;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -76,76 +78,176 @@ struct WinArgs {
 };
 
 __device__ __forceinline__ int length_of(const WinArgs& a, int b) { return a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk; }
-__device__ __forceinline__ bool visible(const WinArgs& a, int len, int t, int j) {
-  return j <= t + a.right && (j >= t - a.left || j < a.sinks) && j < len;
-}
 
-// LDS image of a tile: rows of DP values, 16-byte chunks permuted within the row
+// LDS image of a tile: rows of DP values, 16-byte chunks permuted within the row by swz(row), which is linear over xor and looks at the
+// row's low four bits only.  So a lane's address for any operand of a tile is one base of its own, xor and plus constants.
 template <typename T, int DP>
 struct Tile {
   static constexpr int RB = DP * (int)sizeof(T), CPR = RB / 16, EPC = 16 / (int)sizeof(T);
   typedef typename Types<T>::frag frag;
-  // 128-byte rows: two rows per turn of the banks, so the row's lowest bit is a half already
-  static __device__ __forceinline__ int swz(int row) {
-    if constexpr (RB == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
-    else return (row & 1) << 3 | (row & 2) << 1 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+  static __device__ __forceinline__ constexpr int swz(int row) {
+    // 128-byte rows: two rows per turn of the banks, so the row's lowest bit is a half already
+    if (RB == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+    // transposing reads take four rows of 64 bytes at a time: these go to the four quarters of the banks
+    if (sizeof(T) == 2) return (row & 1) << 3 | ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+    // single words take rows r and r + 4, half of the banks each
+    return ((row >> 2) & 1) << 3 | (row & 1) << 2 | ((row >> 1) & 1) << 1 | ((row >> 3) & 1);
   }
   static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swz(row)) << 4); }
-  // 8 values along the row: columns 16 s + 8 h .. + 7 of row
-  static __device__ __forceinline__ frag row_frag(const unsigned char* m, int row, int s, int h) {
-    if constexpr (sizeof(T) == 2) return *reinterpret_cast<const bf16x8*>(m + at(row, 2 * s + h));
+  // rows: lane base for 8 values along row `row` (16 s + 8 h of it)
+  static __device__ __forceinline__ int row_base(int row, int h) { return at(row, sizeof(T) == 2 ? h : 2 * h); }
+  static __device__ __forceinline__ frag row_frag(const unsigned char* m, int base, int s) {
+    if constexpr (sizeof(T) == 2) return *reinterpret_cast<const bf16x8*>(m + (base ^ (s << 5)));
     else {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(m + at(row, 4 * s + 2 * h)), y = *reinterpret_cast<const f32x4*>(m + at(row, 4 * s + 2 * h + 1));
+      const f32x4 x = *reinterpret_cast<const f32x4*>(m + (base ^ (s << 6))), y = *reinterpret_cast<const f32x4*>(m + (base ^ (s << 6) ^ 16));
       const frag f = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       return f;
     }
   }
-  // 8 values down a column: rows row0 + 8 (e >> 2) + 4 h + (e & 3) of column 32 db + lane % 32
-  static __device__ __forceinline__ frag col_frag(const unsigned char* m, int row0, int db, int lane) {
+  // columns: lane base for 8 values down column 32 db + lane % 32: rows row0 + 8 (e >> 2) + 4 h + (e & 3), row0 a multiple of 16
+  static __device__ __forceinline__ int col_base(int lane) {
     const int h = lane >> 5;
     if constexpr (sizeof(T) == 2) {
-      const int tq = (lane >> 2) & 3, tp = lane & 3, tg = (lane >> 4) & 1, c = db * 4 + tg * 2 + (tp >> 1);
-      const int r0 = row0 + 4 * h + tq, r1 = r0 + 8;
-      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(m + at(r0, c) + (tp & 1) * 8));
-      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(m + at(r1, c) + (tp & 1) * 8));
-      const s16x8 f = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      return __builtin_bit_cast(bf16x8, f);
+      const int tq = (lane >> 2) & 3, tp = lane & 3, tg = (lane >> 4) & 1;
+      return at(4 * h + tq, tg * 2 + (tp >> 1)) + (tp & 1) * 8;
     } else {
-      const int d = db * 32 + (lane & 31);
-      frag f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int r = row0 + 8 * (e >> 2) + 4 * h + (e & 3);
-        f[e] = *reinterpret_cast<const float*>(m + at(r, d / 4) + (d & 3) * 4);
-      }
-      return f;
+      const int d = lane & 31;
+      return at(4 * h, d / 4) + (d & 3) * 4;
     }
   }
 };
 
-// R rows of a tile on their way from memory to LDS; rows from `limit` on and columns from D on are zeros
-template <typename T, int DP, int R>
-struct Stage {
-  typedef Tile<T, DP> tile;
-  static constexpr int N = R * tile::CPR / 256;
-  static_assert(N >= 1, "tile too small for the workgroup");
-  u32x4 x[N];
-  __device__ __forceinline__ void load(const T* __restrict__ base, int64_t stride, int row0, int limit, int D) {
+// The column operands of 32 rows of a tile, all columns: f[s2][db] are rows OFF / RB + 16 s2 .. + 15.
+// bf16: the transposing reads are asm with their wait: the compiler takes the builtin for one that may read what LDS-DMA is still
+// writing and waits for every load in flight, which are the next tile's.  The caller's barriers order them.
+template <typename T, int DP> struct Cols;
+template <int DP>
+struct Cols<__bf16, DP> {
+  typedef Tile<__bf16, DP> tile;
+  static constexpr int RB = tile::RB, ND = DP / 32;
+  unsigned x[ND], y[ND];
+  __device__ __forceinline__ Cols(const unsigned char* m, int base) {
+    const unsigned at = (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned char*)m + base;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = threadIdx.x + 256 * i, row = row0 + e / tile::CPR, c = (e % tile::CPR) * tile::EPC;
-      x[i] = u32x4{0u, 0u, 0u, 0u};
-      if (row >= 0 && row < limit && c < D) x[i] = *reinterpret_cast<const u32x4*>(base + row * stride + c);
+    for (int db = 0; db < ND; ++db) {
+      x[db] = at ^ (db << 6);
+      y[db] = x[db] ^ (tile::swz(8) << 4);
     }
   }
-  __device__ __forceinline__ void store(unsigned char* m) const {
+  template <int OFF>
+  __device__ __forceinline__ void read(bf16x8 (&f)[2][ND]) const {
+    s16x4 r[4][ND];
+    if constexpr (ND == 4) {
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %4, %20 offset:%25\n\t"
+          "ds_read_b64_tr_b16 %1, %17 offset:%24\n\tds_read_b64_tr_b16 %5, %21 offset:%25\n\t"
+          "ds_read_b64_tr_b16 %2, %18 offset:%24\n\tds_read_b64_tr_b16 %6, %22 offset:%25\n\t"
+          "ds_read_b64_tr_b16 %3, %19 offset:%24\n\tds_read_b64_tr_b16 %7, %23 offset:%25\n\t"
+          "ds_read_b64_tr_b16 %8, %16 offset:%26\n\tds_read_b64_tr_b16 %12, %20 offset:%27\n\t"
+          "ds_read_b64_tr_b16 %9, %17 offset:%26\n\tds_read_b64_tr_b16 %13, %21 offset:%27\n\t"
+          "ds_read_b64_tr_b16 %10, %18 offset:%26\n\tds_read_b64_tr_b16 %14, %22 offset:%27\n\t"
+          "ds_read_b64_tr_b16 %11, %19 offset:%26\n\tds_read_b64_tr_b16 %15, %23 offset:%27\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3]),
+            "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[2][2]), "=&v"(r[2][3]), "=&v"(r[3][0]), "=&v"(r[3][1]), "=&v"(r[3][2]), "=&v"(r[3][3])
+          : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]), "i"(OFF), "i"(OFF + 8 * RB), "i"(OFF + 16 * RB),
+            "i"(OFF + 24 * RB));
+    } else {
+      static_assert(ND == 2, "64 or 128 columns");
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %10 offset:%13\n\t"
+          "ds_read_b64_tr_b16 %1, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%13\n\t"
+          "ds_read_b64_tr_b16 %4, %8 offset:%14\n\tds_read_b64_tr_b16 %6, %10 offset:%15\n\t"
+          "ds_read_b64_tr_b16 %5, %9 offset:%14\n\tds_read_b64_tr_b16 %7, %11 offset:%15\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[3][0]), "=&v"(r[3][1])
+          : "v"(x[0]), "v"(x[1]), "v"(y[0]), "v"(y[1]), "i"(OFF), "i"(OFF + 8 * RB), "i"(OFF + 16 * RB), "i"(OFF + 24 * RB));
+    }
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int db = 0; db < ND; ++db) {
+        const s16x4 p = r[2 * s2][db], q = r[2 * s2 + 1][db];
+        const s16x8 v = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
+        f[s2][db] = __builtin_bit_cast(bf16x8, v);
+      }
+  }
+};
+template <int DP>
+struct Cols<float, DP> {
+  typedef Tile<float, DP> tile;
+  static constexpr int RB = tile::RB, ND = DP / 32;
+  const unsigned char* m;
+  int base;
+  __device__ __forceinline__ Cols(const unsigned char* m_, int base_) : m(m_), base(base_) {}
+  template <int OFF>
+  __device__ __forceinline__ void read(f32x8 (&f)[2][ND]) const {
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int r = 8 * (e >> 2) + (e & 3);
+          f[s2][db][e] = *reinterpret_cast<const float*>(m + OFF + (16 * s2 + r) * RB + (base ^ (tile::swz(r) << 4) ^ (db << 7)));
+        }
+  }
+};
+// acc[db] += (columns of 32 rows)^T . p, p the registers of a score tile over these rows
+template <typename T, int DP, int OFF>
+__device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const Cols<T, DP>& cols, const f32x16& p) {
+  typename Types<T>::frag f[2][DP / 32];
+  cols.template read<OFF>(f);
+#pragma unroll
+  for (int s2 = 0; s2 < 2; ++s2) {
+    typename Types<T>::frag x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (T)p[8 * s2 + e];
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], x, acc[db]);
+  }
+}
+
+// R rows of a tile straight from memory to LDS (LDS-DMA: no registers, nothing for the compiler to wait for), by TH threads.  A wave
+// writes 1 KB at a time, lane after lane, so the order of the chunks is made by the addresses that the lanes read from.  Rows behind
+// the last one are that row again and columns behind D the row's first ones: such scores are masked or meet zeros of the other
+// operand, and what such columns give is not stored.
+template <typename T, int DP, int R, int TH>
+struct Dma {
+  typedef Tile<T, DP> tile;
+  static constexpr int RB = tile::RB, W = TH / 64, ROWS = W * 1024 / RB, N = R / ROWS;     // rows per turn of all waves, turns
+  static_assert(N >= 1 && R % ROWS == 0, "tile too small for the workgroup");
+  int row, col[2];                                       // row and column of this lane in the first turn (and in odd turns of 8 rows)
+  __device__ __forceinline__ Dma(int D) {
+    const int byte = threadIdx.x * 16;
+    row = byte / RB;
+    const int chunk = (byte % RB / 16) ^ tile::swz(row);
+    col[0] = chunk * tile::EPC < D ? chunk * tile::EPC : 0;
+    col[1] = (chunk ^ tile::swz(ROWS)) * tile::EPC < D ? (chunk ^ tile::swz(ROWS)) * tile::EPC : 0;
+  }
+  __device__ __forceinline__ void operator()(const T* __restrict__ base, int64_t stride, int row0, int limit, unsigned char* m) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), st = (int)stride, last = limit - 1 - row0;   // row0 < limit
+    base += row0 * stride;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = threadIdx.x + 256 * i;
-      *reinterpret_cast<u32x4*>(m + tile::at(e / tile::CPR, e % tile::CPR)) = x[i];
+      const int c = col[ROWS % 16 ? i & 1 : 0];
+      unsigned off;
+      const T* from = base;
+      if (R - 1 <= last) {                               // uniform: a whole tile
+        off = (unsigned)(row * st + c);
+        from += (int64_t)i * ROWS * st;
+      } else {
+        off = (unsigned)(min(row + i * ROWS, last) * st + c);
+      }
+      __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + off), (lds_ptr_t)(m + (i * W + wave) * 1024), 16, 0, 0);
     }
   }
 };
+// loads to LDS of this wave have arrived; the barrier behind it says so of all waves
+__device__ __forceinline__ void dma_wait() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
 
 // 8 values of row `row` from memory, as an operand
 template <typename T>
@@ -154,13 +256,6 @@ __device__ __forceinline__ typename Types<T>::frag global_frag(const T* __restri
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = (T)0.f;
   if (row < limit && c < D) f = *reinterpret_cast<const typename Types<T>::frag*>(base + row * stride + c);
-  return f;
-}
-template <typename T>
-__device__ __forceinline__ typename Types<T>::frag pack(const f32x16& p, int s2) {
-  typename Types<T>::frag f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = (T)p[8 * s2 + e];
   return f;
 }
 // a transposed result (lane: row `row` of the output, registers: columns) times x
@@ -188,22 +283,63 @@ __device__ __forceinline__ void key_tiles(const WinArgs& a, int len, int t0, int
   from = max(lo / KT, first);
   to = hi < lo ? from : max(hi / KT + 1, from);
 }
+// Scores of invisible pairs to -infinity: keys along the registers of a transposed tile (KEYS) or along the lanes
+template <bool KEYS>
+__device__ __forceinline__ void mask_tile(const WinArgs& a, int len, int t, int key, int h, f32x16& st, int last = 0x7FFFFFFF) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int step = (r & 3) + 8 * (r >> 2) + 4 * h, tt = KEYS ? t : t + step, j = KEYS ? key + step : key;
+    const bool on = (j <= tt + a.right) & ((j >= tt - a.left) | (j < a.sinks)) & (j < len) & (KEYS | (tt <= last));
+    st[r] = on ? st[r] : -INFINITY;
+  }
+}
+// Workgroups go to the 8 XCDs in turn, each with an L2 of its own: XCD x gets a run of neighbours in the order of the work, so that
+// workgroups that read the same keys (or rows) share an L2
+__device__ __forceinline__ int work_item(int id, int total) {
+  const int q = total / 8, r = total % 8, x = id % 8;
+  return x * q + min(x, r) + id / 8;
+}
+struct Place { int tile, head, kvh, b; };
+// order of the work: query heads of a group, tiles, key heads, sequences
+__device__ __forceinline__ Place place(const WinArgs& a, int tiles) {
+  const int group = a.H / a.Hk;
+  int n = work_item(blockIdx.x, gridDim.x);
+  Place p;
+  const int g = n % group; n /= group;
+  p.tile = n % tiles; n /= tiles;
+  p.kvh = n % a.Hk;
+  p.b = n / a.Hk;
+  p.head = p.kvh * group + g;
+  return p;
+}
+template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 2 || DP == 64 ? 64 : 32; }
 
 // ---------------------------------------------------------------------------
 // Forward: 4 waves of 32 rows each over common key tiles
 // ---------------------------------------------------------------------------
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs a) {
-  constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32;
+__global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fwd_kernel(const WinArgs a) {
+  constexpr int KT = key_tile<T, DP>(), NB = KT / 32;
   typedef Tile<T, DP> tile;
-  __shared__ __attribute__((aligned(1024))) unsigned char Ks[KT * tile::RB], Vs[KT * tile::RB];
+  constexpr int TB = KT * tile::RB;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];      // [2][K tile | V tile]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int head = blockIdx.y, b = blockIdx.z, kvh = head / (a.H / a.Hk);
+  const Place at = place(a, (a.Nq + 127) / 128);
+  const int head = at.head, b = at.b, i00 = at.tile * 128;
   const int len = length_of(a, b), shift = a.Nk - a.Nq;
-  const int i0 = blockIdx.x * 128 + wave * 32, row = i0 + col, t = row + shift;
-  const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + kvh * a.sk[2];
-  const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + kvh * a.sv[2];
+  const int i0 = i00 + wave * 32, row = i0 + col, t = row + shift;
+  const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + at.kvh * a.sk[2];
+  const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + at.kvh * a.sv[2];
   const T* __restrict__ Q = (const T*)a.q + b * a.sq[0] + head * a.sq[2];
+  int first, from, to;
+  key_tiles<KT>(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift, first, from, to);
+  const int tiles = first + (to - from);
+  auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
+  const Dma<T, DP, KT, 256> dma(a.D);
+  if (tiles > 0) {
+    dma(K, a.sk[1], key_of(0), len, win_smem);
+    dma(V, a.sv[1], key_of(0), len, win_smem + TB);
+  }
   typename Types<T>::frag qf[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) qf[s] = global_frag(Q, a.sq[1], row, a.Nq, 16 * s + 8 * h, a.D);
@@ -211,73 +347,57 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs a) {
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) o[db] = zero16();
   float m = -INFINITY, l = 0.f;
-  int first, from, to;
-  const int T0 = blockIdx.x * 128 + shift, T1 = min(blockIdx.x * 128 + 127, a.Nq - 1) + shift;
-  key_tiles<KT>(a, len, T0, T1, first, from, to);
-  const int tiles = first + (to - from);
   const int w0 = i0 + shift, w1 = min(i0 + 31, a.Nq - 1) + shift;        // positions of this wave
-  Stage<T, DP, KT> sk, sv;
-  if (tiles > 0) {
-    const int k0 = (first ? 0 : from) * KT;
-    sk.load(K, a.sk[1], k0, len, a.D);
-    sv.load(V, a.sv[1], k0, len, a.D);
-  }
+  const int rb = tile::row_base(col, h), cb = tile::col_base(lane);
+  dma_wait();
   for (int n = 0; n < tiles; ++n) {
-    const int k0 = (n < first ? n : from + n - first) * KT, k1 = k0 + KT - 1;
-    __syncthreads();
-    sk.store(Ks);
-    sv.store(Vs);
-    __syncthreads();
-    if (n + 1 < tiles) {
-      const int kn = (n + 1 < first ? n + 1 : from + n + 1 - first) * KT;
-      sk.load(K, a.sk[1], kn, len, a.D);
-      sv.load(V, a.sv[1], kn, len, a.D);
+    const unsigned char* Ks = win_smem + (n & 1) * 2 * TB;
+    const unsigned char* Vs = Ks + TB;
+    const int k0 = key_of(n), k1 = k0 + KT - 1;
+    if (n + 1 < tiles) {                                                 // into the other buffer: its readers passed the last barrier
+      unsigned char* next = win_smem + ((n + 1) & 1) * 2 * TB;
+      dma(K, a.sk[1], key_of(n + 1), len, next);
+      dma(V, a.sv[1], key_of(n + 1), len, next + TB);
     }
-    if (i0 >= a.Nq || k0 > w1 + a.right || (k1 < w0 - a.left && k0 >= a.sinks)) continue;
-    f32x16 st[NB];
+    if (i0 < a.Nq && k0 <= w1 + a.right && (k1 >= w0 - a.left || k0 < a.sinks)) {
+      f32x16 st[NB];
 #pragma unroll
-    for (int x = 0; x < NB; ++x) {
-      st[x] = zero16();
+      for (int x = 0; x < NB; ++x) {
+        st[x] = zero16();
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s) st[x] = mma(tile::row_frag(Ks, 32 * x + col, s, h), qf[s], st[x]);
-    }
-    if (!(k1 <= w0 + a.right && k1 < len && (k0 >= w1 - a.left || k1 < a.sinks))) {
+        for (int s = 0; s < DP / 16; ++s) st[x] = mma(tile::row_frag(Ks + 32 * x * tile::RB, rb, s), qf[s], st[x]);
+      }
+      if (!(k1 <= w0 + a.right && k1 < len && (k0 >= w1 - a.left || k1 < a.sinks)))
+#pragma unroll
+        for (int x = 0; x < NB; ++x) mask_tile<true>(a, len, t, k0 + 32 * x, h, st[x]);
+      float mx = st[0][0];
 #pragma unroll
       for (int x = 0; x < NB; ++x)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          st[x][r] = visible(a, len, t, k0 + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * h) ? st[x][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[x][r]);
+      mx = fmaxf(mx, half_other(mx)) * a.sc;
+      const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;  // nothing visible so far: every exponential is 0
+      const float alpha = __builtin_amdgcn_exp2f(m - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -base));
+          sum += st[x][r];
+        }
+      l = l * alpha + sum;                                               // this lane's half of the column; joined at the end
+      m = mn;
+      if (__ballot(alpha != 1.f))                                        // most tiles leave every row's maximum where it is
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+      const Cols<T, DP> vc(Vs, cb);                                      // probabilities in [0, 1] to bf16: 2^-9 of each
+      add_product<T, DP, 0>(o, vc, st[0]);
+      if constexpr (NB > 1) add_product<T, DP, 32 * tile::RB>(o, vc, st[1]);
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < NB; ++x)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[x][r]);
-    mx = fmaxf(mx, half_other(mx)) * a.sc;
-    const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;    // nothing visible so far: every exponential is 0
-    const float alpha = __builtin_amdgcn_exp2f(m - base);
-    float sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < NB; ++x)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -base));
-        sum += st[x][r];
-      }
-    l = l * alpha + sum;                                                 // this lane's half of the column; joined at the end
-    m = mn;
-#pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-#pragma unroll
-    for (int x = 0; x < NB; ++x)
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const auto pf = pack<T>(st[x], s2);                              // probabilities in [0, 1] to bf16: 2^-9 of each
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) o[db] = mma(tile::col_frag(Vs, 32 * x + 16 * s2, db, lane), pf, o[db]);
-      }
+    dma_wait();
   }
   if (row >= a.Nq) return;
   l += half_other(l);
@@ -288,19 +408,31 @@ __global__ __launch_bounds__(256, 2) void win_fwd_kernel(const WinArgs a) {
 // ---------------------------------------------------------------------------
 // Backward, dQ (and delta): rows and key tiles as forward
 // ---------------------------------------------------------------------------
+template <typename T, int DP> constexpr int key_tile_q() { return sizeof(T) * DP <= 128 ? 64 : 32; }   // 256 registers hold no more
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(const WinArgs a) {
-  constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32;
+__global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bwd_q_kernel(const WinArgs a) {
+  constexpr int KT = key_tile_q<T, DP>(), NB = KT / 32;
   typedef Tile<T, DP> tile;
-  __shared__ __attribute__((aligned(1024))) unsigned char Ks[KT * tile::RB], Vs[KT * tile::RB];
+  constexpr int TB = KT * tile::RB;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int head = blockIdx.y, b = blockIdx.z, kvh = head / (a.H / a.Hk);
+  const Place at = place(a, (a.Nq + 127) / 128);
+  const int head = at.head, b = at.b, i00 = at.tile * 128;
   const int len = length_of(a, b), shift = a.Nk - a.Nq;
-  const int i0 = blockIdx.x * 128 + wave * 32, row = i0 + col, t = row + shift;
-  const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + kvh * a.sk[2];
-  const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + kvh * a.sv[2];
+  const int i0 = i00 + wave * 32, row = i0 + col, t = row + shift;
+  const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + at.kvh * a.sk[2];
+  const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + at.kvh * a.sv[2];
   const T* __restrict__ Q = (const T*)a.q + b * a.sq[0] + head * a.sq[2];
   const int64_t so = (int64_t)a.H * a.D, ob = ((int64_t)b * a.Nq * a.H + head) * a.D;
+  int first, from, to;
+  key_tiles<KT>(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift, first, from, to);
+  const int tiles = first + (to - from);
+  auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
+  const Dma<T, DP, KT, 256> dma(a.D);
+  if (tiles > 0) {
+    dma(K, a.sk[1], key_of(0), len, win_smem);
+    dma(V, a.sv[1], key_of(0), len, win_smem + TB);
+  }
   typename Types<T>::frag qf[DP / 16], gf[DP / 16];
   float delta = 0.f;
 #pragma unroll
@@ -313,185 +445,268 @@ __global__ __launch_bounds__(256, 2) void win_bwd_q_kernel(const WinArgs a) {
   }
   delta += half_other(delta);
   const int64_t li = ((int64_t)b * a.H + head) * a.Nq + row;
-  const float lse = row < a.Nq ? a.lse[li] : INFINITY;
+  float lse = row < a.Nq ? a.lse[li] : INFINITY;
   if (row < a.Nq && h == 0) a.delta[li] = delta;
+  asm volatile("" : "+v"(lse), "+v"(delta));             // here, not in the loop, where the wait for them would be one for the tiles too
   f32x16 dq[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) dq[db] = zero16();
-  int first, from, to;
-  const int T0 = blockIdx.x * 128 + shift, T1 = min(blockIdx.x * 128 + 127, a.Nq - 1) + shift;
-  key_tiles<KT>(a, len, T0, T1, first, from, to);
-  const int tiles = first + (to - from);
   const int w0 = i0 + shift, w1 = min(i0 + 31, a.Nq - 1) + shift;
-  Stage<T, DP, KT> sk, sv;
-  if (tiles > 0) {
-    const int k0 = (first ? 0 : from) * KT;
-    sk.load(K, a.sk[1], k0, len, a.D);
-    sv.load(V, a.sv[1], k0, len, a.D);
-  }
+  const int rb = tile::row_base(col, h), cb = tile::col_base(lane);
+  dma_wait();
   for (int n = 0; n < tiles; ++n) {
-    const int k0 = (n < first ? n : from + n - first) * KT, k1 = k0 + KT - 1;
-    __syncthreads();
-    sk.store(Ks);
-    sv.store(Vs);
-    __syncthreads();
-    if (n + 1 < tiles) {
-      const int kn = (n + 1 < first ? n + 1 : from + n + 1 - first) * KT;
-      sk.load(K, a.sk[1], kn, len, a.D);
-      sv.load(V, a.sv[1], kn, len, a.D);
+    const unsigned char* Ks = win_smem + (n & 1) * 2 * TB;
+    const unsigned char* Vs = Ks + TB;
+    const int k0 = key_of(n), k1 = k0 + KT - 1;
+    if (n + 1 < tiles) {                                                 // into the other buffer: its readers passed the last barrier
+      unsigned char* next = win_smem + ((n + 1) & 1) * 2 * TB;
+      dma(K, a.sk[1], key_of(n + 1), len, next);
+      dma(V, a.sv[1], key_of(n + 1), len, next + TB);
     }
-    if (i0 >= a.Nq || k0 > w1 + a.right || (k1 < w0 - a.left && k0 >= a.sinks)) continue;
-    const bool all = k1 <= w0 + a.right && k1 < len && (k0 >= w1 - a.left || k1 < a.sinks);
+    if (i0 < a.Nq && k0 <= w1 + a.right && (k1 >= w0 - a.left || k0 < a.sinks)) {
+      const bool all = k1 <= w0 + a.right && k1 < len && (k0 >= w1 - a.left || k1 < a.sinks);
+      f32x16 st[NB], dp[NB];
 #pragma unroll
-    for (int x = 0; x < NB; ++x) {
-      f32x16 st = zero16(), dp = zero16();
+      for (int x = 0; x < NB; ++x) {
+        st[x] = zero16();
+        dp[x] = zero16();
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        st = mma(tile::row_frag(Ks, 32 * x + col, s, h), qf[s], st);
-        dp = mma(tile::row_frag(Vs, 32 * x + col, s, h), gf[s], dp);
+        for (int s = 0; s < DP / 16; ++s) {
+          st[x] = mma(tile::row_frag(Ks + 32 * x * tile::RB, rb, s), qf[s], st[x]);
+          dp[x] = mma(tile::row_frag(Vs + 32 * x * tile::RB, rb, s), gf[s], dp[x]);
+        }
       }
+      if (!all)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], a.sc, -lse)), ds = p * (dp[r] - delta);
-        st[r] = all || visible(a, len, t, k0 + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * h) ? ds : 0.f;
-      }
+        for (int x = 0; x < NB; ++x) mask_tile<true>(a, len, t, k0 + 32 * x, h, st[x]);
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const auto df = pack<T>(st, s2);
+      for (int x = 0; x < NB; ++x)
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) dq[db] = mma(tile::col_frag(Ks, 32 * x + 16 * s2, db, lane), df, dq[db]);
-      }
+        for (int r = 0; r < 16; ++r)
+          st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -lse)) * (dp[x][r] - delta);
+      const Cols<T, DP> kc(Ks, cb);                                      // dS to bf16: 2^-9 of each
+      add_product<T, DP, 0>(dq, kc, st[0]);
+      if constexpr (NB > 1) add_product<T, DP, 32 * tile::RB>(dq, kc, st[1]);
     }
+    dma_wait();
   }
   if (row < a.Nq) store_transposed<T, DP>((T*)a.dq + (((int64_t)b * a.Nq + row) * a.H + head) * a.D, dq, h, a.D, a.scale);
 }
 
 // ---------------------------------------------------------------------------
-// Backward, dK and dV: 4 waves of 32 keys each over common tiles of 32 rows, all query heads of the group in turn.
+// Backward, dK and dV: 8 waves over tiles of 64 rows, all query heads of the group in turn: 4 blocks of 32 keys, for each one wave
+// on the tile's first 32 rows and one on the others, added up at the end (there are too few blocks of keys to fill the chip with
+// 4 waves each).  The keys stay in registers as operands; rows of more than 128 bytes leave no room for the values beside them (two
+// waves a SIMD have 256 registers each, half of them hold the results), so these are read from LDS, where they stay too.
 // SINK: the rows far behind the window, which see the first 32-key blocks as sinks only.  There are as many of these rows as the
-// sequence is long and only a few keys, so the four waves take the SAME keys and a quarter of the rows each, the rows are cut
-// into chunks, and every wave leaves its share in fp32; win_bwd_join_kernel adds the shares in order.
+// sequence is long and only a few keys, so the waves take the SAME keys and 32 rows of a tile each, the rows are cut into
+// chunks, and every workgroup leaves its share in fp32; win_bwd_join_kernel adds the shares in order.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, bool SINK>
-__global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 2 : 1) void win_bwd_kv_kernel(const WinArgs a) {
-  constexpr int QT = SINK ? 128 : 32;
+struct KvPlan {
+  static constexpr int RB = Tile<T, DP>::RB;
+  static constexpr int SETS = SINK || RB > 256 ? 1 : 2;                  // waves per block of keys; 512-byte rows need a SIMD's registers for one
+  static constexpr int TH = 256 * SETS, QT = SINK ? (RB > 256 ? 64 : 128) : 32 * SETS, TB = QT * RB, LB = (QT < 64 ? 64 : QT) * 4;
+  static constexpr bool V_LDS = RB > 128;
+  static constexpr int KEYS = SINK ? 32 : 128;
+  static constexpr int VB = V_LDS ? KEYS * RB : 0;
+  static constexpr int ONE = 2 * TB + 2 * LB;                            // Q tile | dO tile | lse | delta
+  static constexpr int BUF = SINK ? 1 : 2;
+  static constexpr int JOIN = (SINK ? 2 : 4) * 32 * (DP + 4) * 4;        // fp32 results on their way from wave to wave
+  static constexpr int LDS = VB + BUF * ONE > JOIN ? VB + BUF * ONE : JOIN;
+  static_assert(LDS <= 160 * 1024 && BUF * ONE <= 128 * 1024, "LDS, and what LDS-DMA reaches of it");
+};
+template <typename T, int DP, bool SINK>
+__global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bwd_kv_kernel(const WinArgs a) {
+  typedef KvPlan<T, DP, SINK> plan;
+  constexpr int QT = plan::QT, TB = plan::TB, ONE = plan::ONE, LB = plan::LB, SETS = plan::SETS, TH = plan::TH;
   typedef Tile<T, DP> tile;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];
-  unsigned char* Qs = win_smem;
-  unsigned char* Gs = Qs + QT * tile::RB;
-  float* ls = reinterpret_cast<float*>(Gs + QT * tile::RB);
-  float* ds_ = ls + QT;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];      // [BUF][ONE] | values
+  unsigned char* bufs = win_smem;
+  unsigned char* Vs = win_smem + plan::BUF * ONE;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int group = a.H / a.Hk, shift = a.Nk - a.Nq, b = blockIdx.z;
+  const int group = a.H / a.Hk, shift = a.Nk - a.Nq;
   const int blocks = (a.sinks + 31) / 32;                                // of 32 first keys
-  const int kvh = SINK ? blockIdx.y / group : blockIdx.y;
+  int b, kvh, kb, item, chunk = 0;                                       // kb: first key of the workgroup
+  if constexpr (SINK) {
+    item = blockIdx.x;
+    kb = item % blocks * 32; item /= blocks;
+    chunk = item % a.far_chunks; item /= a.far_chunks;
+    b = item / a.H;
+    item %= a.H;                                                         // the query head
+    kvh = item / group;
+  } else {
+    const int tiles = (a.Nk + 127) / 128;
+    item = work_item(blockIdx.x, gridDim.x);
+    kb = item % tiles * 128; item /= tiles;
+    kvh = item % a.Hk;
+    b = item / a.Hk;
+  }
   const int len = length_of(a, b);
-  const int k0 = SINK ? (blockIdx.x % blocks) * 32 : blockIdx.x * 128 + wave * 32, key = k0 + col;
+  const int k0 = SINK ? kb : kb + (wave & 3) * 32, key = k0 + col;
+  const int sub = SINK ? wave * 32 : (wave >> 2) * 32;                   // this wave's rows of a tile
   const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + kvh * a.sk[2];
   const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + kvh * a.sv[2];
-  typename Types<T>::frag kf[DP / 16], vf[DP / 16];
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    kf[s] = global_frag(K, a.sk[1], key, len, 16 * s + 8 * h, a.D);
-    vf[s] = global_frag(V, a.sv[1], key, len, 16 * s + 8 * h, a.D);
-  }
-  f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db) { dk[db] = zero16(); dv[db] = zero16(); }
   // rows that this workgroup looks at
   int r0, r1;
   if constexpr (SINK) {
-    r0 = a.far + (blockIdx.x / blocks) * a.far_rows;
-    r1 = min(r0 + a.far_rows, a.Nq);
+    r0 = a.far + chunk * a.far_rows;
+    r1 = kb >= len ? 0 : min(r0 + a.far_rows, a.Nq);                     // no such key: nothing is read, the share is zeros
   } else {
-    const int kb = blockIdx.x * 128;
     r0 = max(kb - a.right - shift, 0) / QT * QT;
     r1 = kb >= len ? 0 : (int)min((int64_t)kb + 127 + a.left - shift + 1, (int64_t)a.Nq);
   }
   const int per = r1 > r0 ? (r1 - r0 + QT - 1) / QT : 0, total = SINK ? per : per * group;
   const int64_t so = (int64_t)a.H * a.D;
-  Stage<T, DP, QT> sq, sg;
-  float nl = INFINITY, nd = 0.f;
-  auto fetch = [&](int n) {
-    const int head = SINK ? (int)blockIdx.y : kvh * group + n / per, rr = r0 + (n % per) * QT;
-    sq.load((const T*)a.q + b * a.sq[0] + head * a.sq[2], a.sq[1], rr, a.Nq, a.D);
-    sg.load((const T*)a.dod + ((int64_t)b * a.Nq * a.H + head) * a.D, so, rr, a.Nq, a.D);
-    if (threadIdx.x < QT) {
-      const int i = rr + threadIdx.x;
-      const int64_t li = ((int64_t)b * a.H + head) * a.Nq + i;
-      nl = i < r1 ? a.lse[li] : INFINITY;                                // a row of no weight
-      nd = i < r1 ? a.delta[li] : 0.f;
+  const Dma<T, DP, QT, TH> dma(a.D);
+  const int wave_id = __builtin_amdgcn_readfirstlane(wave);
+  int fh = SINK ? item : kvh * group, fr = r0;                           // head and first row of the next tile
+  auto fetch = [&](unsigned char* m) {
+    dma((const T*)a.q + b * a.sq[0] + fh * a.sq[2], a.sq[1], fr, a.Nq, m);
+    dma((const T*)a.dod + ((int64_t)b * a.Nq * a.H + fh) * a.D, so, fr, a.Nq, m + TB);
+    // lse by the first wave(s), delta by the next; rows behind the last one are masked
+    if (wave_id < 2 * LB / 256) {
+      const int part = wave_id % (LB / 256);
+      const float* from = (wave_id < LB / 256 ? a.lse : a.delta) + ((int64_t)b * a.H + fh) * a.Nq;
+      __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + min(fr + part * 64 + lane, a.Nq - 1)), (lds_ptr_t)(m + 2 * TB + wave_id * 256), 4, 0, 0);
     }
+    fr += QT;
+    if (fr >= r1) { fr = r0; ++fh; }
   };
-  if (total > 0) fetch(0);
-  for (int n = 0; n < total; ++n) {
-    __syncthreads();
-    sq.store(Qs);
-    sg.store(Gs);
-    if (threadIdx.x < QT) { ls[threadIdx.x] = nl; ds_[threadIdx.x] = nd; }
-    __syncthreads();
-    if (n + 1 < total) fetch(n + 1);
-    const int sub = SINK ? wave * 32 : 0, t0 = r0 + (n % per) * QT + sub + shift, t1 = t0 + 31;
-    if (k0 > t1 + a.right || (k0 + 31 < t0 - a.left && k0 >= a.sinks) || k0 >= len) continue;
-    const bool all = k0 + 31 <= t0 + a.right && k0 + 31 < len && (k0 >= t1 - a.left || k0 + 31 < a.sinks);
-    f32x16 st = zero16(), dp = zero16();
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      st = mma(tile::row_frag(Qs, sub + col, s, h), kf[s], st);
-      dp = mma(tile::row_frag(Gs, sub + col, s, h), vf[s], dp);
-    }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 L4 = *reinterpret_cast<const f32x4*>(ls + sub + 8 * g + 4 * h), D4 = *reinterpret_cast<const f32x4*>(ds_ + sub + 8 * g + 4 * h);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * g + e;
-        const bool on = all || visible(a, len, t0 + 8 * g + 4 * h + e, key);
-        const float p = on ? __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], a.sc, -L4[e])) : 0.f;
-        dp[r] = on ? p * (dp[r] - D4[e]) : 0.f;
-        st[r] = p;
+  if (total > 0) {
+    if constexpr (!SINK) fetch(bufs);
+    // through registers: LDS-DMA does not reach behind 128 KB.  Zeros behind the last key and behind D
+    if constexpr (plan::V_LDS)
+#pragma unroll 4
+      for (int e = threadIdx.x; e < plan::KEYS * tile::CPR; e += TH) {
+        const int r = e / tile::CPR, c = e % tile::CPR * tile::EPC;
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (kb + r < len && c < a.D) x = *reinterpret_cast<const u32x4*>(V + (kb + r) * a.sv[1] + c);
+        *reinterpret_cast<u32x4*>(Vs + tile::at(r, c / tile::EPC)) = x;
       }
-    }
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const auto pf = pack<T>(st, s2);
-      const auto df = pack<T>(dp, s2);
-#pragma unroll
-      for (int db = 0; db < DP / 32; ++db) {
-        dv[db] = mma(tile::col_frag(Gs, sub + 16 * s2, db, lane), pf, dv[db]);
-        dk[db] = mma(tile::col_frag(Qs, sub + 16 * s2, db, lane), df, dk[db]);
-      }
-    }
   }
+  typename Types<T>::frag kf[DP / 16], vf[plan::V_LDS ? 1 : DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    kf[s] = global_frag(K, a.sk[1], key, len, 16 * s + 8 * h, a.D);
+    if constexpr (!plan::V_LDS) vf[s] = global_frag(V, a.sv[1], key, len, 16 * s + 8 * h, a.D);
+  }
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) { dk[db] = zero16(); dv[db] = zero16(); }
+  const int rb = tile::row_base(col, h), cb = tile::col_base(lane);
+  const unsigned char* Vw = Vs + (SINK ? 0 : (wave & 3) * 32 * tile::RB);
+  if constexpr (!SINK) dma_wait();
+  int cr = r0;                                                           // first row of the current tile
+  for (int n = 0; n < total; ++n) {
+    if constexpr (SINK) {                                                // few tiles: one buffer, and two workgroups on a CU
+      fetch(bufs);
+      dma_wait();
+    }
+    const int t0 = cr + sub + shift, t1 = t0 + 31;
+    cr = cr + QT >= r1 ? r0 : cr + QT;
+    const unsigned char* Qs = bufs + (SINK ? 0 : (n & 1) * ONE) + sub * tile::RB;
+    const unsigned char* Gs = Qs + TB;
+    const float* ls = reinterpret_cast<const float*>(bufs + (SINK ? 0 : (n & 1) * ONE) + 2 * TB) + sub;
+    if (!SINK && n + 1 < total) fetch(bufs + ((n + 1) & 1) * ONE);
+    if (sub < QT && k0 <= t1 + a.right && (k0 + 31 >= t0 - a.left || k0 < a.sinks) && k0 < len) {
+      const bool all = k0 + 31 <= t0 + a.right && k0 + 31 < len && (k0 >= t1 - a.left || k0 + 31 < a.sinks) && t1 - shift < r1;
+      f32x16 st = zero16(), dp = zero16();
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        st = mma(tile::row_frag(Qs, rb, s), kf[s], st);
+        if constexpr (plan::V_LDS) dp = mma(tile::row_frag(Gs, rb, s), tile::row_frag(Vw, rb, s), dp);
+        else dp = mma(tile::row_frag(Gs, rb, s), vf[s], dp);
+      }
+      if (!all) mask_tile<false>(a, len, t0, key, h, st, r1 - 1 + shift);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 L4 = *reinterpret_cast<const f32x4*>(ls + 8 * g + 4 * h), D4 = *reinterpret_cast<const f32x4*>(ls + LB / 4 + 8 * g + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          st[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], a.sc, -L4[e]));
+          dp[r] = st[r] * (dp[r] - D4[e]);
+        }
+      }
+      add_product<T, DP, 0>(dv, Cols<T, DP>(Gs, cb), st);
+      add_product<T, DP, 0>(dk, Cols<T, DP>(Qs, cb), dp);
+    }
+    if constexpr (SINK) __syncthreads();
+    else dma_wait();
+  }
+  // the waves of one block of keys, one after the other (behind the last barrier the tiles are free)
+  float* join = reinterpret_cast<float*>(win_smem);
+  constexpr int JW = DP + 4;                                             // words of a key's row: 16-byte pieces of 32 rows on different banks
+  auto pass = [&](f32x16 (&x)[DP / 32], float* m, bool put) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4* p = reinterpret_cast<f32x4*>(m + col * JW + db * 32 + 8 * g + 4 * h);
+        if (put) *p = f32x4{x[db][4 * g], x[db][4 * g + 1], x[db][4 * g + 2], x[db][4 * g + 3]};
+        else {
+          const f32x4 y = *p;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[db][4 * g + e] += y[e];
+        }
+      }
+  };
   if constexpr (SINK) {
-    if (key >= a.sinks) return;
+#pragma unroll 1
+    for (int w = 4 * SETS - 1; w > 0; --w) {                                        // wave w hands its sums to wave w - 1
+      if (wave == w) { pass(dk, join, true); pass(dv, join + 32 * JW, true); }
+      __syncthreads();
+      if (wave == w - 1) { pass(dk, join, false); pass(dv, join + 32 * JW, false); }
+      __syncthreads();
+    }
+    if (wave || key >= a.sinks) return;
     // share [slot][b][kvh][2][sinks][D]; slot 0 is the window's part
-    const int slot = 1 + ((blockIdx.x / blocks) * group + blockIdx.y % group) * 4 + wave;
+    const int slot = 1 + chunk * group + item % group;
     float* out = a.part + ((((int64_t)slot * a.B + b) * a.Hk + kvh) * 2 * a.sinks + key) * a.D;
     store_transposed<float, DP>(out, dk, h, a.D, a.scale);
     store_transposed<float, DP>(out + (int64_t)a.sinks * a.D, dv, h, a.D, 1.f);
   } else {
+    if constexpr (SETS == 2) {
+      float* mine = join + (wave & 3) * 32 * JW;
+      if (wave >= 4) pass(dk, mine, true);
+      __syncthreads();
+      if (wave < 4) pass(dk, mine, false);
+      __syncthreads();
+      if (wave >= 4) pass(dv, mine, true);
+      __syncthreads();
+      if (wave >= 4) return;
+      pass(dv, mine, false);
+    }
     if (key >= a.Nk) return;
     if (a.part && key < a.sinks) {
       float* out = a.part + (((int64_t)b * a.Hk + kvh) * 2 * a.sinks + key) * a.D;
       store_transposed<float, DP>(out, dk, h, a.D, a.scale);
       store_transposed<float, DP>(out + (int64_t)a.sinks * a.D, dv, h, a.D, 1.f);
     } else {
-      const int64_t at = (((int64_t)b * a.Nk + key) * a.Hk + kvh) * a.D;
-      store_transposed<T, DP>((T*)a.dk + at, dk, h, a.D, a.scale);
-      store_transposed<T, DP>((T*)a.dv + at, dv, h, a.D, 1.f);
+      const int64_t to = (((int64_t)b * a.Nk + key) * a.Hk + kvh) * a.D;
+      store_transposed<T, DP>((T*)a.dk + to, dk, h, a.D, a.scale);
+      store_transposed<T, DP>((T*)a.dv + to, dv, h, a.D, 1.f);
     }
   }
 }
 
-// the first keys' gradients: the shares in order
+// the first keys' gradients: 16 values a workgroup, each the sum of 16 runs of the shares
 template <typename T>
 __global__ __launch_bounds__(256) void win_bwd_join_kernel(const WinArgs a, int slots) {
-  const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sinks * a.D, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
+  const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sinks * a.D, i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+  __shared__ float red[16][16];
   float s = 0.f;
+  if (i < n) {
 #pragma unroll 8
-  for (int k = 0; k < slots; ++k) s += a.part[k * n + i];
+    for (int k = threadIdx.x >> 4; k < slots; k += 16) s += a.part[k * n + i];
+  }
+  red[threadIdx.x >> 4][threadIdx.x & 15] = s;
+  __syncthreads();
+  if (threadIdx.x >= 16 || i >= n) return;
+  s = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) s += red[k][threadIdx.x];
   int64_t r = i;
   const int d = (int)(r % a.D); r /= a.D;
   const int key = (int)(r % a.sinks); r /= a.sinks;
@@ -655,6 +870,7 @@ static int check_win(const char* who, int B, int Nq, int Nk, int H, int Hk, int 
   PT_CHECK(B >= 1 && B <= 65535 && Nq >= 1 && Nk >= Nq && Nk <= WIN_MAX, "%s: %d sequences of %d rows and %d keys", who, B, Nq, Nk);
   PT_CHECK(H >= 1 && H <= 65535 && Hk >= 1 && H % Hk == 0, "%s: %d query heads over %d key heads", who, H, Hk);
   PT_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "%s: head dimension %d (a multiple of 8 up to 128)", who, D);
+  PT_CHECK((int64_t)((Nk + 127) / 128) * H * B < (1 << 28), "%s: too many rows and heads", who);
   PT_CHECK(left >= -1 && right >= -1 && sinks >= 0 && sinks <= 128, "%s: window of %d left, %d right, %d first keys (up to 128)", who, left, right, sinks);
   PT_CHECK(scale > 0.f && scale < INFINITY && (dtype == 0 || dtype == 1), "%s: scale %g, dtype %d", who, scale, dtype);
   return 0;
@@ -665,6 +881,12 @@ static bool aligned16(const void* p, const int64_t* s, int n, int dtype) {
   bool ok = !((uintptr_t)p & 15);
   for (int i = 0; i < n; ++i) ok = ok && s[i] % v == 0;
   return ok;
+}
+// a tile's rows are addressed by 32-bit offsets from its first
+static bool near_rows(const int64_t* s) {
+  for (int i = 0; i < 9; i += 3)
+    if (s[i + 1] < 0 || s[i + 1] > (1 << 20)) return false;
+  return true;
 }
 static WinArgs win_args(const void* q, const void* k, const void* v, const int64_t* st, const int* lengths, int B, int Nq, int Nk, int H, int Hk, int D,
                         int left, int right, int sinks, float scale) {
@@ -680,28 +902,34 @@ static WinArgs win_args(const void* q, const void* k, const void* v, const int64
   const int64_t far = std::max<int64_t>((int64_t)128 + a.left - (Nk - Nq), 0);
   if (a.sinks > 0 && far < Nq) {
     a.far = (int)far;
-    const int rows = Nq - a.far, want = std::max(1, 1024 / (B * H));       // about four workgroups per CU
-    a.far_rows = std::max(512, ((rows + want - 1) / want + 127) / 128 * 128);
+    const int rows = Nq - a.far, want = std::max(1, 1024 / (B * H));       // about four workgroups per CU, a tile of 256 rows each at least
+    a.far_rows = std::max(256, ((rows + want - 1) / want + 255) / 256 * 256);
     a.far_chunks = (rows + a.far_rows - 1) / a.far_rows;
   }
   return a;
 }
 
+static int64_t win_blocks(const WinArgs& a) { return (int64_t)((a.Nq + 127) / 128) * a.H * a.B; }
+
 template <typename T, int DP>
 static int run_win_fwd(const WinArgs& a, hipStream_t s) {
-  PT_LAUNCH((win_fwd_kernel<T, DP>), dim3((a.Nq + 127) / 128, a.H, a.B), dim3(256), 0, s, a);
+  constexpr int lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB;
+  PT_ENSURE_LDS((win_fwd_kernel<T, DP>), lds);
+  PT_LAUNCH((win_fwd_kernel<T, DP>), dim3((unsigned)win_blocks(a)), dim3(256), lds, s, a);
   return 0;
 }
 template <typename T, int DP>
 static int run_win_bwd(const WinArgs& a, hipStream_t s) {
-  constexpr int lds = 2 * 32 * Tile<T, DP>::RB + 2 * 32 * 4, lds_sink = 2 * 128 * Tile<T, DP>::RB + 2 * 128 * 4;
-  PT_LAUNCH((win_bwd_q_kernel<T, DP>), dim3((a.Nq + 127) / 128, a.H, a.B), dim3(256), 0, s, a);
-  PT_LAUNCH((win_bwd_kv_kernel<T, DP, false>), dim3((a.Nk + 127) / 128, a.Hk, a.B), dim3(256), lds, s, a);
+  constexpr int lds = 4 * key_tile_q<T, DP>() * Tile<T, DP>::RB, lds_kv = KvPlan<T, DP, false>::LDS, lds_sink = KvPlan<T, DP, true>::LDS;
+  PT_ENSURE_LDS((win_bwd_q_kernel<T, DP>), lds);
+  PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false>), lds_kv);
+  PT_LAUNCH((win_bwd_q_kernel<T, DP>), dim3((unsigned)win_blocks(a)), dim3(256), lds, s, a);
+  PT_LAUNCH((win_bwd_kv_kernel<T, DP, false>), dim3((unsigned)((a.Nk + 127) / 128) * a.Hk * a.B), dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
   if (a.far_chunks) {
     PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, true>), lds_sink);
-    PT_LAUNCH((win_bwd_kv_kernel<T, DP, true>), dim3((a.sinks + 31) / 32 * a.far_chunks, a.H, a.B), dim3(256), lds_sink, s, a);
+    PT_LAUNCH((win_bwd_kv_kernel<T, DP, true>), dim3((unsigned)((a.sinks + 31) / 32 * a.far_chunks) * a.H * a.B), dim3(KvPlan<T, DP, true>::TH), lds_sink, s, a);
     const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sinks * a.D;
-    PT_LAUNCH(win_bwd_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, 1 + a.far_chunks * (a.H / a.Hk) * 4);
+    PT_LAUNCH(win_bwd_join_kernel<T>, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, a, 1 + a.far_chunks * (a.H / a.Hk));
   }
   return 0;
 }
@@ -712,6 +940,7 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* o, floa
   PT_CHECK(q && k && v && o && st, "attention_window_fwd: null argument");
   PT_CHECK(aligned16(q, st, 3, dtype) && aligned16(k, st + 3, 3, dtype) && aligned16(v, st + 6, 3, dtype) && !((uintptr_t)o & 15),
            "attention_window_fwd: addresses and strides must be multiples of 16 bytes");
+  PT_CHECK(near_rows(st) && (int64_t)H * D <= (1 << 20), "attention_window_fwd: rows are more than 2^20 values apart");
   const WinArgs w = win_args(q, k, v, st, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale);
   WinArgs a = w;
   a.o = o; a.lse = lse;
@@ -724,7 +953,7 @@ size_t window_bwd_workspace(int B, int Nq, int Nk, int H, int Hk, int D, int lef
   const int64_t st[9] = {};
   const WinArgs a = win_args(nullptr, nullptr, nullptr, st, nullptr, B, Nq, Nk, H, Hk, D, left, right, sinks, 1.f);
   const size_t delta = ((size_t)B * H * Nq * 4 + 255) / 256 * 256;
-  return delta + (a.far_chunks ? (size_t)(1 + a.far_chunks * (H / Hk) * 4) * B * Hk * 2 * a.sinks * D * 4 : 0);
+  return delta + (a.far_chunks ? (size_t)(1 + a.far_chunks * (H / Hk)) * B * Hk * 2 * a.sinks * D * 4 : 0);
 }
 
 int launch_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv,
@@ -735,6 +964,7 @@ int launch_window_bwd(const void* q, const void* k, const void* v, const void* o
   PT_CHECK(aligned16(q, st, 3, dtype) && aligned16(k, st + 3, 3, dtype) && aligned16(v, st + 6, 3, dtype) &&
                !(((uintptr_t)o | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15),
            "attention_window_bwd: addresses and strides must be multiples of 16 bytes");
+  PT_CHECK(near_rows(st) && (int64_t)H * D <= (1 << 20), "attention_window_bwd: rows are more than 2^20 values apart");
   const size_t need = window_bwd_workspace(B, Nq, Nk, H, Hk, D, left, right, sinks);
   PT_CHECK(ws_bytes >= need, "attention_window_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
   WinArgs a = win_args(q, k, v, st, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale);

@@ -420,7 +420,8 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
     if k.shape[1] < q.shape[1]:
         raise RuntimeError(f"window_attention: {q.shape[1]} rows for {k.shape[1]} keys")
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    return WindowAttention.apply(_vectors(q), _vectors(k), _vectors(v), lengths, *args, grad)
+    q, k, v = (_vectors(t if t.shape[1] == 1 or 0 <= t.stride(1) <= 1 << 20 else t.contiguous()) for t in (q, k, v))
+    return WindowAttention.apply(q, k, v, lengths, *args, grad)
 
 
 def window_attention_step(q, k, v, lengths, left=None, sinks=0, scale=None):
