@@ -194,10 +194,8 @@ struct Cols<float, DP> {
   }
 };
 // acc[db] += (columns of 32 rows)^T . p, p the registers of a score tile over these rows
-template <typename T, int DP, int OFF>
-__device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const Cols<T, DP>& cols, const f32x16& p) {
-  typename Types<T>::frag f[2][DP / 32];
-  cols.template read<OFF>(f);
+template <typename T, int DP>
+__device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const typename Types<T>::frag (&f)[2][DP / 32], const f32x16& p) {
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
     typename Types<T>::frag x;
@@ -217,32 +215,48 @@ struct Dma {
   typedef Tile<T, DP> tile;
   static constexpr int RB = tile::RB, W = TH / 64, ROWS = W * 1024 / RB, N = R / ROWS;     // rows per turn of all waves, turns
   static_assert(N >= 1 && R % ROWS == 0, "tile too small for the workgroup");
-  int row, col[2];                                       // row and column of this lane in the first turn (and in odd turns of 8 rows)
-  __device__ __forceinline__ Dma(int D) {
+  int row, col[2];                                       // row and first byte of this lane in the first turn (and in odd turns of 8 rows)
+  unsigned off[2];
+  int64_t stride;                                        // bytes of a row
+  __device__ __forceinline__ Dma(int D, int64_t stride_) : stride(stride_ * (int64_t)sizeof(T)) {
     const int byte = threadIdx.x * 16;
     row = byte / RB;
-    const int chunk = (byte % RB / 16) ^ tile::swz(row);
-    col[0] = chunk * tile::EPC < D ? chunk * tile::EPC : 0;
-    col[1] = (chunk ^ tile::swz(ROWS)) * tile::EPC < D ? (chunk ^ tile::swz(ROWS)) * tile::EPC : 0;
+    const int chunk = (byte % RB / 16) ^ tile::swz(row), odd = chunk ^ tile::swz(ROWS);
+    col[0] = chunk * tile::EPC < D ? chunk * 16 : 0;
+    col[1] = odd * tile::EPC < D ? odd * 16 : 0;
+    off[0] = (unsigned)(row * (int)stride + col[0]);
+    off[1] = (unsigned)(row * (int)stride + col[1]);
   }
-  __device__ __forceinline__ void operator()(const T* __restrict__ base, int64_t stride, int row0, int limit, unsigned char* m) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), st = (int)stride, last = limit - 1 - row0;   // row0 < limit
-    base += row0 * stride;
+  // rows row0 .. row0 + R - 1 of base, row0 < limit
+  __device__ __forceinline__ void operator()(const T* __restrict__ base, int row0, int limit, unsigned char* m) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), last = limit - 1 - row0;
+    const char* from = reinterpret_cast<const char*>(base) + row0 * stride;
+    if (R - 1 <= last) {                                 // a whole tile: uniform address, a lane's offset that stays the same
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = col[ROWS % 16 ? i & 1 : 0];
-      unsigned off;
-      const T* from = base;
-      if (R - 1 <= last) {                               // uniform: a whole tile
-        off = (unsigned)(row * st + c);
-        from += (int64_t)i * ROWS * st;
-      } else {
-        off = (unsigned)(min(row + i * ROWS, last) * st + c);
+      for (int i = 0; i < N; ++i) {
+        const unsigned o = off[ROWS % 16 ? i & 1 : 0];
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + i * ROWS * stride + o), (lds_ptr_t)(m + (i * W + wave) * 1024), 16, 0, 0);
       }
-      __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + off), (lds_ptr_t)(m + (i * W + wave) * 1024), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + (min(row + i * ROWS, last) * (int)stride + col[ROWS % 16 ? i & 1 : 0])),
+                                         (lds_ptr_t)(m + (i * W + wave) * 1024), 16, 0, 0);
+      asm volatile("");                                  // keeps the two apart: merged, every tile pays for the last one's arithmetic
     }
   }
 };
+// The order of a block of products with their operands from LDS: P reads ahead, then R reads with each M products.  Left to itself the
+// compiler reads an operand, waits for it, multiplies, and reads the next.
+template <int P, int R, int M, int PRODUCTS>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, P, 0);
+#pragma unroll
+  for (int i = 0; i < PRODUCTS / M; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+}
 // loads to LDS of this wave have arrived; the barrier behind it says so of all waves
 __device__ __forceinline__ void dma_wait() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -320,10 +334,11 @@ template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 2 |
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fwd_kernel(const WinArgs a) {
   constexpr int KT = key_tile<T, DP>(), NB = KT / 32;
+  constexpr bool BF = sizeof(T) == 2;
   typedef Tile<T, DP> tile;
   constexpr int TB = KT * tile::RB;
   extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];      // [2][K tile | V tile]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
   const Place at = place(a, (a.Nq + 127) / 128);
   const int head = at.head, b = at.b, i00 = at.tile * 128;
   const int len = length_of(a, b), shift = a.Nk - a.Nq;
@@ -335,10 +350,10 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
   key_tiles<KT>(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift, first, from, to);
   const int tiles = first + (to - from);
   auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
-  const Dma<T, DP, KT, 256> dma(a.D);
+  const Dma<T, DP, KT, 256> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
   if (tiles > 0) {
-    dma(K, a.sk[1], key_of(0), len, win_smem);
-    dma(V, a.sv[1], key_of(0), len, win_smem + TB);
+    dma_k(K, key_of(0), len, win_smem);
+    dma_v(V, key_of(0), len, win_smem + TB);
   }
   typename Types<T>::frag qf[DP / 16];
 #pragma unroll
@@ -356,8 +371,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
     const int k0 = key_of(n), k1 = k0 + KT - 1;
     if (n + 1 < tiles) {                                                 // into the other buffer: its readers passed the last barrier
       unsigned char* next = win_smem + ((n + 1) & 1) * 2 * TB;
-      dma(K, a.sk[1], key_of(n + 1), len, next);
-      dma(V, a.sv[1], key_of(n + 1), len, next + TB);
+      dma_k(K, key_of(n + 1), len, next);
+      dma_v(V, key_of(n + 1), len, next + TB);
     }
     if (i0 < a.Nq && k0 <= w1 + a.right && (k1 >= w0 - a.left || k0 < a.sinks)) {
       f32x16 st[NB];
@@ -366,6 +381,14 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
         st[x] = zero16();
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) st[x] = mma(tile::row_frag(Ks + 32 * x * tile::RB, rb, s), qf[s], st[x]);
+      }
+      if constexpr (BF) reads_ahead<6, 1, 1, NB * DP / 16>(); else reads_ahead<4, 2, 8, NB * DP / 2>();
+      // bf16: the values' columns are on their way while the matrix cores finish the scores
+      typename Types<T>::frag vf[NB][2][DP / 32];
+      const Cols<T, DP> vc(Vs, cb);
+      if constexpr (BF) {
+        vc.template read<0>(vf[0]);
+        vc.template read<32 * tile::RB>(vf[1]);
       }
       if (!(k1 <= w0 + a.right && k1 < len && (k0 >= w1 - a.left || k1 < a.sinks)))
 #pragma unroll
@@ -393,9 +416,12 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
         for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-      const Cols<T, DP> vc(Vs, cb);                                      // probabilities in [0, 1] to bf16: 2^-9 of each
-      add_product<T, DP, 0>(o, vc, st[0]);
-      if constexpr (NB > 1) add_product<T, DP, 32 * tile::RB>(o, vc, st[1]);
+      if constexpr (!BF) vc.template read<0>(vf[0]);
+      add_product<T, DP>(o, vf[0], st[0]);                               // probabilities in [0, 1] to bf16: 2^-9 of each
+      if constexpr (NB > 1) {
+        if constexpr (!BF) vc.template read<32 * tile::RB>(vf[1]);
+        add_product<T, DP>(o, vf[1], st[1]);
+      }
     }
     dma_wait();
   }
@@ -412,10 +438,11 @@ template <typename T, int DP> constexpr int key_tile_q() { return sizeof(T) * DP
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bwd_q_kernel(const WinArgs a) {
   constexpr int KT = key_tile_q<T, DP>(), NB = KT / 32;
+  constexpr bool BF = sizeof(T) == 2;
   typedef Tile<T, DP> tile;
   constexpr int TB = KT * tile::RB;
   extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
   const Place at = place(a, (a.Nq + 127) / 128);
   const int head = at.head, b = at.b, i00 = at.tile * 128;
   const int len = length_of(a, b), shift = a.Nk - a.Nq;
@@ -428,10 +455,10 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
   key_tiles<KT>(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift, first, from, to);
   const int tiles = first + (to - from);
   auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
-  const Dma<T, DP, KT, 256> dma(a.D);
+  const Dma<T, DP, KT, 256> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
   if (tiles > 0) {
-    dma(K, a.sk[1], key_of(0), len, win_smem);
-    dma(V, a.sv[1], key_of(0), len, win_smem + TB);
+    dma_k(K, key_of(0), len, win_smem);
+    dma_v(V, key_of(0), len, win_smem + TB);
   }
   typename Types<T>::frag qf[DP / 16], gf[DP / 16];
   float delta = 0.f;
@@ -460,8 +487,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
     const int k0 = key_of(n), k1 = k0 + KT - 1;
     if (n + 1 < tiles) {                                                 // into the other buffer: its readers passed the last barrier
       unsigned char* next = win_smem + ((n + 1) & 1) * 2 * TB;
-      dma(K, a.sk[1], key_of(n + 1), len, next);
-      dma(V, a.sv[1], key_of(n + 1), len, next + TB);
+      dma_k(K, key_of(n + 1), len, next);
+      dma_v(V, key_of(n + 1), len, next + TB);
     }
     if (i0 < a.Nq && k0 <= w1 + a.right && (k1 >= w0 - a.left || k0 < a.sinks)) {
       const bool all = k1 <= w0 + a.right && k1 < len && (k0 >= w1 - a.left || k1 < a.sinks);
@@ -476,6 +503,13 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
           dp[x] = mma(tile::row_frag(Vs + 32 * x * tile::RB, rb, s), gf[s], dp[x]);
         }
       }
+      if constexpr (BF) reads_ahead<6, 1, 1, NB * DP / 8>(); else reads_ahead<4, 2, 8, NB * DP>();
+      typename Types<T>::frag kf[NB][2][DP / 32];
+      const Cols<T, DP> kc(Ks, cb);
+      if constexpr (BF) {
+        kc.template read<0>(kf[0]);
+        if constexpr (NB > 1) kc.template read<32 * tile::RB>(kf[NB - 1]);
+      }
       if (!all)
 #pragma unroll
         for (int x = 0; x < NB; ++x) mask_tile<true>(a, len, t, k0 + 32 * x, h, st[x]);
@@ -484,9 +518,12 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -lse)) * (dp[x][r] - delta);
-      const Cols<T, DP> kc(Ks, cb);                                      // dS to bf16: 2^-9 of each
-      add_product<T, DP, 0>(dq, kc, st[0]);
-      if constexpr (NB > 1) add_product<T, DP, 32 * tile::RB>(dq, kc, st[1]);
+      if constexpr (!BF) kc.template read<0>(kf[0]);
+      add_product<T, DP>(dq, kf[0], st[0]);                              // dS to bf16: 2^-9 of each
+      if constexpr (NB > 1) {
+        if constexpr (!BF) kc.template read<32 * tile::RB>(kf[NB - 1]);
+        add_product<T, DP>(dq, kf[NB - 1], st[NB - 1]);
+      }
     }
     dma_wait();
   }
@@ -519,12 +556,13 @@ struct KvPlan {
 template <typename T, int DP, bool SINK>
 __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bwd_kv_kernel(const WinArgs a) {
   typedef KvPlan<T, DP, SINK> plan;
+  constexpr bool BF = sizeof(T) == 2;
   constexpr int QT = plan::QT, TB = plan::TB, ONE = plan::ONE, LB = plan::LB, SETS = plan::SETS, TH = plan::TH;
   typedef Tile<T, DP> tile;
   extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];      // [BUF][ONE] | values
   unsigned char* bufs = win_smem;
   unsigned char* Vs = win_smem + plan::BUF * ONE;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
   const int group = a.H / a.Hk, shift = a.Nk - a.Nq;
   const int blocks = (a.sinks + 31) / 32;                                // of 32 first keys
   int b, kvh, kb, item, chunk = 0;                                       // kb: first key of the workgroup
@@ -558,17 +596,16 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
   }
   const int per = r1 > r0 ? (r1 - r0 + QT - 1) / QT : 0, total = SINK ? per : per * group;
   const int64_t so = (int64_t)a.H * a.D;
-  const Dma<T, DP, QT, TH> dma(a.D);
-  const int wave_id = __builtin_amdgcn_readfirstlane(wave);
+  const Dma<T, DP, QT, TH> dma_q(a.D, a.sq[1]), dma_g(a.D, so);
   int fh = SINK ? item : kvh * group, fr = r0;                           // head and first row of the next tile
   auto fetch = [&](unsigned char* m) {
-    dma((const T*)a.q + b * a.sq[0] + fh * a.sq[2], a.sq[1], fr, a.Nq, m);
-    dma((const T*)a.dod + ((int64_t)b * a.Nq * a.H + fh) * a.D, so, fr, a.Nq, m + TB);
+    dma_q((const T*)a.q + b * a.sq[0] + fh * a.sq[2], fr, a.Nq, m);
+    dma_g((const T*)a.dod + ((int64_t)b * a.Nq * a.H + fh) * a.D, fr, a.Nq, m + TB);
     // lse by the first wave(s), delta by the next; rows behind the last one are masked
-    if (wave_id < 2 * LB / 256) {
-      const int part = wave_id % (LB / 256);
-      const float* from = (wave_id < LB / 256 ? a.lse : a.delta) + ((int64_t)b * a.H + fh) * a.Nq;
-      __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + min(fr + part * 64 + lane, a.Nq - 1)), (lds_ptr_t)(m + 2 * TB + wave_id * 256), 4, 0, 0);
+    if (wave < 2 * LB / 256) {
+      const int part = wave % (LB / 256);
+      const float* from = (wave < LB / 256 ? a.lse : a.delta) + ((int64_t)b * a.H + fh) * a.Nq;
+      __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + min(fr + part * 64 + lane, a.Nq - 1)), (lds_ptr_t)(m + 2 * TB + wave * 256), 4, 0, 0);
     }
     fr += QT;
     if (fr >= r1) { fr = r0; ++fh; }
@@ -618,6 +655,10 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
         if constexpr (plan::V_LDS) dp = mma(tile::row_frag(Gs, rb, s), tile::row_frag(Vw, rb, s), dp);
         else dp = mma(tile::row_frag(Gs, rb, s), vf[s], dp);
       }
+      constexpr int READS = plan::V_LDS ? 3 : 2;                         // for two products
+      if constexpr (BF) reads_ahead<2 * READS, READS, 2, DP / 8>(); else reads_ahead<2 * READS, READS * 2, 16, DP>();
+      typename Types<T>::frag f[2][DP / 32];
+      if constexpr (BF) Cols<T, DP>(Gs, cb).template read<0>(f);
       if (!all) mask_tile<false>(a, len, t0, key, h, st, r1 - 1 + shift);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -629,8 +670,10 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
           dp[r] = st[r] * (dp[r] - D4[e]);
         }
       }
-      add_product<T, DP, 0>(dv, Cols<T, DP>(Gs, cb), st);
-      add_product<T, DP, 0>(dk, Cols<T, DP>(Qs, cb), dp);
+      if constexpr (!BF) Cols<T, DP>(Gs, cb).template read<0>(f);
+      add_product<T, DP>(dv, f, st);
+      Cols<T, DP>(Qs, cb).template read<0>(f);
+      add_product<T, DP>(dk, f, dp);
     }
     if constexpr (SINK) __syncthreads();
     else dma_wait();
