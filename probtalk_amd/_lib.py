@@ -162,8 +162,14 @@ def ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+# the current stream's handle without a torch.cuda.Stream object around it (3 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    if _raw_stream is None:
+        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return C.c_void_p(_raw_stream(torch.cuda.current_device()))
 
 
 def dev_f32(t, device=None):

@@ -86,32 +86,46 @@ __device__ __forceinline__ int column(int i) {
 
 __device__ __forceinline__ unsigned short to_bf16(float x) { return __builtin_bit_cast(unsigned short, (__bf16)x); }
 
+// a lane's values of a row as they lie in memory: what is loaded ahead waits in half the registers where it is bf16
 template <typename T, int WPR, bool VEC>
-__device__ __forceinline__ void load_row(const T* __restrict__ p, int cols, float (&v)[PER]) {
-  constexpr int V = 16 / sizeof(T);
+struct Raw {
+  static constexpr int V = 16 / (int)sizeof(T), N = PER / V;
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 x[N];
+  __device__ __forceinline__ void load(const T* __restrict__ p, int cols) {
 #pragma unroll
-  for (int c = 0; c < PER / V; ++c) {
-    const int c0 = column<T, WPR>(c * V);
-    if constexpr (VEC) {
-      if constexpr (V == 4) {
-        f32x4 q = {0.f, 0.f, 0.f, 0.f};
-        if (c0 < cols) q = *reinterpret_cast<const f32x4*>(p + c0);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[c * V + j] = q[j];
+    for (int c = 0; c < N; ++c) {
+      const int c0 = column<T, WPR>(c * V);
+      if constexpr (VEC) {
+        // lanes behind the last column read the last ones again: nothing they compute is summed up or stored, and a load without
+        // a branch is one that nobody waits for before its value is needed
+        x[c] = *reinterpret_cast<const u32x4*>(p + min(c0, cols - V));
       } else {
-        u16x8 q = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (c0 < cols) q = *reinterpret_cast<const u16x8*>(p + c0);
+        x[c] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[c * V + j] = __uint_as_float((unsigned)q[j] << 16);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if constexpr (V == 4) v[c * V + j] = c0 + j < cols ? p[c0 + j] : 0.f;
-        else v[c * V + j] = c0 + j < cols ? __uint_as_float((unsigned)p[c0 + j] << 16) : 0.f;
+        for (int j = 0; j < V; ++j)
+          if (c0 + j < cols) {
+            if constexpr (V == 4) x[c][j] = __float_as_uint(p[c0 + j]);
+            else x[c][j / 2] |= (unsigned)p[c0 + j] << (16 * (j & 1));
+          }
       }
     }
   }
+  __device__ __forceinline__ void get(float (&v)[PER]) const {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if constexpr (V == 4) { const unsigned u = x[c][j]; v[c * V + j] = __uint_as_float(u); }
+        else { const unsigned u = x[c][j / 2]; v[c * V + j] = __uint_as_float(j & 1 ? u & 0xFFFF0000u : u << 16); }
+      }
+  }
+};
+template <typename T, int WPR, bool VEC>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, int cols, float (&v)[PER]) {
+  Raw<T, WPR, VEC> r;
+  r.load(p, cols);
+  r.get(v);
 }
 template <typename T, int WPR, bool VEC>
 __device__ __forceinline__ void store_row(T* __restrict__ p, int cols, const float (&v)[PER]) {
@@ -171,7 +185,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[PER], int cols, float
   if constexpr (LAYER) {
     float s = 0.f, z = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s += v[i];
+    for (int i = 0; i < PER; ++i) s += column<T, WPR>(i) < cols ? v[i] : 0.f;
     sum(s, z);
     mean = s * inv_cols;
   }
@@ -204,22 +218,21 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
   load_cols<T, WPR>(g.b2, cols, 0.f, b2);
 #pragma unroll
   for (int i = 0; i < PER; ++i) gt[i] = a[i];
-  float nx[PER], nt[PER];
-  if (r0 < r1) {
-    load_row<T, WPR, VEC>(X + (size_t)r0 * g.ldx, cols, nx);
-    if (Tt) load_row<T, WPR, VEC>(Tt + (size_t)r0 * g.ldt, cols, nt);
-  }
+  Raw<T, WPR, VEC> nx, nt;                               // without t: x in its place, not used
+  auto fetch = [&](int row) {
+    row = min(row, g.rows - 1);
+    nx.load(X + (size_t)row * g.ldx, cols);
+    nt.load(Tt ? Tt + (size_t)row * g.ldt : X + (size_t)row * g.ldx, cols);
+  };
+  fetch(r0);
   int left = 0;                                          // rows left of the current clip
   for (int k = 0; k < g.run; ++k) {                      // the same count for every worker of the block: barriers inside
     const int row = r0 + k;
     const bool on = row < r1;
     float x[PER], t[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) { x[i] = nx[i]; t[i] = nt[i]; }
-    if (row + 1 < r1) {
-      load_row<T, WPR, VEC>(X + (size_t)(row + 1) * g.ldx, cols, nx);
-      if (Tt) load_row<T, WPR, VEC>(Tt + (size_t)(row + 1) * g.ldt, cols, nt);
-    }
+    nx.get(x);
+    nt.get(t);
+    fetch(row + 1);
     if (g.gate && on && left == 0) {
       const int clip = row / g.clip;
       left = (clip + 1) * g.clip - row;
@@ -245,8 +258,6 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
     }
     if (g.w2) {
       // from the sum in fp32, not from the stored y: one rounding less in h
-#pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] = column<T, WPR>(i) < cols ? x[i] : 0.f;
       row_stats<T, WPR, LAYER>(x, cols, inv_cols, g.eps, sum, my, ry);
 #pragma unroll
       for (int i = 0; i < PER; ++i) x[i] = (x[i] - my) * ry * w2[i] + b2[i];
@@ -259,8 +270,9 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
   }
 }
 
-template <typename T, int WPR, bool LAYER, bool VEC>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_bwd_kernel(const GatedArgs g) {
+// BIAS: with biases (b1, or a bias' gradient is wanted)
+template <typename T, int WPR, bool LAYER, bool VEC, bool BIAS>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void gated_norm_bwd_kernel(const GatedArgs g) {
   constexpr int L = 64 * WPR, THREADS = WPR > 4 ? L : 256, RPB = THREADS / L;
   __shared__ float red[2 * 2 * (THREADS / 64)];
   __shared__ float join[RPB > 1 ? RPB * L * PER : 1];
@@ -277,29 +289,32 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_bwd_kerne
   // 16 waves leave 128 registers a lane: the column vectors are then read for every row (they stay in the caches) and the
   // next row's loads do not run ahead; with both kept the kernel would spill 150 registers
   constexpr bool WIDE = WPR == 16;
-  float a[PER], w1[PER], b1[PER], w2[PER], gt[PER];
+  float w1[PER], b1[PER], w2[PER], gt[PER];              // w1 a, b1 a, w2, the gate
   auto columns = [&]() {
+    float a[PER];
     load_cols<T, WPR>(g.a, cols, 1.f, a);
     load_cols<T, WPR>(g.w1, cols, 1.f, w1);
-    load_cols<T, WPR>(g.b1, cols, 0.f, b1);
+    if constexpr (BIAS) load_cols<T, WPR>(g.b1, cols, 0.f, b1);
     load_cols<T, WPR>(g.w2, cols, 1.f, w2);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { w1[i] *= a[i]; b1[i] = BIAS ? b1[i] * a[i] : 0.f; }
   };
   if constexpr (!WIDE) columns();
   float aw[PER], ab[PER], bw[PER], bb[PER], dg[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) { gt[i] = 1.f; aw[i] = ab[i] = bw[i] = bb[i] = dg[i] = 0.f; }
-  float nx[PER], nt[PER], ny[PER], nh[PER];
+  Raw<T, WPR, VEC> nx, nt, ny, nh;
   f32x4 ns = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < PER; ++i) nx[i] = nt[i] = ny[i] = nh[i] = 0.f;
-  auto fetch = [&](int row) {
-    load_row<T, WPR, VEC>(X + (size_t)row * g.ldx, cols, nx);
-    if (Tt) load_row<T, WPR, VEC>(Tt + (size_t)row * g.ldt, cols, nt);
-    if (DY) load_row<T, WPR, VEC>(DY + (size_t)row * cols, cols, ny);
-    if (DH) load_row<T, WPR, VEC>(DH + (size_t)row * cols, cols, nh);
+  auto fetch = [&](int row) {                            // what is left out: x in its place, not used
+    row = min(row, g.rows - 1);
+    const T* x = X + (size_t)row * g.ldx;
+    nx.load(x, cols);
+    nt.load(Tt ? Tt + (size_t)row * g.ldt : x, cols);
+    ny.load(DY ? DY + (size_t)row * cols : x, cols);
+    nh.load(DH ? DH + (size_t)row * cols : x, cols);
     ns = *reinterpret_cast<const f32x4*>(g.stats + (size_t)row * 4);
   };
-  if (!WIDE && r0 < r1) fetch(r0);
+  if (!WIDE) fetch(r0);
   int left = 0, clip = 0;
   for (int k = 0; k < g.run; ++k) {
     const int row = r0 + k;
@@ -307,65 +322,71 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_bwd_kerne
     if constexpr (WIDE) {
       asm volatile("" ::: "memory");                       // keeps the reads in the loop
       columns();
-      if (on) fetch(row);
+      fetch(row);
     }
     float x[PER], t[PER], dy[PER], dh[PER];
     const f32x4 st = ns;
+    nx.get(x);
+    nt.get(t);
+    ny.get(dy);
+    nh.get(dh);
+    if (!on || !DY)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) { x[i] = nx[i]; t[i] = nt[i]; dy[i] = ny[i]; dh[i] = nh[i]; }
-    if (!WIDE && row + 1 < r1) fetch(row + 1);
-    if (!on) {
+      for (int i = 0; i < PER; ++i) dy[i] = 0.f;
+    if (!on || !Tt)
 #pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] = t[i] = dy[i] = dh[i] = 0.f;
-    }
+      for (int i = 0; i < PER; ++i) t[i] = 0.f;
+    if (!on)                                               // a row that is another's: finite or not, it adds nothing
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = dh[i] = 0.f;
+    if (!WIDE) fetch(row + 1);
     if (g.gate && on && left == 0) {
       clip = row / g.clip;
       left = (clip + 1) * g.clip - row;
       load_row<T, WPR, VEC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
     }
     --left;
-    float tn[PER], u[PER], yn[PER], dn[PER], s1 = 0.f, s2 = 0.f;
+    // t: t^, x: y^
+    float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      tn[i] = g.w1 ? (t[i] - st[0]) * st[1] : t[i];
-      u[i] = tn[i] * w1[i] + b1[i];
-      const float y = x[i] + gt[i] * a[i] * u[i];
-      yn[i] = (y - st[2]) * st[3];
-      dn[i] = column<T, WPR>(i) < cols ? dh[i] * w2[i] : 0.f;
-      s1 += dn[i];
-      s2 += dn[i] * yn[i];
+      t[i] = g.w1 ? (t[i] - st[0]) * st[1] : t[i];
+      x[i] += gt[i] * (t[i] * w1[i] + (BIAS ? b1[i] : 0.f));
+      x[i] = (x[i] - st[2]) * st[3];
+      const float dn = column<T, WPR>(i) < cols ? dh[i] * w2[i] : 0.f;
+      s1 += dn;
+      s2 += dn * x[i];
     }
     if (DH) {
       sum(s1, s2);
       const float m1 = LAYER ? s1 * inv_cols : 0.f, m2 = s2 * inv_cols;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        bw[i] += dh[i] * yn[i];
-        bb[i] += dh[i];
-        dy[i] += st[3] * (dn[i] - m1 - yn[i] * m2);
+        bw[i] += dh[i] * x[i];
+        if constexpr (BIAS) bb[i] += dh[i];
+        dy[i] += st[3] * (dh[i] * w2[i] - m1 - x[i] * m2);
       }
     }
     if (on) store_row<T, WPR, VEC>((T*)g.dx + (size_t)row * cols, cols, dy);
     if (Tt) {
-      float s3 = 0.f, s4 = 0.f, dm[PER];
+      float s3 = 0.f, s4 = 0.f;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const float d = on && column<T, WPR>(i) < cols ? dy[i] : 0.f;
-        const float gd = gt[i] * d;
-        aw[i] += gd * tn[i];
-        ab[i] += gd;
-        dg[i] += d * a[i] * u[i];
-        dm[i] = gd * a[i] * w1[i];
-        s3 += dm[i];
-        s4 += dm[i] * tn[i];
+        const float d = on && column<T, WPR>(i) < cols ? dy[i] : 0.f, gd = gt[i] * d;
+        aw[i] += gd * t[i];
+        if constexpr (BIAS) ab[i] += gd;
+        dg[i] += d * (t[i] * w1[i] + (BIAS ? b1[i] : 0.f));
+        dy[i] = gd * w1[i];                              // the gradient of t^
+        s3 += dy[i];
+        s4 += dy[i] * t[i];
       }
       if (g.w1) {
         sum(s3, s4);
         const float m3 = LAYER ? s3 * inv_cols : 0.f, m4 = s4 * inv_cols;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) dm[i] = st[1] * (dm[i] - m3 - tn[i] * m4);
+        for (int i = 0; i < PER; ++i) dy[i] = st[1] * (dy[i] - m3 - t[i] * m4);
       }
-      if (on && g.dt) store_row<T, WPR, VEC>((T*)g.dt + (size_t)row * cols, cols, dm);
+      if (on && g.dt) store_row<T, WPR, VEC>((T*)g.dt + (size_t)row * cols, cols, dy);
     }
     if (g.dgate && on && (left == 0 || row + 1 == r1)) {
       if (g.gpart) {
@@ -382,6 +403,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_bwd_kerne
   float* __restrict__ out = g.part + (size_t)blockIdx.x * 4 * cols;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
+    if (!BIAS && (q & 1)) continue;
     float v[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) v[i] = q == 0 ? aw[i] : q == 1 ? ab[i] : q == 2 ? bw[i] : bb[i];
@@ -411,7 +433,7 @@ struct GatedFinish {
   const float* a; const float* w1; const float* b1;
   float* da; float* dw1; float* db1; float* dw2; float* db2;
   void* dgate;
-  int blocks, cols, spc;
+  int blocks, cols, spc, bias;
   int col_blocks, n_first;             // part 1: 2 * col_blocks blocks
 };
 template <typename T>
@@ -425,7 +447,7 @@ __global__ __launch_bounds__(1024) void gated_norm_finish_kernel(const GatedFini
 #pragma unroll 8
       for (int b = wave; b < f.blocks; b += 16) {
         p += s[(size_t)b * 4 * f.cols];
-        q += s[(size_t)b * 4 * f.cols + f.cols];
+        if (f.bias) q += s[(size_t)b * 4 * f.cols + f.cols];
       }
     }
     __shared__ float red[2][16][64];
@@ -458,12 +480,14 @@ __global__ __launch_bounds__(1024) void gated_norm_finish_kernel(const GatedFini
 
 // ---------------------------------------------------------------------------
 struct GatedPlan { int wpr, rpb, run, spc, workers, blocks; };
-// Two blocks per CU, each with rows of its own to walk: enough loads in flight (a wave holds two rows' worth), and few partial sums.
-static GatedPlan gated_plan(int rows, int cols, int clip, bool gate) {
+// As many waves as a CU holds (backward: half of that, for the registers), each with rows of its own to walk: enough loads in flight (a
+// wave holds two rows' worth), and few partial sums
+constexpr int FWD_WAVES = 16, BWD_WAVES = 8;
+static GatedPlan gated_plan(int rows, int cols, int clip, bool gate, int waves) {
   GatedPlan p;
   p.wpr = cols <= 512 ? 1 : cols <= 1024 ? 2 : cols <= 2048 ? 4 : cols <= 4096 ? 8 : 16;
   p.rpb = p.wpr >= 4 ? 1 : 4 / p.wpr;
-  const int64_t want = (int64_t)device_cus() * 2 * p.rpb;
+  const int64_t want = (int64_t)device_cus() * waves / p.wpr;
   const int64_t run = std::max<int64_t>(1, (rows + want - 1) / want);
   p.spc = 0;
   if (!gate) {
@@ -483,24 +507,25 @@ static GatedPlan gated_plan(int rows, int cols, int clip, bool gate) {
 
 size_t gated_norm_workspace(int rows, int cols, int clip) {
   if (rows < 1 || cols < 1 || cols > 8192 || clip < 0) return 0;
-  const GatedPlan p = gated_plan(rows, cols, clip ? clip : rows, clip > 0);
+  const GatedPlan p = gated_plan(rows, cols, clip ? clip : rows, clip > 0, BWD_WAVES);
   return ((size_t)p.blocks * 4 + (p.spc ? p.workers : 0)) * cols * sizeof(float);
 }
 
 template <typename T, int WPR, bool LAYER, bool VEC>
-static int run_gated(const GatedArgs& g, const GatedPlan& p, bool back, hipStream_t s) {
+static int run_gated(const GatedArgs& g, const GatedPlan& p, int back, hipStream_t s) {
   constexpr int threads = WPR > 4 ? 64 * WPR : 256;
-  if (back) PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, LAYER, VEC>), dim3(p.blocks), dim3(threads), 0, s, g);
+  if (back == 2) PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, LAYER, VEC, true>), dim3(p.blocks), dim3(threads), 0, s, g);
+  else if (back) PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, LAYER, VEC, false>), dim3(p.blocks), dim3(threads), 0, s, g);
   else PT_LAUNCH((gated_norm_fwd_kernel<T, WPR, LAYER, VEC>), dim3(p.blocks), dim3(threads), 0, s, g);
   return 0;
 }
 template <typename T, int WPR>
-static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, bool vec, bool back, hipStream_t s) {
+static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, bool vec, int back, hipStream_t s) {
   return layer ? (vec ? run_gated<T, WPR, true, true>(g, p, back, s) : run_gated<T, WPR, true, false>(g, p, back, s))
                : (vec ? run_gated<T, WPR, false, true>(g, p, back, s) : run_gated<T, WPR, false, false>(g, p, back, s));
 }
 template <typename T>
-static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, bool vec, bool back, hipStream_t s) {
+static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, bool vec, int back, hipStream_t s) {
   switch (p.wpr) {
     case 1: return run_gated<T, 1>(g, p, layer, vec, back, s);
     case 2: return run_gated<T, 2>(g, p, layer, vec, back, s);
@@ -533,10 +558,10 @@ int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   GatedArgs g = {};
   g.x = x; g.t = t; g.gate = gate; g.a = a; g.w1 = w1; g.b1 = b1; g.w2 = w2; g.b2 = b2; g.y = y; g.h = h; g.stats = stats;
   g.ldx = (size_t)ldx; g.ldt = (size_t)ldt; g.rows = (int)rows; g.cols = cols; g.clip = gate ? clip : (int)rows; g.eps = eps;
-  const GatedPlan p = gated_plan(g.rows, cols, g.clip, gate != nullptr);
+  const GatedPlan p = gated_plan(g.rows, cols, g.clip, gate != nullptr, FWD_WAVES);
   g.run = p.run; g.spc = p.spc;
   const bool vec = gated_vec(g, dtype);
-  return dtype ? run_gated<unsigned short>(g, p, kind == 0, vec, false, s) : run_gated<float>(g, p, kind == 0, vec, false, s);
+  return dtype ? run_gated<unsigned short>(g, p, kind == 0, vec, 0, s) : run_gated<float>(g, p, kind == 0, vec, 0, s);
 }
 
 int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1,
@@ -551,16 +576,17 @@ int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   g.x = x; g.t = t; g.gate = gate; g.a = a; g.w1 = w1; g.b1 = b1; g.w2 = w2; g.dy = dy; g.dh = dh; g.stats = const_cast<float*>(stats);
   g.dx = dx; g.dt = dt; g.dgate = dgate;
   g.ldx = (size_t)ldx; g.ldt = (size_t)ldt; g.rows = (int)rows; g.cols = cols; g.clip = gate ? clip : (int)rows;
-  const GatedPlan p = gated_plan(g.rows, cols, g.clip, gate != nullptr);
+  const GatedPlan p = gated_plan(g.rows, cols, g.clip, gate != nullptr, BWD_WAVES);
   g.run = p.run; g.spc = p.spc;
   g.part = (float*)ws;
   g.gpart = p.spc && dgate ? g.part + (size_t)p.blocks * 4 * cols : nullptr;
   const bool vec = gated_vec(g, dtype);
-  if (dtype ? run_gated<unsigned short>(g, p, kind == 0, vec, true, s) : run_gated<float>(g, p, kind == 0, vec, true, s)) return 1;
+  const int bias = b1 || db1 || db2 ? 1 : 0;
+  if (dtype ? run_gated<unsigned short>(g, p, kind == 0, vec, 1 + bias, s) : run_gated<float>(g, p, kind == 0, vec, 1 + bias, s)) return 1;
   GatedFinish f = {};
   f.part = g.part; f.gpart = g.gpart; f.a = a; f.w1 = w1; f.b1 = b1;
   f.da = t ? da : nullptr; f.dw1 = t ? dw1 : nullptr; f.db1 = t ? db1 : nullptr; f.dw2 = dw2; f.db2 = db2;
-  f.dgate = dgate; f.blocks = p.blocks; f.cols = cols; f.spc = p.spc;
+  f.dgate = dgate; f.bias = bias; f.blocks = p.blocks; f.cols = cols; f.spc = p.spc;
   f.col_blocks = (cols + 63) / 64;
   f.n_first = 2 * f.col_blocks;
   const int64_t gate_blocks = g.gpart ? (int64_t)(rows / clip) * ((cols + 1023) / 1024) : 0;

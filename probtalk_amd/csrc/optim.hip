@@ -44,9 +44,8 @@ __device__ __forceinline__ unsigned hash_bits(unsigned c, unsigned key) {
 
 template <int M>
 __device__ __forceinline__ float code_value(unsigned c) {
-  const float lin = (float)c;
-  const float flt = __uint_as_float((c << (23 - M)) + ((126u + M) << 23));
-  return c < (1u << M) ? lin : flt;
+  // with the code's exponent bits in the place of fp32's, fp32 reads the same number as a multiple of 2^-126-M, denormals included
+  return ldexpf(__uint_as_float(c << (23 - M)), 126 + M);
 }
 
 // |x| -> code, z = |x| / scale in [0, TOP], r: 16 random bits
@@ -58,10 +57,20 @@ __device__ __forceinline__ unsigned value_code(float z, unsigned r) {
   return z < (float)(1 << M) ? lin : flt;
 }
 
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_umax(unsigned v) {
+  return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
+}
+// the maximum over the wave in every lane, without the LDS crossbar
 __device__ __forceinline__ unsigned wave_umax(unsigned v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
-  return v;
+  v = dpp_umax<0xB1>(v);       // quad_perm [1,0,3,2]
+  v = dpp_umax<0x4E>(v);       // quad_perm [2,3,0,1]
+  v = dpp_umax<0x141>(v);      // row_half_mirror
+  v = dpp_umax<0x140>(v);      // row_mirror
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(b[0], b[1]);
 }
 
 // ---------------------------------------------------------------------------
@@ -110,8 +119,8 @@ __device__ __forceinline__ float bf2f(unsigned short x) { return __uint_as_float
 // bf16 parameters are rounded stochastically too: the step of a parameter is mostly below half of its last bf16 bit
 __device__ __forceinline__ unsigned short f2bf_sr(float x, unsigned r16) {
   const unsigned u = __float_as_uint(x);
-  if ((u & 0x7F800000u) == 0x7F800000u) return (unsigned short)((u >> 16) | ((u & 0xFFFFu) ? 0x40u : 0u));
-  return (unsigned short)((u + r16) >> 16);
+  const unsigned odd = (u >> 16) | ((u & 0xFFFFu) ? 0x40u : 0u);                  // infinities stay, a NaN stays one
+  return (unsigned short)((u & 0x7F800000u) == 0x7F800000u ? odd : (u + r16) >> 16);
 }
 
 // What a tensor without the vector path (odd address) or the last block of a tensor does: one value at a time
@@ -181,16 +190,12 @@ __device__ __forceinline__ void moments32(float g, float gs, float b1, float c1,
   v = fmaf(gr, c2 * gr, b2 * v);
 }
 
-// T: float or bf16 bits (unsigned short); S8: 8-bit moments.
-template <typename T, bool S8>
-__global__ __launch_bounds__(256) void adamw_multi_kernel(const AdamTab tab, const AdamHyper h) {
-  const int i = find_tensor(tab, h.count, blockIdx.x);
-  const unsigned unit = blockIdx.x - tab.first[i];
-  const size_t n = (size_t)(tab.n[i] >> 1);
+// One wave's 1024 values of tensor i from e0 on.  T: float or bf16 bits (unsigned short); S8: 8-bit moments; FULL: all of them are there and
+// aligned, so the loads are plain vectors and all of them go out before the first is waited for.
+template <typename T, bool S8, bool FULL>
+__device__ __forceinline__ void adamw_wave(const AdamTab& tab, const AdamHyper& h, const int i, const size_t e0, const size_t n) {
   const bool aligned = tab.n[i] & 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const size_t e0 = (size_t)unit * UNIT + wave * (UNIT / 4);
-  if (e0 >= n) return;                                   // whole waves leave; nothing below is shared between waves
+  const int lane = threadIdx.x & 63;
   T* __restrict__ P = (T*)tab.p[i];
   const T* __restrict__ G = (const T*)tab.g[i];
   const float gs = h.gscale ? *h.gscale : 1.f;
@@ -206,14 +211,14 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AdamTab tab, con
 #pragma unroll
   for (int k = 0; k < NB; ++k) {
     const size_t e = e0 + k * QBLOCK + lane * 4;
-    const bool vec = aligned && e + 4 <= n;
+    const bool vec = FULL || (aligned && e + 4 <= n);
     load4(P, e, n, vec, p[k]);
     load4(G, e, n, vec, g[k]);
     if constexpr (S8) {
       cm[k] = load4b((const unsigned char*)tab.m[i], e, n, vec);
       cv[k] = load4b((const unsigned char*)tab.v[i], e, n, vec);
       const size_t b = e0 / QBLOCK + k;
-      const bool in = b * QBLOCK < n;
+      const bool in = FULL || b * QBLOCK < n;
       sm[k] = in ? tab.s[i][2 * b] : 0.f;
       sv[k] = in ? tab.s[i][2 * b + 1] : 0.f;
     } else {
@@ -221,16 +226,17 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AdamTab tab, con
       load4((const float*)tab.v[i], e, n, vec, v[k]);
     }
   }
+  // 8-bit moments: the new moments of all four blocks, then the scales of these eight (block, moment) pairs in eight lanes at once:
+  // a division and a reciprocal cost ten instructions each, and every lane of the wave would compute the same
+  float inv_m[NB], inv_v[NB];
+  if constexpr (S8) {
+    unsigned top[2 * NB];
 #pragma unroll
-  for (int k = 0; k < NB; ++k) {
-    const size_t e = e0 + k * QBLOCK + lane * 4;
-    const bool vec = aligned && e + 4 <= n;
-    float inv_m = 0.f, inv_v = 0.f;
-    if constexpr (S8) {
+    for (int k = 0; k < NB; ++k) {
       unsigned am = 0, av = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const unsigned c = (cm[k] >> (8 * j)) & 255u;
+        const unsigned c = cm[k] >> (8 * j);
         const float mag = code_value<M_BITS>(c & 127u) * sm[k];
         m[k][j] = c & 128u ? -mag : mag;
         v[k][j] = code_value<V_BITS>((cv[k] >> (8 * j)) & 255u) * sv[k];
@@ -239,43 +245,77 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AdamTab tab, con
         am = max(am, __float_as_uint(m[k][j]) & 0x7FFFFFFFu);
         av = max(av, __float_as_uint(v[k][j]) & 0x7FFFFFFFu);
       }
-      const float bm = __uint_as_float(wave_umax(am)), bv = __uint_as_float(wave_umax(av));
-      sm[k] = bm < SCALE_MIN ? 0.f : bm / TOP_M;         // a block with a NaN or an infinity: that scale, codes 0, NaN from here on
-      sv[k] = bv < SCALE_MIN ? 0.f : bv / TOP_V;
-      inv_m = bm >= SCALE_MIN && bm < INFINITY ? 1.f / sm[k] : 0.f;
-      inv_v = bv >= SCALE_MIN && bv < INFINITY ? 1.f / sv[k] : 0.f;
+      top[2 * k] = wave_umax(am);
+      top[2 * k + 1] = wave_umax(av);
     }
+    unsigned mine = top[0];
+#pragma unroll
+    for (int i = 1; i < 2 * NB; ++i) mine = (lane & 7) == i ? top[i] : mine;
+    const float big = __uint_as_float(mine);
+    // a block with a NaN or an infinity: that scale, codes 0, NaN from here on
+    const float scale = big < SCALE_MIN ? 0.f : big / (lane & 1 ? TOP_V : TOP_M);
+    const float inv = big >= SCALE_MIN && big < INFINITY ? 1.f / scale : 0.f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      sm[k] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 2 * k));
+      sv[k] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 2 * k + 1));
+      inv_m[k] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(inv), 2 * k));
+      inv_v[k] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(inv), 2 * k + 1));
+    }
+  }
+  const float bc2_inv = 1.f / bc2_sqrt;
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    const size_t e = e0 + k * QBLOCK + lane * 4;
+    const bool vec = FULL || (aligned && e + 4 <= n);
     unsigned short pb[4];
-    unsigned om = 0, ov = 0;
+    unsigned om = 0, ov = 0, sign = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if constexpr (!S8) moments32(g[k][j], gs, h.b1, c1, h.b2, c2, m[k][j], v[k][j]);
-      const float denom = sqrtf(v[k][j]) / bc2_sqrt + h.eps;
-      const float pv = fmaf(decay, p[k][j], -(step_size * (m[k][j] / denom)));
+      float pv;
+      if constexpr (S8) {
+        // nothing here decides a code: the hardware's root and reciprocal (1 ulp each) for the IEEE ones' forty instructions
+        const float denom = fmaf(__builtin_amdgcn_sqrtf(v[k][j]), bc2_inv, h.eps);
+        pv = fmaf(decay, p[k][j], -(step_size * (m[k][j] * __builtin_amdgcn_rcpf(denom))));
+      } else {
+        moments32(g[k][j], gs, h.b1, c1, h.b2, c2, m[k][j], v[k][j]);
+        const float denom = sqrtf(v[k][j]) / bc2_sqrt + h.eps;
+        pv = fmaf(decay, p[k][j], -(step_size * (m[k][j] / denom)));
+      }
       p[k][j] = pv;
       unsigned r = 0;
       if constexpr (S8 || sizeof(T) == 2)
         r = hash_bits((tab.blk[i] + (unsigned)(e0 / QBLOCK) + k) * (unsigned)QBLOCK + lane * 4 + j, key);
       if constexpr (S8) {
-        const float zm = fminf(fabsf(m[k][j]) * inv_m, TOP_M), zv = fminf(v[k][j] * inv_v, TOP_V);
-        unsigned a = inv_m > 0.f ? value_code<M_BITS>(zm, r & 0xFFFFu) : 0u, b = inv_v > 0.f ? value_code<V_BITS>(zv, r >> 16) : 0u;
-        if (inv_v > 0.f && zv > 0.f && b == 0u) b = 1u;
-        om |= (a | (m[k][j] < 0.f ? 128u : 0u)) << (8 * j);
-        ov |= b << (8 * j);
+        const float zm = fminf(fabsf(m[k][j]) * inv_m[k], TOP_M), zv = fminf(v[k][j] * inv_v[k], TOP_V);
+        om |= value_code<M_BITS>(zm, r & 0xFFFFu) << (8 * j);
+        ov |= max(value_code<V_BITS>(zv, r >> 16), zv > 0.f ? 1u : 0u) << (8 * j);
+        sign |= (m[k][j] < 0.f ? 128u : 0u) << (8 * j);
       }
       if constexpr (sizeof(T) == 2) pb[j] = f2bf_sr(pv, ((r * 0xBB67AE85u) >> 16) & 0xFFFFu);
     }
     if constexpr (sizeof(T) == 2) store4((unsigned short*)P, e, n, vec, pb); else store4((float*)P, e, n, vec, p[k]);
     if constexpr (S8) {
-      store4b((unsigned char*)tab.m[i], e, n, vec, om);
-      store4b((unsigned char*)tab.v[i], e, n, vec, ov);
+      store4b((unsigned char*)tab.m[i], e, n, vec, (inv_m[k] > 0.f ? om : 0u) | sign);      // no finite scale: codes 0
+      store4b((unsigned char*)tab.v[i], e, n, vec, inv_v[k] > 0.f ? ov : 0u);
       const size_t b = e0 / QBLOCK + k;
-      if (lane == 0 && b * QBLOCK < n) { tab.s[i][2 * b] = sm[k]; tab.s[i][2 * b + 1] = sv[k]; }
+      if (lane == 0 && (FULL || b * QBLOCK < n)) { tab.s[i][2 * b] = sm[k]; tab.s[i][2 * b + 1] = sv[k]; }
     } else {
       store4((float*)tab.m[i], e, n, vec, m[k]);
       store4((float*)tab.v[i], e, n, vec, v[k]);
     }
   }
+}
+
+template <typename T, bool S8>
+__global__ __launch_bounds__(256) void adamw_multi_kernel(const AdamTab tab, const AdamHyper h) {
+  const int i = find_tensor(tab, h.count, blockIdx.x);
+  const size_t n = (size_t)(tab.n[i] >> 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const size_t e0 = (size_t)(blockIdx.x - tab.first[i]) * UNIT + wave * (UNIT / 4);
+  if (e0 >= n) return;                                   // whole waves leave; nothing is shared between waves
+  if ((tab.n[i] & 1) && e0 + UNIT / 4 <= n) adamw_wave<T, S8, true>(tab, h, i, e0, n);
+  else adamw_wave<T, S8, false>(tab, h, i, e0, n);
 }
 
 // the step count of a captured step lives on the device

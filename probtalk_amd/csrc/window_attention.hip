@@ -38,7 +38,7 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* glb_ptr_t;
 
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, SLACK = 8.f;
 
 template <typename T> struct Types;
 template <> struct Types<__bf16> { typedef bf16x8 frag; typedef bf16x4 quad; };
@@ -399,23 +399,25 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[x][r]);
       mx = fmaxf(mx, half_other(mx)) * a.sc;
-      const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;  // nothing visible so far: every exponential is 0
-      const float alpha = __builtin_amdgcn_exp2f(m - base);
-      float sum = 0.f;
+      // The base of the exponentials follows the maximum only where that has grown by 8 (or is the first one): the sums stay below
+      // 2^8 times what they would be, far from fp32's range, and the results need no factor in most tiles
+      if (__ballot(mx > m + SLACK)) {
+        const float mn = mx > m + SLACK ? mx : m, alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+      }
+      const float base = m == -INFINITY ? 0.f : m;                       // nothing visible so far: every exponential is 0
 #pragma unroll
       for (int x = 0; x < NB; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -base));
-          sum += st[x][r];
+          l += st[x][r];                                                 // this lane's half of the column; joined at the end
         }
-      l = l * alpha + sum;                                               // this lane's half of the column; joined at the end
-      m = mn;
-      if (__ballot(alpha != 1.f))                                        // most tiles leave every row's maximum where it is
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
       if constexpr (!BF) vc.template read<0>(vf[0]);
       add_product<T, DP>(o, vf[0], st[0]);                               // probabilities in [0, 1] to bf16: 2^-9 of each
       if constexpr (NB > 1) {

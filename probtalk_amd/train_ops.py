@@ -175,24 +175,31 @@ def _row_stride(v):
     return 0 if v is None else v.stride(0) if v.shape[0] > 1 else v.shape[1]
 
 
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _gated_norm(x, t, gate, res_scale, post_w, post_b, pre_w, pre_b, clip, kind, eps, grad):
+    rows, cols = x.shape
+    y = None if t is None else torch.empty(rows, cols, device=x.device, dtype=x.dtype)
+    h = None if pre_w is None else torch.empty(rows, cols, device=x.device, dtype=x.dtype)
+    stats = torch.empty(rows, 4, device=x.device, dtype=torch.float32) if grad else None
+    with _on(x.device):
+        check(_lib.lib().pt_train_gated_norm_fwd(_at(x), _row_stride(x), _at(t), _row_stride(t), _at(gate), _at(res_scale), _at(post_w),
+                                                 _at(post_b), _at(pre_w), _at(pre_b), _at(y), _at(h), _at(stats), rows, cols, clip, kind, eps,
+                                                 int(x.dtype is torch.bfloat16), stream()))
+    return y, h, stats
+
+
 class GatedNorm(torch.autograd.Function):
     """y = x + res_scale * gate * N(t; post), h = N(y; pre) (see gated_norm)."""
 
     @staticmethod
-    def forward(ctx, x, t, gate, res_scale, post_w, post_b, pre_w, pre_b, clip, kind, eps, grad):
-        rows, cols = x.shape
-        bf = int(x.dtype is torch.bfloat16)
-        y = None if t is None else torch.empty(rows, cols, device=x.device, dtype=x.dtype)
-        h = None if pre_w is None else torch.empty(rows, cols, device=x.device, dtype=x.dtype)
-        stats = torch.empty(rows, 4, device=x.device, dtype=torch.float32) if grad else None
-        with _on(x.device):
-            check(_lib.lib().pt_train_gated_norm_fwd(ptr(x), _row_stride(x), ptr(t), _row_stride(t), ptr(gate), ptr(res_scale),
-                                                     ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(y), ptr(h), ptr(stats), rows, cols,
-                                                     clip, kind, eps, bf, stream()))
-        if grad:
-            ctx.save_for_backward(x, t, gate, res_scale, post_w, post_b, pre_w, stats)
-            ctx.meta = (clip, kind, bf)
-            ctx.set_materialize_grads(False)
+    def forward(ctx, x, t, gate, res_scale, post_w, post_b, pre_w, pre_b, clip, kind, eps):
+        y, h, stats = _gated_norm(x, t, gate, res_scale, post_w, post_b, pre_w, pre_b, clip, kind, eps, True)
+        ctx.save_for_backward(x, t, gate, res_scale, post_w, post_b, pre_w, stats)
+        ctx.meta = (clip, kind, int(x.dtype is torch.bfloat16))
+        ctx.set_materialize_grads(False)
         return y, h
 
     @staticmethod
@@ -200,23 +207,22 @@ class GatedNorm(torch.autograd.Function):
         x, t, gate, res_scale, post_w, post_b, pre_w, stats = ctx.saved_tensors
         clip, kind, bf = ctx.meta
         if dy is None and dh is None:
-            return (None,) * 12
+            return (None,) * 11
         rows, cols = x.shape
         need = ctx.needs_input_grad
         dy, dh = (None if d is None else d.contiguous() for d in (dy, dh))
         new = lambda like: torch.empty(like.shape, device=x.device, dtype=like.dtype)  # noqa: E731
-        vec = lambda i: torch.empty(cols, device=x.device, dtype=torch.float32) if need[i] else None  # noqa: E731
         dx = new(x)
         dt = new(t) if need[1] else None
         dgate = new(gate) if need[2] else None
-        da, dw1, db1, dw2, db2 = vec(3), vec(4), vec(5), vec(6), vec(7)
+        vec = [torch.empty(cols, device=x.device, dtype=torch.float32) if n else None for n in need[3:8]]
         L = _lib.lib()
         with _on(x.device):
-            ws = torch.empty(int(L.pt_train_gated_norm_workspace_bytes(rows, cols, clip if gate is not None else 0)), dtype=torch.uint8, device=x.device)
-            check(L.pt_train_gated_norm_bwd(ptr(x), _row_stride(x), ptr(t), _row_stride(t), ptr(gate), ptr(res_scale), ptr(post_w),
-                                            ptr(post_b), ptr(pre_w), ptr(stats), ptr(dy), ptr(dh), ptr(dx), ptr(dt), ptr(dgate), ptr(da), ptr(dw1),
-                                            ptr(db1), ptr(dw2), ptr(db2), ptr(ws), ws.numel(), rows, cols, clip, kind, bf, stream()))
-        return dx, dt, dgate, da, dw1, db1, dw2, db2, None, None, None, None
+            ws = torch.empty(L.pt_train_gated_norm_workspace_bytes(rows, cols, clip if gate is not None else 0), dtype=torch.uint8, device=x.device)
+            check(L.pt_train_gated_norm_bwd(_at(x), _row_stride(x), _at(t), _row_stride(t), _at(gate), _at(res_scale), _at(post_w), _at(post_b),
+                                            _at(pre_w), _at(stats), _at(dy), _at(dh), _at(dx), _at(dt), _at(dgate), *map(_at, vec), _at(ws),
+                                            ws.numel(), rows, cols, clip, kind, bf, stream()))
+        return dx, dt, dgate, *vec, None, None, None
 
 
 def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, rows_per_clip=None,
@@ -225,40 +231,45 @@ def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias
 
         y = x + res_scale * gate * u,   u = N(t) * post_weight + post_bias,   h = N(y) * pre_weight + pre_bias      -> (y, h)
 
-    x, t: rows (R, C) of fp32 or bf16, 1 <= C <= 8192, with neighbouring columns.  gate (R / rows_per_clip, C) of x's type: a row
-    for every rows_per_clip rows (by default as many as it has rows for).  Vectors of C values in fp32.  kind: 'layer' (mean and
-    variance) or 'rms'.  Left out: t (y is x itself), gate, res_scale, post_weight (u = t), pre_weight (h is None).  Statistics and
-    sums are fp32; h is taken from y before it is rounded to bf16.  To capture the backward pass into a HIP graph, make the leaves
-    inside the capture (x.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
-    if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16) or not 1 <= x.shape[1] <= 8192:
+    x, t: rows (R, C) of fp32 or bf16, 1 <= C <= 8192.  gate (R / rows_per_clip, C) of x's type: a row for every rows_per_clip rows
+    (by default as many as it has rows for).  Vectors of C values in fp32.  kind: 'layer' (mean and variance) or 'rms'.  Left out:
+    t (y is x itself), gate, res_scale, post_weight (u = t), pre_weight (h is None).  Statistics and sums are fp32; h is taken from y
+    before that is rounded to bf16.  To capture the backward pass into a HIP graph, make the leaves inside the capture
+    (x.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
+    if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16) or not 1 <= x.shape[1] <= 8192 or x.shape[0] < 1:
         raise RuntimeError(f"gated_norm: rows (R, C) of fp32 or bf16 on the GPU with C up to 8192, got {tuple(x.shape)} {x.dtype} on {x.device}")
-    if kind not in ("layer", "rms"):
+    if kind != "layer" and kind != "rms":
         raise ValueError(f"gated_norm: kind must be 'layer' or 'rms', got {kind!r}")
     rows, cols = x.shape
-    if t is None and (gate is not None or res_scale is not None or post_weight is not None or pre_weight is None):
-        raise RuntimeError("gated_norm: without t there is nothing to gate, scale or norm but x: pass pre_weight alone")
+    gpu = x.get_device()
+    if t is None:
+        if gate is not None or res_scale is not None or post_weight is not None or pre_weight is None:
+            raise RuntimeError("gated_norm: without t there is nothing to gate, scale or norm but x: pass pre_weight alone")
+    elif t.shape != x.shape or t.dtype is not x.dtype or t.get_device() != gpu:
+        raise RuntimeError(f"gated_norm: t must be {tuple(x.shape)} {x.dtype} on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     if (post_bias is not None and post_weight is None) or (pre_bias is not None and pre_weight is None):
         raise RuntimeError("gated_norm: a bias comes with its weight")
-    for name, v, shape, dtype in (("t", t, (rows, cols), x.dtype), ("res_scale", res_scale, (cols,), torch.float32),
-                                  ("post_weight", post_weight, (cols,), torch.float32), ("post_bias", post_bias, (cols,), torch.float32),
-                                  ("pre_weight", pre_weight, (cols,), torch.float32), ("pre_bias", pre_bias, (cols,), torch.float32)):
-        if v is not None and (tuple(v.shape) != shape or v.dtype is not dtype or v.device != x.device):
-            raise RuntimeError(f"gated_norm: {name} must be {shape} {dtype} on {x.device}, got {tuple(v.shape)} {v.dtype} on {v.device}")
-    clip = max(rows, 1)
+    vectors = (res_scale, post_weight, post_bias, pre_weight, pre_bias)
+    for name, v in zip(("res_scale", "post_weight", "post_bias", "pre_weight", "pre_bias"), vectors):
+        if v is not None and (v.shape != (cols,) or v.dtype is not torch.float32 or v.get_device() != gpu):
+            raise RuntimeError(f"gated_norm: {name} must be ({cols},) torch.float32 on {x.device}, got {tuple(v.shape)} {v.dtype} on {v.device}")
+    clip = rows
     if gate is not None:
-        if gate.dim() != 2 or gate.shape[1] != cols or gate.dtype is not x.dtype or gate.device != x.device:
+        if gate.dim() != 2 or gate.shape[1] != cols or gate.dtype is not x.dtype or gate.get_device() != gpu:
             raise RuntimeError(f"gated_norm: gate must be (clips, {cols}) {x.dtype} on {x.device}, got {tuple(gate.shape)} {gate.dtype} on {gate.device}")
         clip = int(rows_per_clip) if rows_per_clip is not None else rows // max(gate.shape[0], 1)
         if clip < 1 or gate.shape[0] * clip != rows:
             raise RuntimeError(f"gated_norm: {rows} rows are not {gate.shape[0]} clips of {clip}")
-    if rows == 0:
-        raise RuntimeError("gated_norm: no rows")
-    near = lambda v: v if v is None or (v.stride(1) == 1 and v.stride(0) >= cols) else v.contiguous()  # noqa: E731
-    flat = lambda v: None if v is None else v.contiguous()  # noqa: E731
-    given = [near(x), near(t), flat(gate), flat(res_scale), flat(post_weight), flat(post_bias), flat(pre_weight), flat(pre_bias)]
-    grad = torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in given)
-    y, h = GatedNorm.apply(*given, clip, 0 if kind == "layer" else 1, float(eps), grad)
-    return (x if t is None else y), h
+        gate = gate.contiguous()
+    own = x
+    x, t = (v if v is None or (v.stride(1) == 1 and v.stride(0) >= cols) else v.contiguous() for v in (x, t))
+    given = (x, t, gate, *(None if v is None else v.contiguous() for v in vectors))
+    mode = 0 if kind == "layer" else 1
+    if torch.is_grad_enabled() and any([v is not None and v.requires_grad for v in given]):
+        y, h = GatedNorm.apply(*given, clip, mode, eps)
+    else:
+        y, h, _ = _gated_norm(*(v if v is None else v.detach() for v in given), clip, mode, eps, False)
+    return (own if t is None else y), h
 
 
 class ModSiLU(torch.autograd.Function):
@@ -334,14 +345,16 @@ def attention_cross(q, kv, B, Nq, Nk, p=0.0, seeds=None):
 
 def _strides(*tensors):
     """Strides of all but the last dimension, as the C entries take them (a dimension of one value has none)."""
-    return array.array("q", [s if n > 1 else 0 for t in tensors for s, n in zip(t.stride()[:-1], t.shape[:-1])])
+    out = []
+    for t in tensors:
+        out += [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+    return array.array("q", out)
 
 
 def _has_vectors(t):
     """Whether rows of channels can be read in 16-byte vectors."""
-    size = t.element_size()
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and
-            all(n == 1 or (s * size) % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])))
+    strides, per = t.stride(), 16 // t.element_size()
+    return strides[-1] == 1 and t.data_ptr() % 16 == 0 and all([n == 1 or s % per == 0 for s, n in zip(strides[:-1], t.shape)])
 
 
 def _vectors(t):
@@ -352,21 +365,23 @@ def _vectors(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _window_attention(q, k, v, lengths, meta, grad):
+    B, Nq, _, H, _, D = meta[:6]
+    o = torch.empty(B, Nq, H, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32) if grad else None
+    with _on(q.device):
+        check(_lib.lib().pt_attention_window_fwd(_at(q), _at(k), _at(v), _at(o), _at(lse), _address(_strides(q, k, v)), _at(lengths), *meta, stream()))
+    return o, lse
+
+
 class WindowAttention(torch.autograd.Function):
     """softmax over a window of keys and a few first ones (see window_attention)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, lengths, left, right, sinks, scale, grad):
-        B, Nq, H, D = q.shape
-        Nk, Hk = k.shape[1], k.shape[2]
-        o = torch.empty(B, Nq, H, D, device=q.device, dtype=q.dtype)
-        lse = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32) if grad else None
-        ctx.meta = (B, Nq, Nk, H, Hk, D, left, right, sinks, scale, int(q.dtype is torch.bfloat16))
-        with _on(q.device):
-            check(_lib.lib().pt_attention_window_fwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), _address(_strides(q, k, v)), ptr(lengths), *ctx.meta,
-                                                     stream()))
-        if grad:
-            ctx.save_for_backward(q, k, v, lengths, o, lse)
+    def forward(ctx, q, k, v, lengths, meta):
+        o, lse = _window_attention(q, k, v, lengths, meta, True)
+        ctx.meta = meta
+        ctx.save_for_backward(q, k, v, lengths, o, lse)
         return o
 
     @staticmethod
@@ -376,23 +391,24 @@ class WindowAttention(torch.autograd.Function):
         do = _vectors(do.contiguous())
         dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
         with _on(q.device):
-            ws = torch.empty(int(L.pt_attention_window_bwd_workspace_bytes(*ctx.meta[:9])), dtype=torch.uint8, device=q.device)
-            check(L.pt_attention_window_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(do), ptr(lse), ptr(dq), ptr(dk), ptr(dv), _address(_strides(q, k, v)),
-                                            ptr(lengths), *ctx.meta, ptr(ws), ws.numel(), stream()))
-        return dq, dk, dv, None, None, None, None, None, None
+            ws = torch.empty(L.pt_attention_window_bwd_workspace_bytes(*ctx.meta[:9]), dtype=torch.uint8, device=q.device)
+            check(L.pt_attention_window_bwd(_at(q), _at(k), _at(v), _at(o), _at(do), _at(lse), _at(dq), _at(dk), _at(dv), _address(_strides(q, k, v)),
+                                            _at(lengths), *ctx.meta, _at(ws), ws.numel(), stream()))
+        return dq, dk, dv, None, None
 
 
 def _check_window(what, q, k, v, heads, batch, lengths, left, right, sinks, scale):
     if k.dim() != 4 or v.shape != k.shape or k.shape[0] != batch or k.shape[3] != q.shape[-1] or k.shape[1] < 1:
         raise RuntimeError(f"{what}: shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} do not go together")
-    if not q.is_cuda or k.device != q.device or v.device != q.device:
+    gpu = q.get_device()
+    if gpu < 0 or k.get_device() != gpu or v.get_device() != gpu:
         raise RuntimeError(f"{what}: tensors must be on one GPU, got {q.device}, {k.device} and {v.device}")
     if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise RuntimeError(f"{what}: fp32 or bf16, one type for all, got {q.dtype}, {k.dtype} and {v.dtype}")
     d = q.shape[-1]
     if d % 8 or not 8 <= d <= 128 or k.shape[2] < 1 or heads < 1 or heads % k.shape[2]:
         raise RuntimeError(f"{what}: {heads} query heads over {k.shape[2]} key heads of {d} channels (a multiple of 8 up to 128)")
-    if lengths is not None and (tuple(lengths.shape) != (batch,) or lengths.dtype is not torch.int32 or lengths.device != q.device or not lengths.is_contiguous()):
+    if lengths is not None and (lengths.shape != (batch,) or lengths.dtype is not torch.int32 or lengths.get_device() != gpu or not lengths.is_contiguous()):
         raise RuntimeError(f"{what}: lengths must be ({batch},) torch.int32 on {q.device}")
     left, right = (-1 if n is None else int(n) for n in (left, right))
     if left < -1 or right < -1 or not 0 <= sinks <= 128:
@@ -416,12 +432,14 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
     leaves inside the capture (q.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if q.dim() != 4 or q.shape[0] < 1 or q.shape[1] < 1:
         raise RuntimeError(f"window_attention: q is (B, Nq, H, D), got {tuple(q.shape)}")
-    args = _check_window("window_attention", q, k, v, q.shape[2], q.shape[0], lengths, left, right, sinks, scale)
+    left, right, sinks, scale = _check_window("window_attention", q, k, v, q.shape[2], q.shape[0], lengths, left, right, sinks, scale)
     if k.shape[1] < q.shape[1]:
         raise RuntimeError(f"window_attention: {q.shape[1]} rows for {k.shape[1]} keys")
-    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    meta = (*q.shape[:2], k.shape[1], q.shape[2], k.shape[2], q.shape[3], left, right, sinks, scale, int(q.dtype is torch.bfloat16))
     q, k, v = (_vectors(t if t.shape[1] == 1 or 0 <= t.stride(1) <= 1 << 20 else t.contiguous()) for t in (q, k, v))
-    return WindowAttention.apply(q, k, v, lengths, *args, grad)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return WindowAttention.apply(q, k, v, lengths, meta)
+    return _window_attention(q.detach(), k.detach(), v.detach(), lengths, meta, False)[0]
 
 
 def window_attention_step(q, k, v, lengths, left=None, sinks=0, scale=None):
@@ -441,9 +459,9 @@ def window_attention_step(q, k, v, lengths, left=None, sinks=0, scale=None):
     o = torch.empty(B, H, D, device=q.device, dtype=q.dtype)
     L = _lib.lib()
     with _on(q.device):
-        ws = torch.empty(int(L.pt_attention_window_step_workspace_bytes(B, N, H, Hk, D, left, sinks)), dtype=torch.uint8, device=q.device)
-        check(L.pt_attention_window_step(ptr(q), ptr(k), ptr(v), ptr(o), _address(_strides(q, k, v)), ptr(lengths), B, N, H, Hk, D, left, sinks, scale,
-                                         int(q.dtype is torch.bfloat16), ptr(ws), ws.numel(), stream()))
+        ws = torch.empty(L.pt_attention_window_step_workspace_bytes(B, N, H, Hk, D, left, sinks), dtype=torch.uint8, device=q.device)
+        check(L.pt_attention_window_step(_at(q), _at(k), _at(v), _at(o), _address(_strides(q, k, v)), _at(lengths), B, N, H, Hk, D, left, sinks, scale,
+                                         int(q.dtype is torch.bfloat16), _at(ws), ws.numel(), stream()))
     return o
 
 
@@ -807,13 +825,14 @@ def _address(a):
 
 
 def _grad_norm(pointers, sizes, is_bf16, max_norm, device):
+    """A device tensor [norm, coef]."""
     L = _lib.lib()
     n = len(pointers)
     out = torch.empty(2, device=device, dtype=torch.float32)
-    ws = torch.empty(int(L.pt_train_grad_norm_workspace_bytes(_address(sizes), n)), dtype=torch.uint8, device=device)
-    check(L.pt_train_grad_norm(_address(pointers), _address(sizes), is_bf16, n, float(max_norm), ptr(out), C.c_void_p(out.data_ptr() + 4),
-                               ptr(ws), ws.numel(), stream()))
-    return out[:1], out[1:]
+    ws = torch.empty(L.pt_train_grad_norm_workspace_bytes(_address(sizes), n), dtype=torch.uint8, device=device)
+    at = out.data_ptr()
+    check(L.pt_train_grad_norm(_address(pointers), _address(sizes), is_bf16, n, max_norm, at, at + 4, _at(ws), ws.numel(), stream()))
+    return out
 
 
 def grad_norm(grads, max_norm):
@@ -825,7 +844,8 @@ def grad_norm(grads, max_norm):
     if any(g.dtype is torch.bfloat16 for g in grads):
         kinds = bytes(g.dtype is torch.bfloat16 for g in grads)
     with _on(device):
-        return _grad_norm(_addresses(grads), array.array("q", [g.numel() for g in grads]), kinds, max_norm, device)
+        out = _grad_norm(_addresses(grads), array.array("q", [g.numel() for g in grads]), kinds, float(max_norm), device)
+    return out[:1], out[1:]
 
 
 def clip_grad_norm(params, max_norm):
@@ -869,7 +889,9 @@ class AdamWList:
                 raise RuntimeError("AdamWList: the same tensor twice")
         self.sizes = [p.numel() for p in params]
         self._n = array.array("q", self.sizes)
-        self._elems = sum(self.sizes)
+        self._bf16 = int(self.dtype is torch.bfloat16)
+        self._kinds = b"\1" * len(params) if self._bf16 else None
+        self._pointers = [*map(_address, self._arrays), _address(self._n)]
 
     def step(self, grads, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, coef=None, max_norm=None, seed=0):
         """One step with `grads` (of the parameters' type and sizes).  coef: device scalar that scales the gradients; max_norm
@@ -897,19 +919,20 @@ class AdamWList:
             _same("AdamWList.step", [coef], (torch.float32,), self.device)
             if coef.numel() != 1:
                 raise RuntimeError("AdamWList.step: coef is one value")
-        norm = None
+        norm = dyn = None
+        scale = _at(coef)
         with _on(self.device):
             if not on_device and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamWList.step: a captured step would repeat one step count: pass `step` as a CUDA int32 tensor")
             g = _addresses(grads)
             if max_norm is not None:
-                norm, coef = _grad_norm(g, self._n, bytes([1]) * len(grads) if self.dtype is torch.bfloat16 else None, max_norm, self.device)
-            dyn = torch.empty(3, device=self.device, dtype=torch.float32) if on_device else None
-            P, M, V, S = map(_address, self._arrays)
-            check(_lib.lib().pt_train_adamw_multi(P, _address(g), M, V, S, _address(self._n), len(grads),
-                                                  int(self.dtype is torch.bfloat16), ptr(coef), lr, betas[0], betas[1], eps, weight_decay,
-                                                  0 if on_device else step, ptr(step) if on_device else None, ptr(dyn), seed & 0xFFFFFFFF,
-                                                  stream()))
+                out = _grad_norm(g, self._n, self._kinds, float(max_norm), self.device)
+                norm, scale = out[:1], out.data_ptr() + 4
+            if on_device:
+                dyn = torch.empty(3, device=self.device, dtype=torch.float32)
+            check(_lib.lib().pt_train_adamw_multi(self._pointers[0], _address(g), *self._pointers[1:], len(g), self._bf16, scale, lr, *betas, eps,
+                                                  weight_decay, 0 if on_device else step, _at(step) if on_device else None, _at(dyn),
+                                                  seed & 0xFFFFFFFF, stream()))
         return norm
 
 
