@@ -24,6 +24,8 @@ typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 // 8-bit moments.  A block of 256 values shares one fp32 scale = (largest magnitude) / TOP; a magnitude code is a float of four
 // exponent bits and M mantissa bits over the quantum `scale`: code c < 2^M stands for c, else for (2^M + (c mod 2^M)) 2^(c / 2^M - 1).
 // First moment: sign bit + M = 3 (TOP = 15 * 2^14).  Second moment, never negative: M = 4 (TOP = 31 * 2^14).
+// The parameters and moments pass through the step once: streaming loads and stores keep the gradients, which the norm has just read,
+// in the caches (norm and step over 40 M fp32 values: 281 -> 217 us, with 8-bit moments 266 -> 217 including the reading of them).
 // Codes are rounded stochastically: with b2 = 0.999 a second moment moves by a thousandth per step, far less than half a code
 // step (1/32 to 1/16 of the value), so rounding to nearest would leave it where it is for ever; a rounding whose MEAN is the
 // value follows.  A positive second moment never becomes code 0 (its square root divides).  The 32 random bits of a value are a
@@ -124,15 +126,16 @@ __device__ __forceinline__ unsigned short f2bf_sr(float x, unsigned r16) {
 }
 
 // What a tensor without the vector path (odd address) or the last block of a tensor does: one value at a time
-template <typename T>
+// NT: a streaming load
+template <bool NT = false, typename T>
 __device__ __forceinline__ void load4(const T* __restrict__ b, size_t e, size_t n, bool vec, float (&x)[4]) {
   if (vec) {
     if constexpr (sizeof(T) == 4) {
-      const f32x4 q = *reinterpret_cast<const f32x4*>(b + e);
+      const f32x4 q = NT ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(b + e)) : *reinterpret_cast<const f32x4*>(b + e);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = q[i];
     } else {
-      const u16x4 q = *reinterpret_cast<const u16x4*>(b + e);
+      const u16x4 q = NT ? __builtin_nontemporal_load(reinterpret_cast<const u16x4*>(b + e)) : *reinterpret_cast<const u16x4*>(b + e);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = bf2f(q[i]);
     }
@@ -147,7 +150,7 @@ __device__ __forceinline__ void load4(const T* __restrict__ b, size_t e, size_t 
 __device__ __forceinline__ void store4(float* __restrict__ b, size_t e, size_t n, bool vec, const float (&x)[4]) {
   if (vec) {
     const f32x4 q = {x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<f32x4*>(b + e) = q;
+    __builtin_nontemporal_store(q, reinterpret_cast<f32x4*>(b + e));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (e + i < n) b[e + i] = x[i];
@@ -156,21 +159,21 @@ __device__ __forceinline__ void store4(float* __restrict__ b, size_t e, size_t n
 __device__ __forceinline__ void store4(unsigned short* __restrict__ b, size_t e, size_t n, bool vec, const unsigned short (&x)[4]) {
   if (vec) {
     const u16x4 q = {x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<u16x4*>(b + e) = q;
+    __builtin_nontemporal_store(q, reinterpret_cast<u16x4*>(b + e));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (e + i < n) b[e + i] = x[i];
   }
 }
 __device__ __forceinline__ unsigned load4b(const unsigned char* __restrict__ b, size_t e, size_t n, bool vec) {
-  if (vec) return *reinterpret_cast<const unsigned*>(b + e);
+  if (vec) return __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(b + e));
   unsigned x = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) if (e + i < n) x |= (unsigned)b[e + i] << (8 * i);
   return x;
 }
 __device__ __forceinline__ void store4b(unsigned char* __restrict__ b, size_t e, size_t n, bool vec, unsigned x) {
-  if (vec) { *reinterpret_cast<unsigned*>(b + e) = x; return; }
+  if (vec) { __builtin_nontemporal_store(x, reinterpret_cast<unsigned*>(b + e)); return; }
 #pragma unroll
   for (int i = 0; i < 4; ++i) if (e + i < n) b[e + i] = (unsigned char)(x >> (8 * i));
 }
@@ -212,7 +215,7 @@ __device__ __forceinline__ void adamw_wave(const AdamTab& tab, const AdamHyper& 
   for (int k = 0; k < NB; ++k) {
     const size_t e = e0 + k * QBLOCK + lane * 4;
     const bool vec = FULL || (aligned && e + 4 <= n);
-    load4(P, e, n, vec, p[k]);
+    load4<true>(P, e, n, vec, p[k]);
     load4(G, e, n, vec, g[k]);
     if constexpr (S8) {
       cm[k] = load4b((const unsigned char*)tab.m[i], e, n, vec);
@@ -222,8 +225,8 @@ __device__ __forceinline__ void adamw_wave(const AdamTab& tab, const AdamHyper& 
       sm[k] = in ? tab.s[i][2 * b] : 0.f;
       sv[k] = in ? tab.s[i][2 * b + 1] : 0.f;
     } else {
-      load4((const float*)tab.m[i], e, n, vec, m[k]);
-      load4((const float*)tab.v[i], e, n, vec, v[k]);
+      load4<true>((const float*)tab.m[i], e, n, vec, m[k]);
+      load4<true>((const float*)tab.v[i], e, n, vec, v[k]);
     }
   }
   // 8-bit moments: the new moments of all four blocks, then the scales of these eight (block, moment) pairs in eight lanes at once:
@@ -431,12 +434,22 @@ template <typename T>
 __device__ __forceinline__ double sumsq_unit(const T* __restrict__ g, size_t e0, size_t n, bool aligned) {
   double s[4] = {0, 0, 0, 0};
   const size_t end = min(n, e0 + (size_t)NORM_UNIT);
-#pragma unroll 4
-  for (size_t e = e0 + threadIdx.x * 4; e < end; e += 1024) {
-    float x[4];
-    load4(g, e, n, aligned && e + 4 <= n, x);
+  if (aligned && end == e0 + NORM_UNIT) {
+    g += e0 + threadIdx.x * 4;
+#pragma unroll 8
+    for (int k = 0; k < NORM_UNIT / 1024; ++k) {
+      float x[4];
+      load4(g, (size_t)k * 1024, 0, true, x);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = fma((double)x[j], (double)x[j], s[j]);
+      for (int j = 0; j < 4; ++j) s[j] = fma((double)x[j], (double)x[j], s[j]);
+    }
+  } else {
+    for (size_t e = e0 + threadIdx.x * 4; e < end; e += 1024) {
+      float x[4];
+      load4(g, e, n, aligned && e + 4 <= n, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = fma((double)x[j], (double)x[j], s[j]);
+    }
   }
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
