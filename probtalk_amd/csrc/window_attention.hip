@@ -761,10 +761,15 @@ __global__ __launch_bounds__(256) void win_bwd_join_kernel(const WinArgs a, int 
 }
 
 // ---------------------------------------------------------------------------
-// One token: scores of G query heads of a group against the visible keys of a slice of the cache.  Bound by HBM (every visible key
-// and value is read once for all heads of the group), so it runs on the vector unit straight from memory: L lanes hold a key's
-// row (8 values each), the wave's 64 / L lane groups walk keys side by side, each with its own running maximum and sum, joined at
-// the end.  Few sequences: the visible keys are cut into slices, joined by a second kernel.
+// One token: scores of the query heads of a group against the visible keys of its sequence.  Bound by HBM: every visible key and value
+// is read once for all heads of the group.  Visible keys are cut into slices where there are few sequences, joined by a second kernel.
+//
+// win_step_kernel: on the vector unit straight from memory: L lanes hold a key's row (8 values each), the wave's 64 / L lane groups walk
+// keys side by side, each with its own running maximum and sum, joined at the end.  fp32, and few short sequences of either type.
+// win_step_group_kernel: bf16 on the matrix cores.
+// Read rates over all visible keys and values: 64 sequences of some 3100 keys, 64 heads over 8, D = 128: 140 us, 6.0 TB/s (vector unit: 303);
+// 32 heads over 8: 157 us for 986 MB, 6.3 TB/s (183); 8 over 8, D = 64, 393 MB: 75 us; one sequence of 18,000 keys, 74 MB: 18 us;
+// fp32, 214 MB: 40 us
 // ---------------------------------------------------------------------------
 struct StepArgs {
   const void* q; const void* k; const void* v; void* o; const int* lengths;
@@ -774,19 +779,17 @@ struct StepArgs {
   float* part;                                           // [B][H][splits][D + 2]: unnormalised output, maximum, sum
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool on, float (&x)[8]) {
-  typename Types<T>::frag f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = (T)0.f;
-  if (on) f = *reinterpret_cast<const typename Types<T>::frag*>(p);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (float)f[e];
+template <bool STREAM, typename F>
+__device__ __forceinline__ F load_cache(const F* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
 }
 
-template <typename T, int L, int G>
-__global__ __launch_bounds__(256) void win_step_kernel(const StepArgs a) {
-  constexpr int KW = 64 / L, U = 4;                      // keys side by side in a wave, and turns whose loads go out together
+// W waves: 16 where one workgroup takes all keys of its heads, 4 otherwise
+template <typename T, int L, int G, int W, bool STREAM>
+__global__ __launch_bounds__(W * 64) void win_step_kernel(const StepArgs a) {
+  constexpr int KW = 64 / L, U = W == 4 || sizeof(T) == 2 ? 4 : 2;   // keys side by side in a wave, and turns whose loads go out together
+  typedef typename Types<T>::frag frag;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane % L, sub = lane / L;
   const int groups = (a.H / a.Hk + G - 1) / G;
   const int split = blockIdx.x, kvh = blockIdx.y / groups, g0 = (blockIdx.y % groups) * G, b = blockIdx.z;
@@ -795,28 +798,35 @@ __global__ __launch_bounds__(256) void win_step_kernel(const StepArgs a) {
   // the visible keys in order: [0, ns) sinks, then [lo, len)
   const int lo = max(t - a.left, 0), ns = min(min(a.sinks, lo), len), seen = len > 0 ? ns + (len - lo) : 0;
   const int per = (seen + a.splits - 1) / a.splits, n0 = min(split * per, seen), n1 = min(n0 + per, seen);
-  const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + kvh * a.sk[2] + li * 8;
-  const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + kvh * a.sv[2] + li * 8;
   const bool in = li * 8 < a.D;
+  const int col = in ? li * 8 : 0;
+  const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + kvh * a.sk[2] + col;
+  const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + kvh * a.sv[2] + col;
+  const frag zero = {};
   float q[G][8], acc[G][8], m[G], l[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    load8((const T*)a.q + b * a.sq[0] + (h0 + min(g, heads - 1)) * a.sq[1] + li * 8, in, q[g]);
+    const frag f = *reinterpret_cast<const frag*>((const T*)a.q + b * a.sq[0] + (h0 + min(g, heads - 1)) * a.sq[1] + col);
     m[g] = -INFINITY;
     l[g] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { q[g][e] *= a.sc; acc[g][e] = 0.f; }
+    for (int e = 0; e < 8; ++e) { q[g][e] = in ? (float)f[e] * a.sc : 0.f; acc[g][e] = 0.f; }
   }
-  for (int n = n0 + wave * KW * U; n < n1; n += 4 * KW * U) {
-    float k[U][8], v[U][8];
-    bool on[U];
+  for (int n = n0 + wave * KW * U; n < n1; n += W * KW * U) {
+    frag k[U], v[U];
+    // all loads first, without branches: rows behind the slice repeat its last one, columns behind D the first ones, and both
+    // count as zeros, whatever they hold
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = n + u * KW + sub;
-      on[u] = i < n1;
-      const int j = i < ns ? i : lo + i - ns;
-      load8(K + (on[u] ? j : 0) * a.sk[1], on[u] && in, k[u]);
-      load8(V + (on[u] ? j : 0) * a.sv[1], on[u] && in, v[u]);
+      const int i = min(n + u * KW + sub, n1 - 1), j = i < ns ? i : lo + i - ns;
+      k[u] = load_cache<STREAM>(reinterpret_cast<const frag*>(K + j * a.sk[1]));
+      v[u] = load_cache<STREAM>(reinterpret_cast<const frag*>(V + j * a.sv[1]));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool on = in && n + u * KW + sub < n1;
+      k[u] = in ? k[u] : zero;
+      v[u] = on ? v[u] : zero;
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -825,10 +835,10 @@ __global__ __launch_bounds__(256) void win_step_kernel(const StepArgs a) {
       for (int u = 0; u < U; ++u) {
         float d = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d = fmaf(q[g][e], k[u][e], d);
+        for (int e = 0; e < 8; ++e) d = fmaf(q[g][e], (float)k[u][e], d);
 #pragma unroll
         for (int x = 1; x < L; x <<= 1) d += __shfl_xor(d, x);
-        s[u] = on[u] ? d : -INFINITY;
+        s[u] = n + u * KW + sub < n1 ? d : -INFINITY;
         mx = fmaxf(mx, s[u]);
       }
       const float base = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m[g] - base);
@@ -841,12 +851,12 @@ __global__ __launch_bounds__(256) void win_step_kernel(const StepArgs a) {
         const float p = __builtin_amdgcn_exp2f(s[u] - base);
         l[g] += p;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[g][e] = fmaf(p, v[u][e], acc[g][e]);
+        for (int e = 0; e < 8; ++e) acc[g][e] = fmaf(p, (float)v[u][e], acc[g][e]);
       }
     }
   }
   // join the lane groups, then the waves
-  __shared__ float red[4][G][L * 8 + 2];
+  __shared__ float red[W][G][L * 8 + 2];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     float top = m[g];
@@ -866,16 +876,16 @@ __global__ __launch_bounds__(256) void win_step_kernel(const StepArgs a) {
     if (lane == 0) { red[wave][g][L * 8] = top; red[wave][g][L * 8 + 1] = l[g]; }
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < heads * L * 8; x += 256) {
+  for (int x = threadIdx.x; x < heads * L * 8; x += W * 64) {
     const int g = x / (L * 8), d = x % (L * 8);
     if (d >= a.D) continue;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, red[w][g][L * 8]);
+    for (int w = 0; w < W; ++w) top = fmaxf(top, red[w][g][L * 8]);
     const float base = top == -INFINITY ? 0.f : top;
     float s = 0.f, y = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float f = __builtin_amdgcn_exp2f(red[w][g][L * 8] - base);
       s += f * red[w][g][L * 8 + 1];
       y += f * red[w][g][d];
@@ -890,22 +900,165 @@ __global__ __launch_bounds__(256) void win_step_kernel(const StepArgs a) {
     }
   }
 }
-template <typename T>
-__global__ __launch_bounds__(128) void win_step_join_kernel(const StepArgs a) {
-  const int64_t oh = blockIdx.x;
-  const int d = threadIdx.x;
-  if (d >= a.D) return;
-  const float* p = a.part + oh * a.splits * (a.D + 2);
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, p[s * (a.D + 2) + a.D]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float l = 0.f, y = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(p[s * (a.D + 2) + a.D] - base);
-    l += f * p[s * (a.D + 2) + a.D + 1];
-    y += f * p[s * (a.D + 2) + d];
+
+// The same in bf16: up to 32 heads of a group are the columns of a 32 x 32 tile, 32 keys its rows, as in the forward kernel.  Columns
+// without a head cost matrix time that the loads leave over: with one head in use it is as fast as the vector unit, with eight, where
+// the vector unit is the bound, more than twice.  Every wave walks tiles of its own through LDS-DMA into two buffers, without
+// barriers; probabilities are rounded to bf16 for the second product (an output in bf16 is rounded as much), their sum is of the
+// unrounded ones.
+constexpr int STEP_WAVES = 4;
+template <int DP, bool STREAM>
+__global__ __launch_bounds__(STEP_WAVES * 64) void win_step_group_kernel(const StepArgs a) {
+  typedef __bf16 T;
+  typedef Tile<T, DP> tile;
+  constexpr int RB = tile::RB, TB = 32 * RB, ROWS = 1024 / RB, N = 32 / ROWS, ND = DP / 32, W = STEP_WAVES;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+  const int group = a.H / a.Hk, groups = (group + 31) / 32;
+  const int split = blockIdx.x, kvh = blockIdx.y / groups, g0 = (blockIdx.y % groups) * 32, b = blockIdx.z;
+  const int heads = min(32, group - g0), h0 = kvh * group + g0;
+  const int len = min(max(a.lengths[b], 0), a.N), t = len - 1;
+  const int lo = max(t - a.left, 0), ns = min(min(a.sinks, lo), len), seen = len > 0 ? ns + (len - lo) : 0;
+  const int per = ((seen + a.splits - 1) / a.splits + 31) / 32 * 32, n0 = min(split * per, seen), n1 = min(n0 + per, seen);
+  const char* K = (const char*)((const T*)a.k + b * a.sk[0] + kvh * a.sk[2]);
+  const char* V = (const char*)((const T*)a.v + b * a.sv[0] + kvh * a.sv[2]);
+  unsigned char* m = lds + wave * 4 * TB;                // two buffers of keys and values
+  const int row = lane * 16 / RB, chunk = (lane * 16 % RB / 16) ^ tile::swz(row);
+  auto fetch = [&](int n, unsigned char* to) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = min(n + i * ROWS + row, n1 - 1), j = x < ns ? x : lo + x - ns, at = chunk ^ tile::swz(i * ROWS & 15);
+      const int col = at * 8 < a.D ? at * 16 : 0;
+      __builtin_amdgcn_global_load_lds((glb_ptr_t)(K + j * a.sk[1] * 2 + col), (lds_ptr_t)(to + i * 1024), 16, 0, STREAM ? 2 : 0);
+      __builtin_amdgcn_global_load_lds((glb_ptr_t)(V + j * a.sv[1] * 2 + col), (lds_ptr_t)(to + TB + i * 1024), 16, 0, STREAM ? 2 : 0);
+    }
+  };
+  const int first = n0 + wave * 32;
+  if (first < n1) fetch(first, m);
+  bf16x8 q[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) q[s] = global_frag<T>((const T*)a.q + b * a.sq[0] + h0 * a.sq[1], a.sq[1], c, heads, 16 * s + 8 * h, a.D);
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = zero16();
+  float top = -INFINITY, l = 0.f;
+  const int kb = tile::row_base(c, h), vb = tile::col_base(lane);
+  int turn = 0;
+  for (int n = first; n < n1; n += W * 32, turn ^= 1) {
+    unsigned char* now = m + turn * 2 * TB;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (n + W * 32 < n1) fetch(n + W * 32, m + (turn ^ 1) * 2 * TB);
+    f32x16 st = zero16();
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) st = mma(tile::row_frag(now, kb, s), q[s], st);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      st[r] *= a.sc;
+      if (n + 32 > n1) st[r] = n + (r & 3) + 8 * (r >> 2) + 4 * h < n1 ? st[r] : -INFINITY;
+      mx = fmaxf(mx, st[r]);
+    }
+    mx = fmaxf(mx, half_other(mx));
+    const float up = fmaxf(top, mx), base = up == -INFINITY ? 0.f : up, alpha = __builtin_amdgcn_exp2f(top - base);
+    top = up;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] *= alpha;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      st[r] = __builtin_amdgcn_exp2f(st[r] - base);
+      l += st[r];
+    }
+    bf16x8 f[2][ND];
+    Cols<T, DP>(now + TB, vb).template read<0>(f);
+    add_product<T, DP>(acc, f, st);
   }
-  ((T*)a.o)[oh * a.D + d] = (T)(l == 0.f ? 0.f : y / l);
+  l += half_other(l);
+  // join the waves
+  float* red = (float*)lds;                              // [W][heads][DP + 4]: output, maximum, sum
+  constexpr int RW = DP + 4;
+  __syncthreads();
+  if (c < heads) {
+    float* out = red + (wave * heads + c) * RW;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = {acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+        *reinterpret_cast<f32x4*>(out + d * 32 + 8 * g + 4 * h) = x;
+      }
+    if (!h) { out[DP] = top; out[DP + 1] = l; }
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < heads * DP; x += W * 64) {
+    const int g = x / DP, d = x % DP;
+    if (d >= a.D) continue;
+    float most = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) most = fmaxf(most, red[(w * heads + g) * RW + DP]);
+    const float base = most == -INFINITY ? 0.f : most;
+    float s = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float* in = red + (w * heads + g) * RW;
+      const float f = __builtin_amdgcn_exp2f(in[DP] - base);
+      s += f * in[DP + 1];
+      y += f * in[d];
+    }
+    const int64_t oh = (int64_t)b * a.H + h0 + g;
+    if (a.splits == 1) {
+      ((T*)a.o)[oh * a.D + d] = (T)(s == 0.f ? 0.f : y / s);
+    } else {
+      float* out = a.part + (oh * a.splits + split) * (a.D + 2);
+      out[d] = y;
+      if (d == 0) { out[a.D] = most; out[a.D + 1] = s; }
+    }
+  }
+}
+// Joins the slices of one head: a lane takes the maximum and the sum of every 64th slice, a thread a column of every JOIN-th (8; 2 where there
+// are no more than 8 slices: 512 heads of 2 slices, 3.5 us less)
+constexpr int STEP_SPLITS = 256;
+template <typename T, int JOIN>
+__global__ __launch_bounds__(JOIN * 128) void win_step_join_kernel(const StepArgs a) {
+  const int64_t oh = blockIdx.x;
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 7, col = threadIdx.x & 127, d = min(col, a.D - 1), row = a.D + 2;
+  const float* p = a.part + oh * a.splits * row;
+  float w[STEP_SPLITS / 64], y[64 / JOIN], l = 0.f, top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < STEP_SPLITS / 64; ++i) {
+    w[i] = i * 64 + lane < a.splits ? p[(i * 64 + lane) * row + a.D] : -INFINITY;
+    top = fmaxf(top, w[i]);
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < STEP_SPLITS / 64; ++i) {
+    w[i] = __builtin_amdgcn_exp2f(w[i] - base);
+    if (i * 64 + lane < a.splits) l += w[i] * p[(i * 64 + lane) * row + a.D + 1];
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < STEP_SPLITS / 64; ++i) {
+    if (i * 64 >= a.splits) break;
+#pragma unroll
+    for (int s = 0; s < 64 / JOIN; ++s) y[s] = p[min(i * 64 + s * JOIN + part, a.splits - 1) * row + d];
+#pragma unroll
+    for (int s = 0; s < 64 / JOIN; ++s) {
+      const float f = __shfl(w[i], s * JOIN + part);
+      if (i * 64 + s * JOIN + part < a.splits) sum += f * y[s];
+    }
+  }
+  __shared__ float red[JOIN][128];
+  red[part][col] = sum;
+  __syncthreads();
+  if ((int)threadIdx.x >= a.D) return;
+  sum = 0.f;
+#pragma unroll
+  for (int x = 0; x < JOIN; ++x) sum += red[x][threadIdx.x];
+  ((T*)a.o)[oh * a.D + d] = (T)(l == 0.f ? 0.f : sum / l);
 }
 
 // ---------------------------------------------------------------------------
@@ -1020,30 +1173,67 @@ int launch_window_bwd(const void* q, const void* k, const void* v, const void* o
   return D <= 64 ? run_win_bwd<float, 64>(a, s) : run_win_bwd<float, 128>(a, s);
 }
 
-// Slices of the visible keys: enough workgroups for every CU (four each), none with fewer than 64 keys
-static int step_splits(int B, int N, int H, int Hk, int left, int sinks) {
-  const int group = H / Hk, groups = (group + 7) / 8;
-  const int64_t most = std::min<int64_t>(N, (int64_t)(left < 0 ? N : left) + 1 + sinks), units = (int64_t)B * Hk * groups;
-  const int64_t want = ((int64_t)device_cus() * 4 + units - 1) / units;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, (most + 63) / 64), 256));
+// How a call is cut.  whole: one workgroup of 16 waves takes all visible keys of a group's heads, and there is no second kernel: few
+// units of few keys, whose time is latency (one sequence of 516 keys: 20.8 -> 15.4 us a call against nine slices and their join; four of
+// 1000: 6.7 us on the GPU against 9.6).  matrix: win_step_group_kernel.  stream: loads that leave the caches alone, where the cache of
+// the step will not stay there: bf16 from 64 MB on (836 MB 158 -> 140 us; 202 MB, six in turn, 51 -> 45; one alone 41 -> 42), fp32
+// from the 256 MB of Infinity Cache on (214 MB, alone and resident: 40 us against 55).
+struct StepPlan { bool whole, matrix, stream; int heads, splits; };
+static StepPlan step_plan(int B, int N, int H, int Hk, int D, int left, int sinks, int dtype) {
+  const int group = H / Hk;
+  const int64_t most = std::min<int64_t>(N, (int64_t)(left < 0 ? N : left) + 1 + sinks), bytes = B * (int64_t)Hk * most * D * (dtype ? 2 : 4) * 2;
+  StepPlan p = {};
+  p.whole = group <= 2 && most <= 1024 && (int64_t)B * Hk <= device_cus();
+  p.matrix = dtype && !p.whole;
+  p.stream = bytes >= (int64_t)(p.matrix ? 64 : 256) << 20;
+  p.heads = p.matrix ? 32 : group == 1 ? 1 : group == 2 ? 2 : group <= 4 ? 4 : 8;
+  // slices of the visible keys: as many workgroups as are there at once (LDS, or the registers of the vector kernel), none with fewer
+  // than 64 keys.  Twice as many: B = 8, 53 MB 16 -> 20 us
+  const int64_t at_once = (int64_t)device_cus() * (p.matrix && D > 64 ? 1 : 2), units = (int64_t)B * Hk * ((group + p.heads - 1) / p.heads);
+  const int64_t slices = std::min<int64_t>(std::min<int64_t>((at_once + units - 1) / units, (most + 63) / 64), STEP_SPLITS);
+  p.splits = p.whole ? 1 : (int)std::max<int64_t>(1, slices);
+  return p;
 }
 size_t window_step_workspace(int B, int N, int H, int Hk, int D, int left, int sinks) {
   if (check_win("attention_window_step", B, 1, N, H, Hk, D, left, 0, sinks, 1.f, 0)) return 0;
-  const int n = step_splits(B, N, H, Hk, left, sinks);
+  const int n = std::max(step_plan(B, N, H, Hk, D, left, sinks, 0).splits, step_plan(B, N, H, Hk, D, left, sinks, 1).splits);
   return n == 1 ? 16 : (size_t)B * H * n * (D + 2) * sizeof(float);
 }
 
-template <typename T, int L, int G>
-static int run_step(const StepArgs& a, hipStream_t s) {
-  const int groups = (a.H / a.Hk + G - 1) / G;
-  PT_LAUNCH((win_step_kernel<T, L, G>), dim3(a.splits, a.Hk * groups, a.B), dim3(256), 0, s, a);
-  if (a.splits > 1) PT_LAUNCH(win_step_join_kernel<T>, dim3((unsigned)(a.B * a.H)), dim3(128), 0, s, a);
+template <typename T, int L, int G, int W>
+static int run_step(const StepArgs& a, const StepPlan& p, hipStream_t s) {
+  const dim3 grid(a.splits, a.Hk * ((a.H / a.Hk + G - 1) / G), a.B);
+  if (p.stream) PT_LAUNCH((win_step_kernel<T, L, G, W, true>), grid, dim3(W * 64), 0, s, a);
+  else PT_LAUNCH((win_step_kernel<T, L, G, W, false>), grid, dim3(W * 64), 0, s, a);
   return 0;
 }
 template <typename T, int L>
-static int run_step(const StepArgs& a, hipStream_t s) {
-  const int group = a.H / a.Hk;
-  return group == 1 ? run_step<T, L, 1>(a, s) : group == 2 ? run_step<T, L, 2>(a, s) : group <= 4 ? run_step<T, L, 4>(a, s) : run_step<T, L, 8>(a, s);
+static int run_step(const StepArgs& a, const StepPlan& p, hipStream_t s) {
+  if (p.whole) return p.heads == 1 ? run_step<T, L, 1, 16>(a, p, s) : run_step<T, L, 2, 16>(a, p, s);
+  if constexpr (sizeof(T) == 4)
+    return p.heads == 1 ? run_step<T, L, 1, 4>(a, p, s) : p.heads == 2 ? run_step<T, L, 2, 4>(a, p, s)
+                        : p.heads == 4 ? run_step<T, L, 4, 4>(a, p, s) : run_step<T, L, 8, 4>(a, p, s);
+  else return 1;
+}
+template <int DP>
+static int run_step_group(const StepArgs& a, const StepPlan& p, hipStream_t s) {
+  constexpr int lds = STEP_WAVES * 4 * 32 * Tile<__bf16, DP>::RB;
+  static_assert(lds >= STEP_WAVES * 32 * (DP + 4) * 4 && lds <= 128 * 1024, "buffers that LDS-DMA reaches");
+  const dim3 grid(a.splits, a.Hk * ((a.H / a.Hk + 31) / 32), a.B);
+  if (p.stream) {
+    PT_ENSURE_LDS((win_step_group_kernel<DP, true>), lds);
+    PT_LAUNCH((win_step_group_kernel<DP, true>), grid, dim3(STEP_WAVES * 64), lds, s, a);
+  } else {
+    PT_ENSURE_LDS((win_step_group_kernel<DP, false>), lds);
+    PT_LAUNCH((win_step_group_kernel<DP, false>), grid, dim3(STEP_WAVES * 64), lds, s, a);
+  }
+  return 0;
+}
+
+template <typename T, int JOIN>
+static int run_step_join(const StepArgs& a, hipStream_t s) {
+  PT_LAUNCH((win_step_join_kernel<T, JOIN>), dim3((unsigned)((int64_t)a.B * a.H)), dim3(JOIN * 128), 0, s, a);
+  return 0;
 }
 
 int launch_window_step(const void* q, const void* k, const void* v, void* o, const int64_t* st, const int* lengths, int B, int N, int H, int Hk, int D,
@@ -1059,10 +1249,16 @@ int launch_window_step(const void* q, const void* k, const void* v, void* o, con
   for (int i = 0; i < 2; ++i) a.sq[i] = st[i];
   for (int i = 0; i < 3; ++i) { a.sk[i] = st[2 + i]; a.sv[i] = st[5 + i]; }
   a.B = B; a.N = N; a.H = H; a.Hk = Hk; a.D = D; a.left = left < 0 || left > WIN_FAR ? WIN_FAR : left; a.sinks = sinks; a.sc = scale * LOG2E;
-  a.splits = step_splits(B, N, H, Hk, left, sinks);
+  const StepPlan p = step_plan(B, N, H, Hk, D, left, sinks, dtype);
+  a.splits = p.splits;
   a.part = (float*)ws;
-  if (dtype) return D <= 64 ? run_step<__bf16, 8>(a, s) : run_step<__bf16, 16>(a, s);
-  return D <= 64 ? run_step<float, 8>(a, s) : run_step<float, 16>(a, s);
+  if (p.matrix ? (D <= 64 ? run_step_group<64>(a, p, s) : run_step_group<128>(a, p, s))
+               : dtype ? (D <= 64 ? run_step<__bf16, 8>(a, p, s) : run_step<__bf16, 16>(a, p, s))
+                       : (D <= 64 ? run_step<float, 8>(a, p, s) : run_step<float, 16>(a, p, s)))
+    return 1;
+  if (p.splits == 1) return 0;
+  if (p.splits <= 8) return dtype ? run_step_join<__bf16, 2>(a, s) : run_step_join<float, 2>(a, s);
+  return dtype ? run_step_join<__bf16, 8>(a, s) : run_step_join<float, 8>(a, s);
 }
 
 }  // namespace pt

@@ -268,7 +268,7 @@ def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias
     if torch.is_grad_enabled() and any([v is not None and v.requires_grad for v in given]):
         y, h = GatedNorm.apply(*given, clip, mode, eps)
     else:
-        y, h, _ = _gated_norm(*(v if v is None else v.detach() for v in given), clip, mode, eps, False)
+        y, h, _ = _gated_norm(*given, clip, mode, eps, False)
     return (own if t is None else y), h
 
 
@@ -451,7 +451,6 @@ def window_attention_step(q, k, v, lengths, left=None, sinks=0, scale=None):
     if lengths is None:
         raise RuntimeError("window_attention_step: lengths are needed")
     left, _, sinks, scale = _check_window("window_attention_step", q, k, v, q.shape[1], q.shape[0], lengths, left, 0, sinks, scale)
-    q, k, v = q.detach(), k.detach(), v.detach()
     if not _has_vectors(k) or not _has_vectors(v):
         raise RuntimeError("window_attention_step: a cache's channels must be neighbours, its address and strides multiples of 16 bytes")
     q = _vectors(q)
