@@ -192,13 +192,14 @@ int pt_attention_bf16(const void* Q, int ldq, const void* K, int ldk, const void
  * rows at most 2^20 values apart.
  * Row i stands at position t = i + Nk - Nq and sees key j where j <= t + right and (j >= t - left or j < sinks) and j < lengths[b].
  * left, right: -1 = no limit; sinks <= 128; lengths: B device int32 (NULL: Nk), taken into [0, Nk]; keys behind are not read.  A row
- * that sees nothing gives zeros.  o, dout, dq (B, Nq, H, D) and dk, dv (B, Nk, Hk, D) are contiguous; lse [B][H][Nq] (16-byte aligned, NULL:
- * not wanted) is what the backward call needs.  Inside lengths[b] keys and values must be finite: one that is not may reach rows
+ * that sees nothing gives zeros.  o, dout, dq (B, Nq, H, D) and dk, dv (B, Nk, Hk, D) are contiguous; stats (16-byte aligned, of
+ * stats_bytes; NULL: not wanted) is what the backward call needs.  Inside lengths[b] keys and values must be finite: one that is not may reach rows
  * within 128 positions of those that see it. */
-int pt_attention_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* strides, const int32_t* lengths, int B,
+size_t pt_attention_window_stats_bytes(int B, int Nq, int Nk, int H, int D, int left, int right, int sinks, int dtype);
+int pt_attention_window_fwd(const void* q, const void* k, const void* v, void* o, void* stats, const int64_t* strides, const int32_t* lengths, int B,
                             int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, void* stream);
 size_t pt_attention_window_bwd_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks);
-int pt_attention_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv,
+int pt_attention_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const void* stats, void* dq, void* dk, void* dv,
                             const int64_t* strides, const int32_t* lengths, int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks,
                             float scale, int dtype, void* ws, size_t ws_bytes, void* stream);
 /* The same for one token per sequence over a cache: q (B, H, D), k and v (B, N, Hk, D), strides: batch and head of q, then batch, row

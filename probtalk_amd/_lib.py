@@ -104,6 +104,8 @@ def _proto(lib):
     lib.pt_train_commit_bwd.argtypes = [vp, vp, vp, vp, f, sz, vp, vp]
     lib.pt_set_option.argtypes = [C.c_char_p, i]
     lib.pt_get_option.argtypes = [C.c_char_p, vp]
+    lib.pt_attention_window_stats_bytes.restype = sz
+    lib.pt_attention_window_stats_bytes.argtypes = [i] * 9
     lib.pt_attention_window_bwd_workspace_bytes.restype = lib.pt_attention_window_step_workspace_bytes.restype = sz
     lib.pt_attention_window_bwd_workspace_bytes.argtypes = [i] * 9
     lib.pt_attention_window_step_workspace_bytes.argtypes = [i] * 7
@@ -126,7 +128,7 @@ EXPORTS = [
     "pt_predictor_workspace_bytes", "pt_predictor_condition", "pt_predictor_logits", "pt_predictor_sample", "pt_predictor_sample_seeded", "pt_predictor_sample_seed_dev", "pt_maskgit_noise", "pt_maskgit_noise_from_bits",
     "pt_refiner_workspace_bytes", "pt_refiner_forward", "pt_interp_blend", "pt_conv1d_cl", "pt_ncl_to_cl",
     "pt_cl_to_ncl", "pt_pq_search_cl", "pt_pq_gather_cl", "pt_attention_cl", "pt_attention_bf16",
-    "pt_attention_window_fwd", "pt_attention_window_bwd_workspace_bytes", "pt_attention_window_bwd",
+    "pt_attention_window_stats_bytes", "pt_attention_window_fwd", "pt_attention_window_bwd_workspace_bytes", "pt_attention_window_bwd",
     "pt_attention_window_step_workspace_bytes", "pt_attention_window_step", "pt_gemm_bf16", "pt_gemm_bf16_lnmod",
     "pt_gemm_bf16_addln", "pt_gemm_bf16_sublayer", "pt_permute_k32", "pt_conv1d_cl_bf16", "pt_postprocess_poses", "pt_prof_enable",
     "pt_prof_read", "pt_embed_pe", "pt_train_wgrad", "pt_train_wgrad_bias", "pt_train_colsum", "pt_train_ln_fwd", "pt_train_ln_bwd",

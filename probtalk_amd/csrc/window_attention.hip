@@ -69,6 +69,7 @@ struct WinArgs {
   void* o; float* lse;                                   // lse [B][H][Nq], in powers of two; +inf for a row that sees nothing
   const void* od; const void* dod;                       // backward: o and its gradient, (B, Nq, H, D)
   void* dq; void* dk; void* dv; float* delta;            // delta [B][H][Nq]
+  signed char* rest;                                     // what o lost when it was rounded, a byte a value (see rest_of), or null
   float* part;                                           // shares of the first keys' gradients (see win_bwd_sink_kernel)
   int64_t sq[3], sk[3], sv[3];                           // strides of batch, row, head in values
   const int* lengths;
@@ -193,8 +194,8 @@ struct Cols<float, DP> {
         }
   }
 };
-// acc[db] += (columns of 32 rows)^T . p, p the registers of a score tile over these rows
-template <typename T, int DP>
+// acc[db] += (columns of 32 rows)^T . p, p the registers of a score tile over these rows.  WIDE: p as the sum of two bf16 values
+template <typename T, int DP, bool WIDE = false>
 __device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const typename Types<T>::frag (&f)[2][DP / 32], const f32x16& p) {
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
@@ -203,7 +204,22 @@ __device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const typena
     for (int e = 0; e < 8; ++e) x[e] = (T)p[8 * s2 + e];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], x, acc[db]);
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (T)(p[8 * s2 + e] - (float)x[e]);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], x, acc[db]);
+    }
   }
+}
+// What a value lost when it was rounded to bf16, in steps of its 24-bit pattern (-128 to 128, of which 128 is taken for 127), and the value
+// that both stand for, off by a step and a half of 2^-15 at most
+__device__ __forceinline__ int rest_of(float x, __bf16 r) {
+  const int d = (int)(__builtin_bit_cast(unsigned, x) - ((unsigned)__builtin_bit_cast(unsigned short, r) << 16));
+  return min((d + 0x80) >> 8, 127);
+}
+__device__ __forceinline__ float with_rest(__bf16 r, int rest) {
+  return __builtin_bit_cast(float, ((unsigned)__builtin_bit_cast(unsigned short, r) << 16) + (unsigned)(rest * 256));
 }
 
 // R rows of a tile straight from memory to LDS (LDS-DMA: no registers, nothing for the compiler to wait for), by TH threads.  A wave
@@ -272,20 +288,47 @@ __device__ __forceinline__ typename Types<T>::frag global_frag(const T* __restri
   if (row < limit && c < D) f = *reinterpret_cast<const typename Types<T>::frag*>(base + row * stride + c);
   return f;
 }
-// a transposed result (lane: row `row` of the output, registers: columns) times x
+// a transposed result (lane: row `row` of the output, registers: columns) times x.  bf16: the two lanes of a row swap, so that each has
+// eight neighbours to store
 template <typename T, int DP>
-__device__ __forceinline__ void store_transposed(T* __restrict__ base, const f32x16 (&acc)[DP / 32], int h, int D, float x) {
-  typedef typename Types<T>::quad quad;
+__device__ __forceinline__ void store_transposed(T* __restrict__ base, const f32x16 (&acc)[DP / 32], int h, int D, float x, signed char* rest = nullptr) {
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
+  for (int db = 0; db < DP / 32; ++db) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int c = db * 32 + 8 * g + 4 * h;
-      if (c < D) {
-        const quad o = {(T)(acc[db][4 * g] * x), (T)(acc[db][4 * g + 1] * x), (T)(acc[db][4 * g + 2] * x), (T)(acc[db][4 * g + 3] * x)};
-        *reinterpret_cast<quad*>(base + c) = o;
+      for (int g = 0; g < 4; ++g) {
+        const int c = db * 32 + 8 * g + 4 * h;
+        const f32x4 o = {acc[db][4 * g] * x, acc[db][4 * g + 1] * x, acc[db][4 * g + 2] * x, acc[db][4 * g + 3] * x};
+        if (c < D) *reinterpret_cast<f32x4*>(base + c) = o;
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        unsigned w[2][2], r[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          bf16x4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = acc[db][4 * (g + k) + e] * x;
+            o[e] = (__bf16)y;
+            r[k] |= (unsigned)(rest_of(y, o[e]) & 255) << 8 * e;
+          }
+          const uint2 u = __builtin_bit_cast(uint2, o);
+          w[k][0] = u.x; w[k][1] = u.y;
+        }
+        const auto s0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false), s1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+        const int c = db * 32 + 8 * (g + h);
+        const u32x4 o = {s0[0], s1[0], s0[1], s1[1]};
+        if (c < D) *reinterpret_cast<u32x4*>(base + c) = o;
+        if (rest) {
+          const auto s = __builtin_amdgcn_permlane32_swap(r[0], r[1], false, false);
+          const uint2 y = {s[0], s[1]};
+          if (c < D) *reinterpret_cast<uint2*>(rest + c) = y;
+        }
       }
     }
+  }
 }
 
 // Key tiles of KT that rows at positions [t0, t1] may see: [0, first) for the sinks, then [from, to)
@@ -331,7 +374,7 @@ template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 2 |
 // ---------------------------------------------------------------------------
 // Forward: 4 waves of 32 rows each over common key tiles
 // ---------------------------------------------------------------------------
-template <typename T, int DP>
+template <typename T, int DP, bool WIDE>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fwd_kernel(const WinArgs a) {
   constexpr int KT = key_tile<T, DP>(), NB = KT / 32;
   constexpr bool BF = sizeof(T) == 2;
@@ -419,17 +462,18 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
           l += st[x][r];                                                 // this lane's half of the column; joined at the end
         }
       if constexpr (!BF) vc.template read<0>(vf[0]);
-      add_product<T, DP>(o, vf[0], st[0]);                               // probabilities in [0, 1] to bf16: 2^-9 of each
+      add_product<T, DP, WIDE>(o, vf[0], st[0]);                         // probabilities in [0, 1] to bf16: 2^-9 of each; WIDE: 2^-17
       if constexpr (NB > 1) {
         if constexpr (!BF) vc.template read<32 * tile::RB>(vf[1]);
-        add_product<T, DP>(o, vf[1], st[1]);
+        add_product<T, DP, WIDE>(o, vf[1], st[1]);
       }
     }
     dma_wait();
   }
   if (row >= a.Nq) return;
   l += half_other(l);
-  store_transposed<T, DP>((T*)a.o + (((int64_t)b * a.Nq + row) * a.H + head) * a.D, o, h, a.D, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
+  const int64_t out = (((int64_t)b * a.Nq + row) * a.H + head) * a.D;
+  store_transposed<T, DP>((T*)a.o + out, o, h, a.D, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), WIDE && a.rest ? a.rest + out : nullptr);
   if (a.lse && h == 0) a.lse[((int64_t)b * a.H + head) * a.Nq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -469,6 +513,13 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
     qf[s] = global_frag(Q, a.sq[1], row, a.Nq, 16 * s + 8 * h, a.D);
     gf[s] = global_frag((const T*)a.dod + ob, so, row, a.Nq, 16 * s + 8 * h, a.D);
     const auto of = global_frag((const T*)a.od + ob, so, row, a.Nq, 16 * s + 8 * h, a.D);
+    if constexpr (BF)
+      if (a.rest && row < a.Nq && 16 * s + 8 * h < a.D) {
+        const uint2 w = *reinterpret_cast<const uint2*>(a.rest + ob + row * so + 16 * s + 8 * h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta += (float)gf[s][e] * with_rest(of[e], (signed char)((e < 4 ? w.x : w.y) >> 8 * (e & 3)));
+        continue;
+      }
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta += (float)gf[s][e] * (float)of[e];
   }
@@ -1109,12 +1160,26 @@ static WinArgs win_args(const void* q, const void* k, const void* v, const int64
 
 static int64_t win_blocks(const WinArgs& a) { return (int64_t)((a.Nq + 127) / 128) * a.H * a.B; }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WIDE = false>
 static int run_win_fwd(const WinArgs& a, hipStream_t s) {
   constexpr int lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB;
-  PT_ENSURE_LDS((win_fwd_kernel<T, DP>), lds);
-  PT_LAUNCH((win_fwd_kernel<T, DP>), dim3((unsigned)win_blocks(a)), dim3(256), lds, s, a);
+  PT_ENSURE_LDS((win_fwd_kernel<T, DP, WIDE>), lds);
+  PT_LAUNCH((win_fwd_kernel<T, DP, WIDE>), dim3((unsigned)win_blocks(a)), dim3(256), lds, s, a);
   return 0;
+}
+// bf16 rows that see at most 512 keys: the rounding of few probabilities does not average out, and dQ, dK feel it in o through delta.
+// There the probabilities enter o's product as sums of two bf16 values and o keeps a byte more for delta: error of dQ and dK for 3 / 129
+// visible keys 2.2 / 1.53 -> 1.42 times that of rounding the exact result (what is left is dS in bf16); beyond 512 keys it is
+// 1.47 at most without.  8192 rows, 16 heads over 4, D = 128, 256 keys: forward 43 -> 53 us, with gradients 183 -> 205; 1024 keys would be 375 -> 410
+constexpr int WIDE_MAX = 512;
+static bool window_wide(int Nk, int left, int right, int sinks, int dtype) {
+  const int64_t seen = left < 0 || right < 0 ? Nk : std::min<int64_t>(Nk, (int64_t)left + right + 1 + sinks);
+  return dtype && seen <= WIDE_MAX;
+}
+static size_t lse_bytes(int B, int Nq, int H) { return ((size_t)B * H * Nq * 4 + 255) / 256 * 256; }
+size_t window_stats_bytes(int B, int Nq, int Nk, int H, int D, int left, int right, int sinks, int dtype) {
+  if (check_win("attention_window_fwd", B, Nq, Nk, H, H, D, left, right, sinks, 1.f, dtype)) return 0;
+  return lse_bytes(B, Nq, H) + (window_wide(Nk, left, right, sinks, dtype) ? (size_t)B * Nq * H * D : 0);
 }
 template <typename T, int DP>
 static int run_win_bwd(const WinArgs& a, hipStream_t s) {
@@ -1132,16 +1197,20 @@ static int run_win_bwd(const WinArgs& a, hipStream_t s) {
   return 0;
 }
 
-int launch_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* st, const int* lengths, int B, int Nq, int Nk,
+int launch_window_fwd(const void* q, const void* k, const void* v, void* o, void* stats, const int64_t* st, const int* lengths, int B, int Nq, int Nk,
                       int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, hipStream_t s) {
   if (check_win("attention_window_fwd", B, Nq, Nk, H, Hk, D, left, right, sinks, scale, dtype)) return 1;
   PT_CHECK(q && k && v && o && st, "attention_window_fwd: null argument");
   PT_CHECK(aligned16(q, st, 3, dtype) && aligned16(k, st + 3, 3, dtype) && aligned16(v, st + 6, 3, dtype) && !((uintptr_t)o & 15),
            "attention_window_fwd: addresses and strides must be multiples of 16 bytes");
   PT_CHECK(near_rows(st) && (int64_t)H * D <= (1 << 20), "attention_window_fwd: rows are more than 2^20 values apart");
-  const WinArgs w = win_args(q, k, v, st, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale);
-  WinArgs a = w;
-  a.o = o; a.lse = lse;
+  PT_CHECK(!((uintptr_t)stats & 15), "attention_window_fwd: stats must be aligned to 16 bytes");
+  WinArgs a = win_args(q, k, v, st, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale);
+  a.o = o; a.lse = (float*)stats;
+  if (window_wide(Nk, left, right, sinks, dtype)) {
+    a.rest = stats ? (signed char*)stats + lse_bytes(B, Nq, H) : nullptr;
+    return D <= 64 ? run_win_fwd<__bf16, 64, true>(a, s) : run_win_fwd<__bf16, 128, true>(a, s);
+  }
   if (dtype) return D <= 64 ? run_win_fwd<__bf16, 64>(a, s) : run_win_fwd<__bf16, 128>(a, s);
   return D <= 64 ? run_win_fwd<float, 64>(a, s) : run_win_fwd<float, 128>(a, s);
 }
@@ -1154,19 +1223,20 @@ size_t window_bwd_workspace(int B, int Nq, int Nk, int H, int Hk, int D, int lef
   return delta + (a.far_chunks ? (size_t)(1 + a.far_chunks * (H / Hk)) * B * Hk * 2 * a.sinks * D * 4 : 0);
 }
 
-int launch_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv,
+int launch_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const void* stats, void* dq, void* dk, void* dv,
                       const int64_t* st, const int* lengths, int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale,
                       int dtype, void* ws, size_t ws_bytes, hipStream_t s) {
   if (check_win("attention_window_bwd", B, Nq, Nk, H, Hk, D, left, right, sinks, scale, dtype)) return 1;
-  PT_CHECK(q && k && v && o && dout && lse && dq && dk && dv && st && ws, "attention_window_bwd: null argument");
+  PT_CHECK(q && k && v && o && dout && stats && dq && dk && dv && st && ws, "attention_window_bwd: null argument");
   PT_CHECK(aligned16(q, st, 3, dtype) && aligned16(k, st + 3, 3, dtype) && aligned16(v, st + 6, 3, dtype) &&
-               !(((uintptr_t)o | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15),
+               !(((uintptr_t)o | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)stats | (uintptr_t)ws) & 15),
            "attention_window_bwd: addresses and strides must be multiples of 16 bytes");
   PT_CHECK(near_rows(st) && (int64_t)H * D <= (1 << 20), "attention_window_bwd: rows are more than 2^20 values apart");
   const size_t need = window_bwd_workspace(B, Nq, Nk, H, Hk, D, left, right, sinks);
   PT_CHECK(ws_bytes >= need, "attention_window_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
   WinArgs a = win_args(q, k, v, st, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale);
-  a.od = o; a.dod = dout; a.lse = const_cast<float*>(lse); a.dq = dq; a.dk = dk; a.dv = dv;
+  a.od = o; a.dod = dout; a.lse = (float*)const_cast<void*>(stats); a.dq = dq; a.dk = dk; a.dv = dv;
+  if (window_wide(Nk, left, right, sinks, dtype)) a.rest = (signed char*)const_cast<void*>(stats) + lse_bytes(B, Nq, H);
   a.delta = (float*)ws;
   a.part = a.far_chunks ? (float*)((char*)ws + ((size_t)B * H * Nq * 4 + 255) / 256 * 256) : nullptr;
   if (dtype) return D <= 64 ? run_win_bwd<__bf16, 64>(a, s) : run_win_bwd<__bf16, 128>(a, s);

@@ -211,10 +211,9 @@ class GatedNorm(torch.autograd.Function):
         rows, cols = x.shape
         need = ctx.needs_input_grad
         dy, dh = (None if d is None else d.contiguous() for d in (dy, dh))
-        new = lambda like: torch.empty(like.shape, device=x.device, dtype=like.dtype)  # noqa: E731
-        dx = new(x)
-        dt = new(t) if need[1] else None
-        dgate = new(gate) if need[2] else None
+        dx = torch.empty(rows, cols, device=x.device, dtype=x.dtype)
+        dt = torch.empty(rows, cols, device=x.device, dtype=x.dtype) if need[1] else None
+        dgate = torch.empty_like(gate) if need[2] else None
         vec = [torch.empty(cols, device=x.device, dtype=torch.float32) if n else None for n in need[3:8]]
         L = _lib.lib()
         with _on(x.device):
@@ -368,10 +367,12 @@ def _vectors(t):
 def _window_attention(q, k, v, lengths, meta, grad):
     B, Nq, _, H, _, D = meta[:6]
     o = torch.empty(B, Nq, H, D, device=q.device, dtype=q.dtype)
-    lse = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32) if grad else None
+    L, stats = _lib.lib(), None
+    if grad:
+        stats = torch.empty(L.pt_attention_window_stats_bytes(*meta[:4], *meta[5:9], meta[10]), device=q.device, dtype=torch.uint8)
     with _on(q.device):
-        check(_lib.lib().pt_attention_window_fwd(_at(q), _at(k), _at(v), _at(o), _at(lse), _address(_strides(q, k, v)), _at(lengths), *meta, stream()))
-    return o, lse
+        check(L.pt_attention_window_fwd(_at(q), _at(k), _at(v), _at(o), _at(stats), _address(_strides(q, k, v)), _at(lengths), *meta, stream()))
+    return o, stats
 
 
 class WindowAttention(torch.autograd.Function):
@@ -379,20 +380,20 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lengths, meta):
-        o, lse = _window_attention(q, k, v, lengths, meta, True)
+        o, stats = _window_attention(q, k, v, lengths, meta, True)
         ctx.meta = meta
-        ctx.save_for_backward(q, k, v, lengths, o, lse)
+        ctx.save_for_backward(q, k, v, lengths, o, stats)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, lengths, o, lse = ctx.saved_tensors
+        q, k, v, lengths, o, stats = ctx.saved_tensors
         L = _lib.lib()
         do = _vectors(do.contiguous())
         dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
         with _on(q.device):
             ws = torch.empty(L.pt_attention_window_bwd_workspace_bytes(*ctx.meta[:9]), dtype=torch.uint8, device=q.device)
-            check(L.pt_attention_window_bwd(_at(q), _at(k), _at(v), _at(o), _at(do), _at(lse), _at(dq), _at(dk), _at(dv), _address(_strides(q, k, v)),
+            check(L.pt_attention_window_bwd(_at(q), _at(k), _at(v), _at(o), _at(do), _at(stats), _at(dq), _at(dk), _at(dv), _address(_strides(q, k, v)),
                                             _at(lengths), *ctx.meta, _at(ws), ws.numel(), stream()))
         return dq, dk, dv, None, None
 

@@ -116,6 +116,29 @@ def test_forward_and_gradients(name, dtype):
     assert all(torch.equal(got[n], again[n]) for n in got)
 
 
+@pytest.mark.parametrize("left", [2, 8, 100])
+def test_gradients_of_few_keys_do_not_feel_the_rounding_of_the_output(left):
+    """bf16.  Two roundings reach dQ and dK: of the factors in front of keys and queries, and of the result; delta is taken from an
+    output that is rounded to 24 bits.  Each rounding is uniform within half a step, so its mean square is at most
+    (2^-8)^2 / 3 of the value's; the roundings are independent, and a mean over 50,000 values is within a tenth of its expectation
+    (delta from the rounded output: 1.6 times the bound for left = 2)."""
+    case = (2, 400, 400, 2, 1, 64, left, 0, 0, None)
+    q, k, v, do, _ = make(case, torch.bfloat16)
+    got = grads(q, k, v, do, case, None)
+    big = lambda t: t.detach().double().transpose(1, 2).repeat_interleave(2 // t.shape[2], 1)  # noqa: E731
+    Q, K, V, G = big(q), big(k), big(v), big(do)
+    i = torch.arange(400, device="cuda")
+    far = (i[None] > i[:, None]) | (i[None] < i[:, None] - left)
+    p = (Q @ K.transpose(2, 3) / 8).masked_fill(far, -math.inf).softmax(-1)
+    ds = p * (G @ V.transpose(2, 3) - (G * (p @ V)).sum(-1, keepdim=True)) / 8
+    e = (2.0 ** -8) ** 2 / 3
+    join = lambda x: x.view(2, 1, 2, 400, 64).sum(2)  # noqa: E731
+    for n, want, square in (("q", ds @ K, ds.square() @ K.square()),
+                            ("k", join(ds.transpose(2, 3) @ Q), join(ds.square().transpose(2, 3) @ Q.square()))):
+        err = (got[n].double().transpose(1, 2) - want).square().sum()
+        assert float(err) <= 1.1 * e * float(square.sum() + want.square().sum()), (n, float(err / (e * (square.sum() + want.square().sum()))))
+
+
 def test_gradients_against_differences():
     case = CASES["a new part of a sequence"]
     q, k, v, do, _ = make(case, torch.float32)
