@@ -105,7 +105,7 @@ def _proto(lib):
     lib.pt_set_option.argtypes = [C.c_char_p, i]
     lib.pt_get_option.argtypes = [C.c_char_p, vp]
     lib.pt_attention_window_stats_bytes.restype = sz
-    lib.pt_attention_window_stats_bytes.argtypes = [i] * 9
+    lib.pt_attention_window_stats_bytes.argtypes = [i] * 5
     lib.pt_attention_window_bwd_workspace_bytes.restype = lib.pt_attention_window_step_workspace_bytes.restype = sz
     lib.pt_attention_window_bwd_workspace_bytes.argtypes = [i] * 9
     lib.pt_attention_window_step_workspace_bytes.argtypes = [i] * 7

@@ -40,7 +40,7 @@ int launch_moment_values(const unsigned char* m, const unsigned char* v, const f
 size_t gated_norm_workspace(int rows, int cols, int clip);
 int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1, const float* b1, const float* w2, const float* b2, void* y, void* h, float* stats, int64_t rows, int cols, int clip, int kind, float eps, int dtype, hipStream_t s);
 int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1, const float* b1, const float* w2, const float* stats, const void* dy, const void* dh, void* dx, void* dt, void* dgate, float* da, float* dw1, float* db1, float* dw2, float* db2, void* ws, size_t ws_bytes, int64_t rows, int cols, int clip, int kind, int dtype, hipStream_t s);
-size_t window_stats_bytes(int B, int Nq, int Nk, int H, int D, int left, int right, int sinks, int dtype);
+size_t window_stats_bytes(int B, int Nq, int H, int D, int dtype);
 int launch_window_fwd(const void* q, const void* k, const void* v, void* o, void* stats, const int64_t* st, const int* lengths, int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, hipStream_t s);
 size_t window_bwd_workspace(int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks);
 int launch_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const void* stats, void* dq, void* dk, void* dv, const int64_t* st, const int* lengths, int B, int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, void* ws, size_t ws_bytes, hipStream_t s);
@@ -456,8 +456,8 @@ int pt_attention_bf16(const void* Q, int ldq, const void* K, int ldk, const void
   return launch_attention_bf16((const unsigned short*)Q, ldq, (const unsigned short*)K, ldk, (const unsigned short*)V, ldv,
                                (unsigned short*)O, ldo, B, Nq, Nk, H, (hipStream_t)stream);
 }
-size_t pt_attention_window_stats_bytes(int B, int Nq, int Nk, int H, int D, int left, int right, int sinks, int dtype) {
-  return window_stats_bytes(B, Nq, Nk, H, D, left, right, sinks, dtype);
+size_t pt_attention_window_stats_bytes(int B, int Nq, int H, int D, int dtype) {
+  return window_stats_bytes(B, Nq, H, D, dtype);
 }
 int pt_attention_window_fwd(const void* q, const void* k, const void* v, void* o, void* stats, const int64_t* strides, const int32_t* lengths, int B,
                             int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, void* stream) {

@@ -69,7 +69,7 @@ struct WinArgs {
   void* o; float* lse;                                   // lse [B][H][Nq], in powers of two; +inf for a row that sees nothing
   const void* od; const void* dod;                       // backward: o and its gradient, (B, Nq, H, D)
   void* dq; void* dk; void* dv; float* delta;            // delta [B][H][Nq]
-  signed char* rest;                                     // what o lost when it was rounded, a byte a value (see rest_of), or null
+  signed char* rest;                                     // bf16: what o lost when it was rounded, a byte a value, where few_keys says so; or null
   float* part;                                           // shares of the first keys' gradients (see win_bwd_sink_kernel)
   int64_t sq[3], sk[3], sv[3];                           // strides of batch, row, head in values
   const int* lengths;
@@ -194,9 +194,9 @@ struct Cols<float, DP> {
         }
   }
 };
-// acc[db] += (columns of 32 rows)^T . p, p the registers of a score tile over these rows.  WIDE: p as the sum of two bf16 values
-template <typename T, int DP, bool WIDE = false>
-__device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const typename Types<T>::frag (&f)[2][DP / 32], const f32x16& p) {
+// acc[db] += (columns of 32 rows)^T . p, p the registers of a score tile over these rows.  wide (bf16): p as the sum of two bf16 values
+template <typename T, int DP>
+__device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const typename Types<T>::frag (&f)[2][DP / 32], const f32x16& p, bool wide = false) {
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
     typename Types<T>::frag x;
@@ -204,13 +204,16 @@ __device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const typena
     for (int e = 0; e < 8; ++e) x[e] = (T)p[8 * s2 + e];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], x, acc[db]);
-    if constexpr (WIDE) {
+  }
+  if (sizeof(T) == 2 && wide)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (T)(p[8 * s2 + e] - (float)x[e]);
+    for (int s2 = 0; s2 < 2; ++s2) {
+      typename Types<T>::frag x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (T)(p[8 * s2 + e] - (float)(T)p[8 * s2 + e]);
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], x, acc[db]);
     }
-  }
 }
 // What a value lost when it was rounded to bf16, in steps of its 24-bit pattern (-128 to 128, of which 128 is taken for 127), and the value
 // that both stand for, off by a step and a half of 2^-15 at most
@@ -340,6 +343,15 @@ __device__ __forceinline__ void key_tiles(const WinArgs& a, int len, int t0, int
   from = max(lo / KT, first);
   to = hi < lo ? from : max(hi / KT + 1, from);
 }
+// Whether rows at positions [t0, t1] see so few keys (512 each, 640 together) that in bf16 the rounding of their probabilities does not
+// average out: dQ and dK feel it, and that of o, through delta.  There the probabilities enter o's product as sums of two bf16 values, and
+// o keeps a byte more for delta: error of dQ and dK for 3 / 129 visible keys 2.2 / 1.53 -> 1.42 times that of rounding the exact
+// result (what is left is dS in bf16).  8192 rows, 16 heads over 4, D = 128: a window of 256 keys forward 43 -> 53 us, with gradients 183 -> 205;
+// 1024 keys, where only the first rows see few, 86 -> 87 and 375 -> 377
+__device__ __forceinline__ bool few_keys(const WinArgs& a, int len, int t0, int t1) {
+  const int hi = min(t1 + a.right, len - 1), lo = max(t0 - a.left, 0);
+  return hi - lo + 1 + min(a.sinks, lo) <= 640;
+}
 // Scores of invisible pairs to -infinity: keys along the registers of a transposed tile (KEYS) or along the lanes
 template <bool KEYS>
 __device__ __forceinline__ void mask_tile(const WinArgs& a, int len, int t, int key, int h, f32x16& st, int last = 0x7FFFFFFF) {
@@ -374,7 +386,7 @@ template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 2 |
 // ---------------------------------------------------------------------------
 // Forward: 4 waves of 32 rows each over common key tiles
 // ---------------------------------------------------------------------------
-template <typename T, int DP, bool WIDE>
+template <typename T, int DP>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fwd_kernel(const WinArgs a) {
   constexpr int KT = key_tile<T, DP>(), NB = KT / 32;
   constexpr bool BF = sizeof(T) == 2;
@@ -392,6 +404,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
   int first, from, to;
   key_tiles<KT>(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift, first, from, to);
   const int tiles = first + (to - from);
+  const bool wide = BF && few_keys(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift);
   auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
   const Dma<T, DP, KT, 256> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
   if (tiles > 0) {
@@ -462,10 +475,10 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
           l += st[x][r];                                                 // this lane's half of the column; joined at the end
         }
       if constexpr (!BF) vc.template read<0>(vf[0]);
-      add_product<T, DP, WIDE>(o, vf[0], st[0]);                         // probabilities in [0, 1] to bf16: 2^-9 of each; WIDE: 2^-17
+      add_product<T, DP>(o, vf[0], st[0], wide);                         // probabilities in [0, 1] to bf16: 2^-9 of each; wide: 2^-17
       if constexpr (NB > 1) {
         if constexpr (!BF) vc.template read<32 * tile::RB>(vf[1]);
-        add_product<T, DP, WIDE>(o, vf[1], st[1]);
+        add_product<T, DP>(o, vf[1], st[1], wide);
       }
     }
     dma_wait();
@@ -473,7 +486,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
   if (row >= a.Nq) return;
   l += half_other(l);
   const int64_t out = (((int64_t)b * a.Nq + row) * a.H + head) * a.D;
-  store_transposed<T, DP>((T*)a.o + out, o, h, a.D, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), WIDE && a.rest ? a.rest + out : nullptr);
+  store_transposed<T, DP>((T*)a.o + out, o, h, a.D, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), wide && a.rest ? a.rest + out : nullptr);
   if (a.lse && h == 0) a.lse[((int64_t)b * a.H + head) * a.Nq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -500,6 +513,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
   int first, from, to;
   key_tiles<KT>(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift, first, from, to);
   const int tiles = first + (to - from);
+  const bool wide = BF && few_keys(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift);
   auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
   const Dma<T, DP, KT, 256> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
   if (tiles > 0) {
@@ -514,7 +528,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
     gf[s] = global_frag((const T*)a.dod + ob, so, row, a.Nq, 16 * s + 8 * h, a.D);
     const auto of = global_frag((const T*)a.od + ob, so, row, a.Nq, 16 * s + 8 * h, a.D);
     if constexpr (BF)
-      if (a.rest && row < a.Nq && 16 * s + 8 * h < a.D) {
+      if (wide && row < a.Nq && 16 * s + 8 * h < a.D) {
         const uint2 w = *reinterpret_cast<const uint2*>(a.rest + ob + row * so + 16 * s + 8 * h);
 #pragma unroll
         for (int e = 0; e < 8; ++e) delta += (float)gf[s][e] * with_rest(of[e], (signed char)((e < 4 ? w.x : w.y) >> 8 * (e & 3)));
@@ -1160,26 +1174,17 @@ static WinArgs win_args(const void* q, const void* k, const void* v, const int64
 
 static int64_t win_blocks(const WinArgs& a) { return (int64_t)((a.Nq + 127) / 128) * a.H * a.B; }
 
-template <typename T, int DP, bool WIDE = false>
+template <typename T, int DP>
 static int run_win_fwd(const WinArgs& a, hipStream_t s) {
   constexpr int lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB;
-  PT_ENSURE_LDS((win_fwd_kernel<T, DP, WIDE>), lds);
-  PT_LAUNCH((win_fwd_kernel<T, DP, WIDE>), dim3((unsigned)win_blocks(a)), dim3(256), lds, s, a);
+  PT_ENSURE_LDS((win_fwd_kernel<T, DP>), lds);
+  PT_LAUNCH((win_fwd_kernel<T, DP>), dim3((unsigned)win_blocks(a)), dim3(256), lds, s, a);
   return 0;
 }
-// bf16 rows that see at most 512 keys: the rounding of few probabilities does not average out, and dQ, dK feel it in o through delta.
-// There the probabilities enter o's product as sums of two bf16 values and o keeps a byte more for delta: error of dQ and dK for 3 / 129
-// visible keys 2.2 / 1.53 -> 1.42 times that of rounding the exact result (what is left is dS in bf16); beyond 512 keys it is
-// 1.47 at most without.  8192 rows, 16 heads over 4, D = 128, 256 keys: forward 43 -> 53 us, with gradients 183 -> 205; 1024 keys would be 375 -> 410
-constexpr int WIDE_MAX = 512;
-static bool window_wide(int Nk, int left, int right, int sinks, int dtype) {
-  const int64_t seen = left < 0 || right < 0 ? Nk : std::min<int64_t>(Nk, (int64_t)left + right + 1 + sinks);
-  return dtype && seen <= WIDE_MAX;
-}
 static size_t lse_bytes(int B, int Nq, int H) { return ((size_t)B * H * Nq * 4 + 255) / 256 * 256; }
-size_t window_stats_bytes(int B, int Nq, int Nk, int H, int D, int left, int right, int sinks, int dtype) {
-  if (check_win("attention_window_fwd", B, Nq, Nk, H, H, D, left, right, sinks, 1.f, dtype)) return 0;
-  return lse_bytes(B, Nq, H) + (window_wide(Nk, left, right, sinks, dtype) ? (size_t)B * Nq * H * D : 0);
+size_t window_stats_bytes(int B, int Nq, int H, int D, int dtype) {
+  if (check_win("attention_window_fwd", B, Nq, Nq, H, H, D, 0, 0, 0, 1.f, dtype)) return 0;
+  return lse_bytes(B, Nq, H) + (dtype ? (size_t)B * Nq * H * D : 0);
 }
 template <typename T, int DP>
 static int run_win_bwd(const WinArgs& a, hipStream_t s) {
@@ -1207,10 +1212,7 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* o, void
   PT_CHECK(!((uintptr_t)stats & 15), "attention_window_fwd: stats must be aligned to 16 bytes");
   WinArgs a = win_args(q, k, v, st, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale);
   a.o = o; a.lse = (float*)stats;
-  if (window_wide(Nk, left, right, sinks, dtype)) {
-    a.rest = stats ? (signed char*)stats + lse_bytes(B, Nq, H) : nullptr;
-    return D <= 64 ? run_win_fwd<__bf16, 64, true>(a, s) : run_win_fwd<__bf16, 128, true>(a, s);
-  }
+  a.rest = dtype && stats ? (signed char*)stats + lse_bytes(B, Nq, H) : nullptr;
   if (dtype) return D <= 64 ? run_win_fwd<__bf16, 64>(a, s) : run_win_fwd<__bf16, 128>(a, s);
   return D <= 64 ? run_win_fwd<float, 64>(a, s) : run_win_fwd<float, 128>(a, s);
 }
@@ -1236,7 +1238,7 @@ int launch_window_bwd(const void* q, const void* k, const void* v, const void* o
   PT_CHECK(ws_bytes >= need, "attention_window_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
   WinArgs a = win_args(q, k, v, st, lengths, B, Nq, Nk, H, Hk, D, left, right, sinks, scale);
   a.od = o; a.dod = dout; a.lse = (float*)const_cast<void*>(stats); a.dq = dq; a.dk = dk; a.dv = dv;
-  if (window_wide(Nk, left, right, sinks, dtype)) a.rest = (signed char*)const_cast<void*>(stats) + lse_bytes(B, Nq, H);
+  if (dtype) a.rest = (signed char*)const_cast<void*>(stats) + lse_bytes(B, Nq, H);
   a.delta = (float*)ws;
   a.part = a.far_chunks ? (float*)((char*)ws + ((size_t)B * H * Nq * 4 + 255) / 256 * 256) : nullptr;
   if (dtype) return D <= 64 ? run_win_bwd<__bf16, 64>(a, s) : run_win_bwd<__bf16, 128>(a, s);

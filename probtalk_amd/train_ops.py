@@ -369,7 +369,7 @@ def _window_attention(q, k, v, lengths, meta, grad):
     o = torch.empty(B, Nq, H, D, device=q.device, dtype=q.dtype)
     L, stats = _lib.lib(), None
     if grad:
-        stats = torch.empty(L.pt_attention_window_stats_bytes(*meta[:4], *meta[5:9], meta[10]), device=q.device, dtype=torch.uint8)
+        stats = torch.empty(L.pt_attention_window_stats_bytes(B, Nq, H, D, meta[10]), device=q.device, dtype=torch.uint8)
     with _on(q.device):
         check(L.pt_attention_window_fwd(_at(q), _at(k), _at(v), _at(o), _at(stats), _address(_strides(q, k, v)), _at(lengths), *meta, stream()))
     return o, stats
