@@ -16,6 +16,7 @@ import torch
 from . import _lib
 from ._lib import check, ptr, stream
 
+_HERE = contextlib.nullcontext()
 _KT = {0: 1, 1: 3, 2: 7, 3: 4, 4: 4}
 
 
@@ -171,6 +172,10 @@ def layer_norm(x, gamma, beta, res=None):
     return LayerNormRes.apply(x, res, gamma, beta)
 
 
+def _row_major(v):
+    return v if v.stride(1) == 1 and v.stride(0) >= v.shape[1] else v.contiguous()
+
+
 def _row_stride(v):
     return 0 if v is None else v.stride(0) if v.shape[0] > 1 else v.shape[1]
 
@@ -181,13 +186,14 @@ def _at(t):
 
 def _gated_norm(x, t, gate, res_scale, post_w, post_b, pre_w, pre_b, clip, kind, eps, grad):
     rows, cols = x.shape
-    y = None if t is None else torch.empty(rows, cols, device=x.device, dtype=x.dtype)
-    h = None if pre_w is None else torch.empty(rows, cols, device=x.device, dtype=x.dtype)
-    stats = torch.empty(rows, 4, device=x.device, dtype=torch.float32) if grad else None
-    with _on(x.device):
-        check(_lib.lib().pt_train_gated_norm_fwd(_at(x), _row_stride(x), _at(t), _row_stride(t), _at(gate), _at(res_scale), _at(post_w),
-                                                 _at(post_b), _at(pre_w), _at(pre_b), _at(y), _at(h), _at(stats), rows, cols, clip, kind, eps,
-                                                 int(x.dtype is torch.bfloat16), stream()))
+    device, dtype = x.device, x.dtype
+    y = None if t is None else torch.empty(rows, cols, device=device, dtype=dtype)
+    h = None if pre_w is None else torch.empty(rows, cols, device=device, dtype=dtype)
+    stats = torch.empty(rows, 4, device=device, dtype=torch.float32) if grad else None
+    at = [None if v is None else v.data_ptr() for v in (x, t, gate, res_scale, post_w, post_b, pre_w, pre_b, y, h, stats)]
+    with _on(device):
+        check(_lib.lib().pt_train_gated_norm_fwd(at[0], _row_stride(x), at[1], _row_stride(t), *at[2:], rows, cols, clip, kind, eps,
+                                                 int(dtype is torch.bfloat16), stream()))
     return y, h, stats
 
 
@@ -211,16 +217,17 @@ class GatedNorm(torch.autograd.Function):
         rows, cols = x.shape
         need = ctx.needs_input_grad
         dy, dh = (None if d is None else d.contiguous() for d in (dy, dh))
-        dx = torch.empty(rows, cols, device=x.device, dtype=x.dtype)
-        dt = torch.empty(rows, cols, device=x.device, dtype=x.dtype) if need[1] else None
+        device, dtype = x.device, x.dtype
+        dx = torch.empty(rows, cols, device=device, dtype=dtype)
+        dt = torch.empty(rows, cols, device=device, dtype=dtype) if need[1] else None
         dgate = torch.empty_like(gate) if need[2] else None
-        vec = [torch.empty(cols, device=x.device, dtype=torch.float32) if n else None for n in need[3:8]]
+        vec = [torch.empty(cols, device=device, dtype=torch.float32) if n else None for n in need[3:8]]
         L = _lib.lib()
-        with _on(x.device):
-            ws = torch.empty(L.pt_train_gated_norm_workspace_bytes(rows, cols, clip if gate is not None else 0), dtype=torch.uint8, device=x.device)
-            check(L.pt_train_gated_norm_bwd(_at(x), _row_stride(x), _at(t), _row_stride(t), _at(gate), _at(res_scale), _at(post_w), _at(post_b),
-                                            _at(pre_w), _at(stats), _at(dy), _at(dh), _at(dx), _at(dt), _at(dgate), *map(_at, vec), _at(ws),
-                                            ws.numel(), rows, cols, clip, kind, bf, stream()))
+        with _on(device):
+            size = L.pt_train_gated_norm_workspace_bytes(rows, cols, clip if gate is not None else 0)
+            ws = torch.empty(size, dtype=torch.uint8, device=device)
+            at = [None if v is None else v.data_ptr() for v in (x, t, gate, res_scale, post_w, post_b, pre_w, stats, dy, dh, dx, dt, dgate, *vec, ws)]
+            check(L.pt_train_gated_norm_bwd(at[0], _row_stride(x), at[1], _row_stride(t), *at[2:], size, rows, cols, clip, kind, bf, stream()))
         return dx, dt, dgate, *vec, None, None, None
 
 
@@ -261,8 +268,11 @@ def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias
             raise RuntimeError(f"gated_norm: {rows} rows are not {gate.shape[0]} clips of {clip}")
         gate = gate.contiguous()
     own = x
-    x, t = (v if v is None or (v.stride(1) == 1 and v.stride(0) >= cols) else v.contiguous() for v in (x, t))
-    given = (x, t, gate, *(None if v is None else v.contiguous() for v in vectors))
+    if not x.is_contiguous():
+        x = _row_major(x)
+    if t is not None and not t.is_contiguous():
+        t = _row_major(t)
+    given = (x, t, gate, *[v if v is None or v.is_contiguous() else v.contiguous() for v in vectors])
     mode = 0 if kind == "layer" else 1
     if torch.is_grad_enabled() and any([v is not None and v.requires_grad for v in given]):
         y, h = GatedNorm.apply(*given, clip, mode, eps)
@@ -797,7 +807,7 @@ MOMENT_BLOCK = 256      # values of an 8-bit moment that share a scale
 
 def _on(device):
     """Launches go to the current stream of the tensors' device."""
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _same(what, tensors, dtypes, device=None):
@@ -824,14 +834,15 @@ def _address(a):
     return None if a is None else (C.c_char * (len(a) * a.itemsize)).from_buffer(a)
 
 
-def _grad_norm(pointers, sizes, is_bf16, max_norm, device):
-    """A device tensor [norm, coef]."""
+def _grad_norm(pointers, sizes, is_bf16, n, max_norm, device, ws_bytes=None):
+    """A device tensor [norm, coef]; pointers and sizes from _address."""
     L = _lib.lib()
-    n = len(pointers)
+    if ws_bytes is None:
+        ws_bytes = L.pt_train_grad_norm_workspace_bytes(sizes, n)
     out = torch.empty(2, device=device, dtype=torch.float32)
-    ws = torch.empty(L.pt_train_grad_norm_workspace_bytes(_address(sizes), n), dtype=torch.uint8, device=device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
     at = out.data_ptr()
-    check(L.pt_train_grad_norm(_address(pointers), _address(sizes), is_bf16, n, max_norm, at, at + 4, _at(ws), ws.numel(), stream()))
+    check(L.pt_train_grad_norm(pointers, sizes, is_bf16, n, max_norm, at, at + 4, ws.data_ptr(), ws_bytes, stream()))
     return out
 
 
@@ -844,7 +855,7 @@ def grad_norm(grads, max_norm):
     if any(g.dtype is torch.bfloat16 for g in grads):
         kinds = bytes(g.dtype is torch.bfloat16 for g in grads)
     with _on(device):
-        out = _grad_norm(_addresses(grads), array.array("q", [g.numel() for g in grads]), kinds, float(max_norm), device)
+        out = _grad_norm(_address(_addresses(grads)), _address(array.array("q", [g.numel() for g in grads])), kinds, len(grads), float(max_norm), device)
     return out[:1], out[1:]
 
 
@@ -892,6 +903,7 @@ class AdamWList:
         self._bf16 = int(self.dtype is torch.bfloat16)
         self._kinds = b"\1" * len(params) if self._bf16 else None
         self._pointers = [*map(_address, self._arrays), _address(self._n)]
+        self._norm_ws = _lib.lib().pt_train_grad_norm_workspace_bytes(self._pointers[-1], len(params))
 
     def step(self, grads, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, coef=None, max_norm=None, seed=0):
         """One step with `grads` (of the parameters' type and sizes).  coef: device scalar that scales the gradients; max_norm
@@ -924,13 +936,13 @@ class AdamWList:
         with _on(self.device):
             if not on_device and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamWList.step: a captured step would repeat one step count: pass `step` as a CUDA int32 tensor")
-            g = _addresses(grads)
+            g = _address(_addresses(grads))
             if max_norm is not None:
-                out = _grad_norm(g, self._n, self._kinds, float(max_norm), self.device)
+                out = _grad_norm(g, self._pointers[-1], self._kinds, len(grads), float(max_norm), self.device, self._norm_ws)
                 norm, scale = out[:1], out.data_ptr() + 4
             if on_device:
                 dyn = torch.empty(3, device=self.device, dtype=torch.float32)
-            check(_lib.lib().pt_train_adamw_multi(self._pointers[0], _address(g), *self._pointers[1:], len(g), self._bf16, scale, lr, *betas, eps,
+            check(_lib.lib().pt_train_adamw_multi(self._pointers[0], g, *self._pointers[1:], len(grads), self._bf16, scale, lr, *betas, eps,
                                                   weight_decay, 0 if on_device else step, _at(step) if on_device else None, _at(dyn),
                                                   seed & 0xFFFFFFFF, stream()))
         return norm
