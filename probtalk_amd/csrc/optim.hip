@@ -186,11 +186,15 @@ __device__ __forceinline__ void moments8(float g, float gs, float b1, float c1, 
   v = b2 * v + (c2 * gr) * gr;
 }
 
-// the moments of the 32-bit form: the contraction is written out, so that these are the bits of adamw_kernel (train.hip)
-__device__ __forceinline__ void moments32(float g, float gs, float b1, float c1, float b2, float c2, float& m, float& v) {
+// the 32-bit form: every operation rounded by itself, the bits of adamw_kernel (train.hip)
+__device__ __forceinline__ float adamw32(float p, float g, float gs, float b1, float c1, float b2, float c2, float decay, float step_size, float bc2_sqrt,
+                                         float eps, float& m, float& v) {
+#pragma clang fp contract(off)
   const float gr = g * gs;
-  m = fmaf(c1, gr, b1 * m);
-  v = fmaf(gr, c2 * gr, b2 * v);
+  m = b1 * m + c1 * gr;
+  v = b2 * v + c2 * gr * gr;
+  const float denom = sqrtf(v) / bc2_sqrt + eps;
+  return p * decay - step_size * (m / denom);
 }
 
 // One wave's 1024 values of tensor i from e0 on.  T: float or bf16 bits (unsigned short); S8: 8-bit moments; FULL: all of them are there and
@@ -281,9 +285,7 @@ __device__ __forceinline__ void adamw_wave(const AdamTab& tab, const AdamHyper& 
         const float denom = fmaf(__builtin_amdgcn_sqrtf(v[k][j]), bc2_inv, h.eps);
         pv = fmaf(decay, p[k][j], -(step_size * (m[k][j] * __builtin_amdgcn_rcpf(denom))));
       } else {
-        moments32(g[k][j], gs, h.b1, c1, h.b2, c2, m[k][j], v[k][j]);
-        const float denom = sqrtf(v[k][j]) / bc2_sqrt + h.eps;
-        pv = fmaf(decay, p[k][j], -(step_size * (m[k][j] / denom)));
+        pv = adamw32(p[k][j], g[k][j], gs, h.b1, c1, h.b2, c2, decay, step_size, bc2_sqrt, h.eps, m[k][j], v[k][j]);
       }
       p[k][j] = pv;
       unsigned r = 0;

@@ -424,7 +424,11 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const float* __restrict__ x
   const float mean = wsum(s) * (1.f / DM);
   float q = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q += (v[i] - mean) * (v[i] - mean);
+  for (int i = 0; i < 8; ++i) {
+#pragma clang fp contract(off)
+    const float d = v[i] - mean;                         // every operation rounded by itself, whatever the compiler would fuse
+    q += d * d;
+  }
   const float rstd = 1.0f / sqrtf(wsum(q) * (1.f / DM) + 1e-5f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -1522,9 +1526,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(float* __restrict__ p, const
                                                     float* __restrict__ v, size_t n, const float* __restrict__ gscale, float lr,
                                                     float beta1, float beta2, float eps, float wd, float bc1, float bc2_sqrt) {
   const float gs = gscale ? *gscale : 1.f;
+  const float decay = fmaf(-lr, wd, 1.f);
   for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (size_t)gridDim.x * 256) {
-    const float gr = g[e] * gs;
-    float pv = p[e] * (1.f - lr * wd);
+#pragma clang fp contract(off)
+    const float gr = g[e] * gs;                          // every operation rounded by itself, whatever the compiler would fuse
+    float pv = p[e] * decay;
     const float mv = beta1 * m[e] + (1.f - beta1) * gr;
     const float vv = beta2 * v[e] + (1.f - beta2) * gr * gr;
     m[e] = mv; v[e] = vv;
