@@ -238,7 +238,7 @@ struct Dma {
   unsigned off[2];
   int64_t stride;                                        // bytes of a row
   __device__ __forceinline__ Dma(int D, int64_t stride_) : stride(stride_ * (int64_t)sizeof(T)) {
-    const int byte = threadIdx.x * 16;
+    const int byte = threadIdx.x % TH * 16;
     row = byte / RB;
     const int chunk = (byte % RB / 16) ^ tile::swz(row), odd = chunk ^ tile::swz(ROWS);
     col[0] = chunk * tile::EPC < D ? chunk * 16 : 0;
@@ -248,7 +248,7 @@ struct Dma {
   }
   // rows row0 .. row0 + R - 1 of base, row0 < limit
   __device__ __forceinline__ void operator()(const T* __restrict__ base, int row0, int limit, unsigned char* m) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), last = limit - 1 - row0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x % TH >> 6), last = limit - 1 - row0;
     const char* from = reinterpret_cast<const char*>(base) + row0 * stride;
     if (R - 1 <= last) {                                 // a whole tile: uniform address, a lane's offset that stays the same
 #pragma unroll
@@ -363,16 +363,19 @@ __device__ __forceinline__ void mask_tile(const WinArgs& a, int len, int t, int 
   }
 }
 // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: XCD x gets a run of neighbours in the order of the work, so that
-// workgroups that read the same keys (or rows) share an L2
-__device__ __forceinline__ int work_item(int id, int total) {
-  const int q = total / 8, r = total % 8, x = id % 8;
-  return x * q + min(x, r) + id / 8;
+// workgroups that read the same keys (or rows) share an L2.  Key heads of a sequence (units of `per` neighbours) go to the XCDs in turn where
+// they share out evenly: sequences of a padded batch differ in length
+__device__ __forceinline__ int work_item(int id, int total, int per) {
+  const int x = id % 8, n = id / 8;
+  if (total / per % 8 == 0) return (n / per * 8 + x) * per + n % per;
+  const int q = total / 8, r = total % 8;
+  return x * q + min(x, r) + n;
 }
 struct Place { int tile, head, kvh, b; };
 // order of the work: query heads of a group, tiles, key heads, sequences
 __device__ __forceinline__ Place place(const WinArgs& a, int tiles) {
   const int group = a.H / a.Hk;
-  int n = work_item(blockIdx.x, gridDim.x);
+  int n = work_item(blockIdx.x, gridDim.x, group * tiles);
   Place p;
   const int g = n % group; n /= group;
   p.tile = n % tiles; n /= tiles;
@@ -381,35 +384,69 @@ __device__ __forceinline__ Place place(const WinArgs& a, int tiles) {
   p.head = p.kvh * group + g;
   return p;
 }
-template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 2 || DP == 64 ? 64 : 32; }
+// A transposed result on its way from one wave to another through LDS: `to` is the column's row of DP + 4 words there
+template <int DP>
+__device__ __forceinline__ void hand_over(const f32x16 (&x)[DP / 32], float* to, int h) {
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(to + db * 32 + 8 * g + 4 * h) = f32x4{x[db][4 * g], x[db][4 * g + 1], x[db][4 * g + 2], x[db][4 * g + 3]};
+}
+template <int DP>
+__device__ __forceinline__ void take_over(f32x16 (&x)[DP / 32], const float* from, int h, float mine, float other) {
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(from + db * 32 + 8 * g + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[db][4 * g + e] = x[db][4 * g + e] * mine + y[e] * other;
+    }
+}
+template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+// The row kernels (forward, dQ): RW waves of 32 rows each, and SETS of them that take every SETS-th key tile and are joined at the end.
+// fp32 with D up to 64 has finer workgroups: 64 rows, two sets, two of them on a CU.  Its products take 16 times bf16's time, so a workgroup of 128 rows
+// is long and the chip ends unevenly: 4 padded sequences of 1200 rows, 8 heads, 257 keys 63 -> 36 us forward, 87 -> 49 dQ; two causal
+// ones of 4096 537 -> 408 forward.  (One set of 64 rows, five workgroups on a CU: 52 and 71 us.)
+template <typename T, int DP>
+struct RowPlan {                                         // WAVES: per SIMD
+  static constexpr bool FINE = sizeof(T) == 4 && DP == 64;
+  static constexpr int RW = FINE ? 2 : 4, SETS = FINE ? 2 : 1, TS = RW * 64, TH = SETS * TS, ROWS = RW * 32, WAVES = DP * (int)sizeof(T) > 256 ? 1 : 2;
+};
 
 // ---------------------------------------------------------------------------
-// Forward: 4 waves of 32 rows each over common key tiles
+// Forward: waves of 32 rows each over common key tiles (RowPlan).  bf16, 8192 rows that see 1028 keys, 16 heads over 4, D = 128: 105 us,
+// 615 TFLOP/s of visible pairs; its products alone take 66 us, the rate of a large matrix product on this card, the rest is softmax, the window's
+// edges and loads that they do not cover.  fp32: see RowPlan
 // ---------------------------------------------------------------------------
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fwd_kernel(const WinArgs a) {
+__global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void win_fwd_kernel(const WinArgs a) {
+  typedef RowPlan<T, DP> plan;
+  constexpr int SETS = plan::SETS, ROWS = plan::ROWS;
   constexpr int KT = key_tile<T, DP>(), NB = KT / 32;
   constexpr bool BF = sizeof(T) == 2;
   typedef Tile<T, DP> tile;
   constexpr int TB = KT * tile::RB;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];      // [2][K tile | V tile]
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-  const Place at = place(a, (a.Nq + 127) / 128);
-  const int head = at.head, b = at.b, i00 = at.tile * 128;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char win_lds[];      // [2][K tile | V tile]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % plan::RW, set = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / plan::RW, h = lane >> 5, col = lane & 31;
+  const Place at = place(a, (a.Nq + ROWS - 1) / ROWS);
+  unsigned char* win_smem = win_lds + set * 4 * TB;
+  const int head = at.head, b = at.b, i00 = at.tile * ROWS;
   const int len = length_of(a, b), shift = a.Nk - a.Nq;
   const int i0 = i00 + wave * 32, row = i0 + col, t = row + shift;
   const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + at.kvh * a.sk[2];
   const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + at.kvh * a.sv[2];
   const T* __restrict__ Q = (const T*)a.q + b * a.sq[0] + head * a.sq[2];
   int first, from, to;
-  key_tiles<KT>(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift, first, from, to);
+  key_tiles<KT>(a, len, i00 + shift, min(i00 + ROWS - 1, a.Nq - 1) + shift, first, from, to);
   const int tiles = first + (to - from);
-  const bool wide = BF && few_keys(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift);
+  const bool wide = BF && few_keys(a, len, i00 + shift, min(i00 + ROWS - 1, a.Nq - 1) + shift);
   auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
-  const Dma<T, DP, KT, 256> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
-  if (tiles > 0) {
-    dma_k(K, key_of(0), len, win_smem);
-    dma_v(V, key_of(0), len, win_smem + TB);
+  const Dma<T, DP, KT, plan::TS> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
+  if (set < tiles) {
+    dma_k(K, key_of(set), len, win_smem);
+    dma_v(V, key_of(set), len, win_smem + TB);
   }
   typename Types<T>::frag qf[DP / 16];
 #pragma unroll
@@ -421,16 +458,17 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
   const int w0 = i0 + shift, w1 = min(i0 + 31, a.Nq - 1) + shift;        // positions of this wave
   const int rb = tile::row_base(col, h), cb = tile::col_base(lane);
   dma_wait();
-  for (int n = 0; n < tiles; ++n) {
-    const unsigned char* Ks = win_smem + (n & 1) * 2 * TB;
+  for (int turn = 0; turn * SETS < tiles; ++turn) {
+    const int n = turn * SETS + set;
+    const unsigned char* Ks = win_smem + (turn & 1) * 2 * TB;
     const unsigned char* Vs = Ks + TB;
     const int k0 = key_of(n), k1 = k0 + KT - 1;
-    if (n + 1 < tiles) {                                                 // into the other buffer: its readers passed the last barrier
-      unsigned char* next = win_smem + ((n + 1) & 1) * 2 * TB;
-      dma_k(K, key_of(n + 1), len, next);
-      dma_v(V, key_of(n + 1), len, next + TB);
+    if (n + SETS < tiles) {                                                 // into the other buffer: its readers passed the last barrier
+      unsigned char* next = win_smem + ((turn + 1) & 1) * 2 * TB;
+      dma_k(K, key_of(n + SETS), len, next);
+      dma_v(V, key_of(n + SETS), len, next + TB);
     }
-    if (i0 < a.Nq && k0 <= w1 + a.right && (k1 >= w0 - a.left || k0 < a.sinks)) {
+    if ((SETS == 1 || n < tiles) && i0 < a.Nq && k0 <= w1 + a.right && (k1 >= w0 - a.left || k0 < a.sinks)) {
       f32x16 st[NB];
 #pragma unroll
       for (int x = 0; x < NB; ++x) {
@@ -445,6 +483,9 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
       if constexpr (BF) {
         vc.template read<0>(vf[0]);
         vc.template read<32 * tile::RB>(vf[1]);
+      } else {
+        vc.template read<0>(vf[0]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (!(k1 <= w0 + a.right && k1 < len && (k0 >= w1 - a.left || k1 < a.sinks)))
 #pragma unroll
@@ -474,14 +515,35 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
           st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -base));
           l += st[x][r];                                                 // this lane's half of the column; joined at the end
         }
-      if constexpr (!BF) vc.template read<0>(vf[0]);
-      add_product<T, DP>(o, vf[0], st[0], wide);                         // probabilities in [0, 1] to bf16: 2^-9 of each; wide: 2^-17
-      if constexpr (NB > 1) {
-        if constexpr (!BF) vc.template read<32 * tile::RB>(vf[1]);
-        add_product<T, DP>(o, vf[1], st[1], wide);
+      if constexpr (!BF && NB > 1) {
+        vc.template read<32 * tile::RB>(vf[1]);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      add_product<T, DP>(o, vf[0], st[0], wide);                         // probabilities in [0, 1] to bf16: 2^-9 of each; wide: 2^-17
+      if constexpr (NB > 1) add_product<T, DP>(o, vf[1], st[1], wide);
     }
     dma_wait();
+  }
+  if constexpr (SETS > 1) {                              // the other sets' sums and maxima to the first (behind the last barrier the tiles are free)
+    constexpr int JW = DP + 4;
+    float* rows = reinterpret_cast<float*>(win_lds) + (wave * 32 + col) * JW;
+    if (set) {
+      float* mine = rows + (set - 1) * ROWS * JW;
+      hand_over<DP>(o, mine, h);
+      if (h == 0) mine[DP] = m;
+      mine[DP + 1 + h] = l;
+    }
+    __syncthreads();
+    if (set) return;
+#pragma unroll
+    for (int x = 0; x < SETS - 1; ++x) {
+      const float* other = rows + x * ROWS * JW;
+      const float m2 = other[DP], top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+      const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+      m = top;
+      l = l * f + other[DP + 1 + h] * f2;
+      take_over<DP>(o, other, h, f, f2);
+    }
   }
   if (row >= a.Nq) return;
   l += half_other(l);
@@ -491,19 +553,22 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_fw
 }
 
 // ---------------------------------------------------------------------------
-// Backward, dQ (and delta): rows and key tiles as forward
+// Backward, dQ (and delta): rows and key tiles as forward.  The case above: 145 us for three products (668 TFLOP/s of visible pairs)
 // ---------------------------------------------------------------------------
 template <typename T, int DP> constexpr int key_tile_q() { return sizeof(T) * DP <= 128 ? 64 : 32; }   // 256 registers hold no more
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bwd_q_kernel(const WinArgs a) {
+__global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void win_bwd_q_kernel(const WinArgs a) {
+  typedef RowPlan<T, DP> plan;
+  constexpr int SETS = plan::SETS, ROWS = plan::ROWS;
   constexpr int KT = key_tile_q<T, DP>(), NB = KT / 32;
   constexpr bool BF = sizeof(T) == 2;
   typedef Tile<T, DP> tile;
   constexpr int TB = KT * tile::RB;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-  const Place at = place(a, (a.Nq + 127) / 128);
-  const int head = at.head, b = at.b, i00 = at.tile * 128;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char win_lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % plan::RW, set = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / plan::RW, h = lane >> 5, col = lane & 31;
+  const Place at = place(a, (a.Nq + ROWS - 1) / ROWS);
+  unsigned char* win_smem = win_lds + set * 4 * TB;
+  const int head = at.head, b = at.b, i00 = at.tile * ROWS;
   const int len = length_of(a, b), shift = a.Nk - a.Nq;
   const int i0 = i00 + wave * 32, row = i0 + col, t = row + shift;
   const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + at.kvh * a.sk[2];
@@ -511,14 +576,14 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
   const T* __restrict__ Q = (const T*)a.q + b * a.sq[0] + head * a.sq[2];
   const int64_t so = (int64_t)a.H * a.D, ob = ((int64_t)b * a.Nq * a.H + head) * a.D;
   int first, from, to;
-  key_tiles<KT>(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift, first, from, to);
+  key_tiles<KT>(a, len, i00 + shift, min(i00 + ROWS - 1, a.Nq - 1) + shift, first, from, to);
   const int tiles = first + (to - from);
-  const bool wide = BF && few_keys(a, len, i00 + shift, min(i00 + 127, a.Nq - 1) + shift);
+  const bool wide = BF && few_keys(a, len, i00 + shift, min(i00 + ROWS - 1, a.Nq - 1) + shift);
   auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
-  const Dma<T, DP, KT, 256> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
-  if (tiles > 0) {
-    dma_k(K, key_of(0), len, win_smem);
-    dma_v(V, key_of(0), len, win_smem + TB);
+  const Dma<T, DP, KT, plan::TS> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
+  if (set < tiles) {
+    dma_k(K, key_of(set), len, win_smem);
+    dma_v(V, key_of(set), len, win_smem + TB);
   }
   typename Types<T>::frag qf[DP / 16], gf[DP / 16];
   float delta = 0.f;
@@ -540,7 +605,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
   delta += half_other(delta);
   const int64_t li = ((int64_t)b * a.H + head) * a.Nq + row;
   float lse = row < a.Nq ? a.lse[li] : INFINITY;
-  if (row < a.Nq && h == 0) a.delta[li] = delta;
+  if (row < a.Nq && h == 0 && set == 0) a.delta[li] = delta;
   asm volatile("" : "+v"(lse), "+v"(delta));             // here, not in the loop, where the wait for them would be one for the tiles too
   f32x16 dq[DP / 32];
 #pragma unroll
@@ -548,16 +613,17 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
   const int w0 = i0 + shift, w1 = min(i0 + 31, a.Nq - 1) + shift;
   const int rb = tile::row_base(col, h), cb = tile::col_base(lane);
   dma_wait();
-  for (int n = 0; n < tiles; ++n) {
-    const unsigned char* Ks = win_smem + (n & 1) * 2 * TB;
+  for (int turn = 0; turn * SETS < tiles; ++turn) {
+    const int n = turn * SETS + set;
+    const unsigned char* Ks = win_smem + (turn & 1) * 2 * TB;
     const unsigned char* Vs = Ks + TB;
     const int k0 = key_of(n), k1 = k0 + KT - 1;
-    if (n + 1 < tiles) {                                                 // into the other buffer: its readers passed the last barrier
-      unsigned char* next = win_smem + ((n + 1) & 1) * 2 * TB;
-      dma_k(K, key_of(n + 1), len, next);
-      dma_v(V, key_of(n + 1), len, next + TB);
+    if (n + SETS < tiles) {                                                 // into the other buffer: its readers passed the last barrier
+      unsigned char* next = win_smem + ((turn + 1) & 1) * 2 * TB;
+      dma_k(K, key_of(n + SETS), len, next);
+      dma_v(V, key_of(n + SETS), len, next + TB);
     }
-    if (i0 < a.Nq && k0 <= w1 + a.right && (k1 >= w0 - a.left || k0 < a.sinks)) {
+    if ((SETS == 1 || n < tiles) && i0 < a.Nq && k0 <= w1 + a.right && (k1 >= w0 - a.left || k0 < a.sinks)) {
       const bool all = k1 <= w0 + a.right && k1 < len && (k0 >= w1 - a.left || k1 < a.sinks);
       f32x16 st[NB], dp[NB];
 #pragma unroll
@@ -576,6 +642,9 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
       if constexpr (BF) {
         kc.template read<0>(kf[0]);
         if constexpr (NB > 1) kc.template read<32 * tile::RB>(kf[NB - 1]);
+      } else {
+        kc.template read<0>(kf[0]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (!all)
 #pragma unroll
@@ -585,7 +654,6 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -lse)) * (dp[x][r] - delta);
-      if constexpr (!BF) kc.template read<0>(kf[0]);
       add_product<T, DP>(dq, kf[0], st[0]);                              // dS to bf16: 2^-9 of each
       if constexpr (NB > 1) {
         if constexpr (!BF) kc.template read<32 * tile::RB>(kf[NB - 1]);
@@ -594,14 +662,24 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bw
     }
     dma_wait();
   }
+  if constexpr (SETS > 1) {
+    float* rows = reinterpret_cast<float*>(win_lds) + (wave * 32 + col) * (DP + 4);
+    if (set) hand_over<DP>(dq, rows + (set - 1) * ROWS * (DP + 4), h);
+    __syncthreads();
+    if (set) return;
+#pragma unroll
+    for (int x = 0; x < SETS - 1; ++x) take_over<DP>(dq, rows + x * ROWS * (DP + 4), h, 1.f, 1.f);
+  }
   if (row < a.Nq) store_transposed<T, DP>((T*)a.dq + (((int64_t)b * a.Nq + row) * a.H + head) * a.D, dq, h, a.D, a.scale);
 }
 
 // ---------------------------------------------------------------------------
 // Backward, dK and dV: 8 waves over tiles of 64 rows, all query heads of the group in turn: 4 blocks of 32 keys, for each one wave
 // on the tile's first 32 rows and one on the others, added up at the end (there are too few blocks of keys to fill the chip with
-// 4 waves each).  The keys stay in registers as operands; rows of more than 128 bytes leave no room for the values beside them (two
+// 4 waves each).  The keys stay in registers as operands; in bf16, rows of more than 128 bytes leave no room for the values beside them (two
 // waves a SIMD have 256 registers each, half of them hold the results), so these are read from LDS, where they stay too.
+// The case above: 170 us for four products (760 TFLOP/s of visible pairs).  fp32 with D up to 64: 2 blocks of keys, values in registers, two
+// workgroups on a CU (105 -> 57 us where the row kernels gain as RowPlan says).
 // SINK: the rows far behind the window, which see the first 32-key blocks as sinks only.  There are as many of these rows as the
 // sequence is long and only a few keys, so the waves take the SAME keys and 32 rows of a tile each, the rows are cut into
 // chunks, and every workgroup leaves its share in fp32; win_bwd_join_kernel adds the shares in order.
@@ -610,13 +688,15 @@ template <typename T, int DP, bool SINK>
 struct KvPlan {
   static constexpr int RB = Tile<T, DP>::RB;
   static constexpr int SETS = SINK || RB > 256 ? 1 : 2;                  // waves per block of keys; 512-byte rows need a SIMD's registers for one
-  static constexpr int TH = 256 * SETS, QT = SINK ? (RB > 256 ? 64 : 128) : 32 * SETS, TB = QT * RB, LB = (QT < 64 ? 64 : QT) * 4;
-  static constexpr bool V_LDS = RB > 128;
-  static constexpr int KEYS = SINK ? 32 : 128;
+  static constexpr bool FINE = !SINK && RB == 256 && sizeof(T) == 4;     // fp32, D up to 64: see RowPlan
+  static constexpr int BLOCKS = FINE ? 2 : 4;                            // of 32 keys (SINK: waves on one)
+  static constexpr int TH = 64 * BLOCKS * SETS, QT = SINK ? (RB > 256 ? 64 : 128) : 32 * SETS, TB = QT * RB, LB = (QT < 64 ? 64 : QT) * 4;
+  static constexpr bool V_LDS = RB > 128 && !FINE;
+  static constexpr int KEYS = SINK ? 32 : 32 * BLOCKS;
   static constexpr int VB = V_LDS ? KEYS * RB : 0;
   static constexpr int ONE = 2 * TB + 2 * LB;                            // Q tile | dO tile | lse | delta
   static constexpr int BUF = SINK ? 1 : 2;
-  static constexpr int JOIN = (SINK ? 2 : 4) * 32 * (DP + 4) * 4;        // fp32 results on their way from wave to wave
+  static constexpr int JOIN = (SINK ? 2 : BLOCKS) * 32 * (DP + 4) * 4;        // fp32 results on their way from wave to wave
   static constexpr int LDS = VB + BUF * ONE > JOIN ? VB + BUF * ONE : JOIN;
   static_assert(LDS <= 160 * 1024 && BUF * ONE <= 128 * 1024, "LDS, and what LDS-DMA reaches of it");
 };
@@ -624,7 +704,7 @@ template <typename T, int DP, bool SINK>
 __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bwd_kv_kernel(const WinArgs a) {
   typedef KvPlan<T, DP, SINK> plan;
   constexpr bool BF = sizeof(T) == 2;
-  constexpr int QT = plan::QT, TB = plan::TB, ONE = plan::ONE, LB = plan::LB, SETS = plan::SETS, TH = plan::TH;
+  constexpr int QT = plan::QT, TB = plan::TB, ONE = plan::ONE, LB = plan::LB, SETS = plan::SETS, TH = plan::TH, BLOCKS = plan::BLOCKS, KEYS = plan::KEYS;
   typedef Tile<T, DP> tile;
   extern __shared__ __attribute__((aligned(1024))) unsigned char win_smem[];      // [BUF][ONE] | values
   unsigned char* bufs = win_smem;
@@ -641,15 +721,15 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
     item %= a.H;                                                         // the query head
     kvh = item / group;
   } else {
-    const int tiles = (a.Nk + 127) / 128;
-    item = work_item(blockIdx.x, gridDim.x);
-    kb = item % tiles * 128; item /= tiles;
+    const int tiles = (a.Nk + KEYS - 1) / KEYS;
+    item = work_item(blockIdx.x, gridDim.x, tiles);
+    kb = item % tiles * KEYS; item /= tiles;
     kvh = item % a.Hk;
     b = item / a.Hk;
   }
   const int len = length_of(a, b);
-  const int k0 = SINK ? kb : kb + (wave & 3) * 32, key = k0 + col;
-  const int sub = SINK ? wave * 32 : (wave >> 2) * 32;                   // this wave's rows of a tile
+  const int k0 = SINK ? kb : kb + wave % BLOCKS * 32, key = k0 + col;
+  const int sub = SINK ? wave * 32 : wave / BLOCKS * 32;                   // this wave's rows of a tile
   const T* __restrict__ K = (const T*)a.k + b * a.sk[0] + kvh * a.sk[2];
   const T* __restrict__ V = (const T*)a.v + b * a.sv[0] + kvh * a.sv[2];
   // rows that this workgroup looks at
@@ -659,7 +739,8 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
     r1 = kb >= len ? 0 : min(r0 + a.far_rows, a.Nq);                     // no such key: nothing is read, the share is zeros
   } else {
     r0 = max(kb - a.right - shift, 0) / QT * QT;
-    r1 = kb >= len ? 0 : (int)min((int64_t)kb + 127 + a.left - shift + 1, (int64_t)a.Nq);
+    // the other kernel takes the sinks' rows from a.far on, which is behind the window of the first 128 keys
+    r1 = kb >= len ? 0 : (int)min((int64_t)(kb < a.sinks ? 127 : kb + KEYS - 1) + a.left - shift + 1, (int64_t)a.Nq);
   }
   const int per = r1 > r0 ? (r1 - r0 + QT - 1) / QT : 0, total = SINK ? per : per * group;
   const int64_t so = (int64_t)a.H * a.D;
@@ -699,7 +780,7 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) { dk[db] = zero16(); dv[db] = zero16(); }
   const int rb = tile::row_base(col, h), cb = tile::col_base(lane);
-  const unsigned char* Vw = Vs + (SINK ? 0 : (wave & 3) * 32 * tile::RB);
+  const unsigned char* Vw = Vs + (SINK ? 0 : wave % BLOCKS * 32 * tile::RB);
   if constexpr (!SINK) dma_wait();
   int cr = r0;                                                           // first row of the current tile
   for (int n = 0; n < total; ++n) {
@@ -725,7 +806,8 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
       constexpr int READS = plan::V_LDS ? 3 : 2;                         // for two products
       if constexpr (BF) reads_ahead<2 * READS, READS, 2, DP / 8>(); else reads_ahead<2 * READS, READS * 2, 16, DP>();
       typename Types<T>::frag f[2][DP / 32];
-      if constexpr (BF) Cols<T, DP>(Gs, cb).template read<0>(f);
+      Cols<T, DP>(Gs, cb).template read<0>(f);
+      if constexpr (!BF) __builtin_amdgcn_sched_barrier(0);
       if (!all) mask_tile<false>(a, len, t0, key, h, st, r1 - 1 + shift);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -737,10 +819,17 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
           dp[r] = st[r] * (dp[r] - D4[e]);
         }
       }
-      if constexpr (!BF) Cols<T, DP>(Gs, cb).template read<0>(f);
-      add_product<T, DP>(dv, f, st);
-      Cols<T, DP>(Qs, cb).template read<0>(f);
-      add_product<T, DP>(dk, f, dp);
+      if constexpr (!BF && plan::V_LDS) {
+        typename Types<T>::frag f2[2][DP / 32];
+        Cols<T, DP>(Qs, cb).template read<0>(f2);
+        __builtin_amdgcn_sched_barrier(0);
+        add_product<T, DP>(dv, f, st);
+        add_product<T, DP>(dk, f2, dp);
+      } else {
+        add_product<T, DP>(dv, f, st);
+        Cols<T, DP>(Qs, cb).template read<0>(f);
+        add_product<T, DP>(dk, f, dp);
+      }
     }
     if constexpr (SINK) __syncthreads();
     else dma_wait();
@@ -778,14 +867,14 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
     store_transposed<float, DP>(out + (int64_t)a.sinks * a.D, dv, h, a.D, 1.f);
   } else {
     if constexpr (SETS == 2) {
-      float* mine = join + (wave & 3) * 32 * JW;
-      if (wave >= 4) pass(dk, mine, true);
+      float* mine = join + wave % BLOCKS * 32 * JW;
+      if (wave >= BLOCKS) pass(dk, mine, true);
       __syncthreads();
-      if (wave < 4) pass(dk, mine, false);
+      if (wave < BLOCKS) pass(dk, mine, false);
       __syncthreads();
-      if (wave >= 4) pass(dv, mine, true);
+      if (wave >= BLOCKS) pass(dv, mine, true);
       __syncthreads();
-      if (wave >= 4) return;
+      if (wave >= BLOCKS) return;
       pass(dv, mine, false);
     }
     if (key >= a.Nk) return;
@@ -1172,13 +1261,14 @@ static WinArgs win_args(const void* q, const void* k, const void* v, const int64
   return a;
 }
 
-static int64_t win_blocks(const WinArgs& a) { return (int64_t)((a.Nq + 127) / 128) * a.H * a.B; }
+static int64_t win_blocks(const WinArgs& a, int rows) { return (int64_t)((a.Nq + rows - 1) / rows) * a.H * a.B; }
 
 template <typename T, int DP>
 static int run_win_fwd(const WinArgs& a, hipStream_t s) {
-  constexpr int lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB;
+  typedef RowPlan<T, DP> plan;
+  constexpr int lds = plan::SETS * 4 * key_tile<T, DP>() * Tile<T, DP>::RB;
   PT_ENSURE_LDS((win_fwd_kernel<T, DP>), lds);
-  PT_LAUNCH((win_fwd_kernel<T, DP>), dim3((unsigned)win_blocks(a)), dim3(256), lds, s, a);
+  PT_LAUNCH((win_fwd_kernel<T, DP>), dim3((unsigned)win_blocks(a, plan::ROWS)), dim3(plan::TH), lds, s, a);
   return 0;
 }
 static size_t lse_bytes(int B, int Nq, int H) { return ((size_t)B * H * Nq * 4 + 255) / 256 * 256; }
@@ -1188,11 +1278,12 @@ size_t window_stats_bytes(int B, int Nq, int H, int D, int dtype) {
 }
 template <typename T, int DP>
 static int run_win_bwd(const WinArgs& a, hipStream_t s) {
-  constexpr int lds = 4 * key_tile_q<T, DP>() * Tile<T, DP>::RB, lds_kv = KvPlan<T, DP, false>::LDS, lds_sink = KvPlan<T, DP, true>::LDS;
+  typedef RowPlan<T, DP> plan;
+  constexpr int lds = plan::SETS * 4 * key_tile_q<T, DP>() * Tile<T, DP>::RB, lds_kv = KvPlan<T, DP, false>::LDS, lds_sink = KvPlan<T, DP, true>::LDS;
   PT_ENSURE_LDS((win_bwd_q_kernel<T, DP>), lds);
   PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false>), lds_kv);
-  PT_LAUNCH((win_bwd_q_kernel<T, DP>), dim3((unsigned)win_blocks(a)), dim3(256), lds, s, a);
-  PT_LAUNCH((win_bwd_kv_kernel<T, DP, false>), dim3((unsigned)((a.Nk + 127) / 128) * a.Hk * a.B), dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
+  PT_LAUNCH((win_bwd_q_kernel<T, DP>), dim3((unsigned)win_blocks(a, plan::ROWS)), dim3(plan::TH), lds, s, a);
+  PT_LAUNCH((win_bwd_kv_kernel<T, DP, false>), dim3((unsigned)((a.Nk + KvPlan<T, DP, false>::KEYS - 1) / KvPlan<T, DP, false>::KEYS) * a.Hk * a.B), dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
   if (a.far_chunks) {
     PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, true>), lds_sink);
     PT_LAUNCH((win_bwd_kv_kernel<T, DP, true>), dim3((unsigned)((a.sinks + 31) / 32 * a.far_chunks) * a.H * a.B), dim3(KvPlan<T, DP, true>::TH), lds_sink, s, a);
