@@ -12,7 +12,7 @@
 // Bound by HBM: forward 2 rows in and 2 out, backward 4 in and 2 out.  y and the statistics' arguments are recomputed from x and t
 // (the same bytes as reading a stored y, and exact where y is held in bf16); only 4 floats a row are kept from the forward pass.
 //
-// A row is held by WPR waves, 8 values a lane; a worker (these waves) walks a run of rows, so the column vectors stay in registers
+// A row is held by WPR waves, PER values a lane; a worker (these waves) walks a run of rows, so the column vectors stay in registers
 // and the column sums of the backward pass are register adds.  A worker's rows lie in one clip, or are whole clips, so the gate's
 // gradient is a register sum too, stored once per clip (or once per worker, and added up in order by the second kernel with the
 // other column sums).  No atomics: the same inputs give the same bits.
@@ -25,8 +25,6 @@ namespace pt {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
-
-constexpr int PER = 8;                 // values of a row per lane
 
 struct GatedArgs {
   const void* x; const void* t; const void* gate;
@@ -78,7 +76,7 @@ struct RowSum {
 };
 
 // columns of a lane: chunks of 16 bytes, neighbouring lanes next to each other
-template <typename T, int WPR>
+template <typename T, int WPR, int PER>
 __device__ __forceinline__ int column(int i) {
   constexpr int V = 16 / sizeof(T), L = 64 * WPR;
   const int lane = threadIdx.x % L;
@@ -87,21 +85,28 @@ __device__ __forceinline__ int column(int i) {
 
 __device__ __forceinline__ unsigned short to_bf16(float x) { return __builtin_bit_cast(unsigned short, (__bf16)x); }
 
+// How rows are read and written: 16 bytes at a time from 16-byte addresses, 16 bytes from any (columns or strides that are no multiples of 16
+// bytes; the hardware takes them), or value by value (rows of less than 16 bytes)
+enum Access { ALIGNED, ANY, SCALAR };
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <typename T> struct Chunk;
+template <> struct Chunk<float> { typedef u32x4 any __attribute__((aligned(4))); static constexpr int V = 4; };
+template <> struct Chunk<unsigned short> { typedef u32x4 any __attribute__((aligned(2))); static constexpr int V = 8; };
+
 // a lane's values of a row as they lie in memory: what is loaded ahead waits in half the registers where it is bf16
-template <typename T, int WPR, bool VEC>
+template <typename T, int WPR, int PER, int ACC>
 struct Raw {
-  static constexpr int V = 16 / (int)sizeof(T), N = PER / V;
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  static constexpr int V = Chunk<T>::V, N = PER / V;
   u32x4 x[N];
   __device__ __forceinline__ void load(const T* __restrict__ p, int cols) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int c0 = column<T, WPR>(c * V);
-      if constexpr (VEC) {
-        // lanes behind the last column read the last ones again: nothing they compute is summed up or stored, and a load without
-        // a branch is one that nobody waits for before its value is needed
-        x[c] = *reinterpret_cast<const u32x4*>(p + min(c0, cols - V));
-      } else {
+      const int c0 = column<T, WPR, PER>(c * V);
+      // lanes behind the last column read the last ones again: nothing they compute is summed up or stored, and a load without
+      // a branch is one that nobody waits for before its value is needed
+      if constexpr (ACC == ALIGNED) x[c] = *reinterpret_cast<const u32x4*>(p + min(c0, cols - V));
+      else if constexpr (ACC == ANY) x[c] = *reinterpret_cast<const typename Chunk<T>::any*>(p + min(c0, cols - V));
+      else {
         x[c] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -112,21 +117,33 @@ struct Raw {
       }
     }
   }
-  __device__ __forceinline__ void get(float (&v)[PER]) const {
+  __device__ __forceinline__ void get(float (&v)[PER], int cols) const {
 #pragma unroll
-    for (int c = 0; c < N; ++c)
+    for (int c = 0; c < N; ++c) {
+      u32x4 y = x[c];
+      if constexpr (ACC == ANY) {
+        // the lane across the row's end read from cols - V on: down by what that is too early
+        const int early = column<T, WPR, PER>(c * V) + V - cols, by = early > 0 && early < V ? early : 0;
+        if constexpr (V == 8) {
+          const u32x4 s = {y[0] >> 16 | y[1] << 16, y[1] >> 16 | y[2] << 16, y[2] >> 16 | y[3] << 16, y[3] >> 16};
+          y = by & 1 ? s : y;
+        }
+        y = by & V / 4 ? u32x4{y[1], y[2], y[3], y[3]} : y;
+        y = by & V / 2 ? u32x4{y[2], y[3], y[3], y[3]} : y;
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if constexpr (V == 4) { const unsigned u = x[c][j]; v[c * V + j] = __uint_as_float(u); }
-        else { const unsigned u = x[c][j / 2]; v[c * V + j] = __uint_as_float(j & 1 ? u & 0xFFFF0000u : u << 16); }
+        if constexpr (V == 4) { const unsigned u = y[j]; v[c * V + j] = __uint_as_float(u); }
+        else { const unsigned u = y[j / 2]; v[c * V + j] = __uint_as_float(j & 1 ? u & 0xFFFF0000u : u << 16); }
       }
+    }
   }
 };
-template <typename T, int WPR, bool VEC>
+template <typename T, int WPR, int PER, int ACC>
 __device__ __forceinline__ void load_row(const T* __restrict__ p, int cols, float (&v)[PER]) {
-  Raw<T, WPR, VEC> r;
+  Raw<T, WPR, PER, ACC> r;
   r.load(p, cols);
-  r.get(v);
+  r.get(v, cols);
 }
 template <typename Q>
 __device__ __forceinline__ void put(Q* p, const Q& q, bool stream) {
@@ -139,40 +156,41 @@ __device__ __forceinline__ void put(Q* p, const Q& q, bool stream) {
   }
 }
 // stream: outputs larger than the caches, which would only push out what is read again
-template <typename T, int WPR, bool VEC>
+template <typename T, int WPR, int PER, int ACC>
 __device__ __forceinline__ void store_row(T* __restrict__ p, int cols, const float (&v)[PER], bool stream = false) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = Chunk<T>::V;
 #pragma unroll
   for (int c = 0; c < PER / V; ++c) {
-    const int c0 = column<T, WPR>(c * V);
-    if constexpr (VEC) {
-      if (c0 < cols) {
-        if constexpr (V == 4) {
-          const f32x4 q = {v[c * V], v[c * V + 1], v[c * V + 2], v[c * V + 3]};
-          put(reinterpret_cast<f32x4*>(p + c0), q, stream);
-        } else {
-          u16x8 q;
+    const int c0 = column<T, WPR, PER>(c * V);
+    unsigned short b[V];
+    if constexpr (V == 8)
 #pragma unroll
-          for (int j = 0; j < V; ++j) q[j] = to_bf16(v[c * V + j]);
-          put(reinterpret_cast<u16x8*>(p + c0), q, stream);
-        }
+      for (int j = 0; j < V; ++j) b[j] = to_bf16(v[c * V + j]);
+    if (ACC != SCALAR && c0 + V <= cols) {
+      u32x4 q;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (V == 4) q[j] = __float_as_uint(v[c * V + j]);
+        else q[j] = b[2 * j] | (unsigned)b[2 * j + 1] << 16;
       }
-    } else {
+      if constexpr (ACC == ALIGNED) put(reinterpret_cast<u32x4*>(p + c0), q, stream);
+      else *reinterpret_cast<typename Chunk<T>::any*>(p + c0) = q;
+    } else if (ACC != ALIGNED) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (c0 + j < cols) {
           if constexpr (V == 4) p[c0 + j] = v[c * V + j];
-          else p[c0 + j] = to_bf16(v[c * V + j]);
+          else p[c0 + j] = b[j];
         }
     }
   }
 }
 // a column vector in fp32 at the columns of T's chunks; `fill` where there is none
-template <typename T, int WPR>
+template <typename T, int WPR, int PER>
 __device__ __forceinline__ void load_cols(const float* __restrict__ p, int cols, float fill, float (&v)[PER]) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int c = column<T, WPR>(i);
+    const int c = column<T, WPR, PER>(i);
     v[i] = p ? (c < cols ? p[c] : 0.f) : fill;
   }
 }
@@ -191,27 +209,27 @@ __device__ __forceinline__ void worker_rows(const GatedArgs& g, int worker, int&
 }
 
 // mean and 1/std of the values; what lies behind the last column is kept out of the sums
-template <typename T, int WPR, bool LAYER>
+template <typename T, int WPR, int PER, bool LAYER>
 __device__ __forceinline__ void row_stats(const float (&v)[PER], int cols, float inv_cols, float eps, RowSum<WPR>& sum, float& mean, float& rstd) {
   mean = 0.f;
   if constexpr (LAYER) {
     float s = 0.f, z = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s += column<T, WPR>(i) < cols ? v[i] : 0.f;
+    for (int i = 0; i < PER; ++i) s += column<T, WPR, PER>(i) < cols ? v[i] : 0.f;
     sum(s, z);
     mean = s * inv_cols;
   }
   float q = 0.f, z = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const float d = column<T, WPR>(i) < cols ? v[i] - mean : 0.f;
+    const float d = column<T, WPR, PER>(i) < cols ? v[i] - mean : 0.f;
     q += d * d;
   }
   sum(q, z);
   rstd = 1.f / sqrtf(q * inv_cols + eps);
 }
 
-template <typename T, int WPR, bool LAYER, bool VEC>
+template <typename T, int WPR, int PER, bool LAYER, int ACC>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kernel(const GatedArgs g) {
   constexpr int L = 64 * WPR, THREADS = WPR > 4 ? L : 256, RPB = THREADS / L;
   __shared__ float red[2 * 2 * (THREADS / 64)];
@@ -223,14 +241,14 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
   const T* __restrict__ X = (const T*)g.x;
   const T* __restrict__ Tt = (const T*)g.t;
   float a[PER], w1[PER], b1[PER], w2[PER], b2[PER], gt[PER];
-  load_cols<T, WPR>(g.a, cols, 1.f, a);
-  load_cols<T, WPR>(g.w1, cols, 1.f, w1);
-  load_cols<T, WPR>(g.b1, cols, 0.f, b1);
-  load_cols<T, WPR>(g.w2, cols, 1.f, w2);
-  load_cols<T, WPR>(g.b2, cols, 0.f, b2);
+  load_cols<T, WPR, PER>(g.a, cols, 1.f, a);
+  load_cols<T, WPR, PER>(g.w1, cols, 1.f, w1);
+  load_cols<T, WPR, PER>(g.b1, cols, 0.f, b1);
+  load_cols<T, WPR, PER>(g.w2, cols, 1.f, w2);
+  load_cols<T, WPR, PER>(g.b2, cols, 0.f, b2);
 #pragma unroll
   for (int i = 0; i < PER; ++i) gt[i] = a[i];
-  Raw<T, WPR, VEC> nx, nt;                               // without t: x in its place, not used
+  Raw<T, WPR, PER, ACC> nx, nt;                               // without t: x in its place, not used
   auto fetch = [&](int row) {
     row = min(row, g.rows - 1);
     nx.load(X + (size_t)row * g.ldx, cols);
@@ -242,13 +260,13 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
     const int row = r0 + k;
     const bool on = row < r1;
     float x[PER], t[PER];
-    nx.get(x);
-    nt.get(t);
+    nx.get(x, cols);
+    nt.get(t, cols);
     fetch(row + 1);
     if (g.gate && on && left == 0) {
       const int clip = row / g.clip;
       left = (clip + 1) * g.clip - row;
-      load_row<T, WPR, VEC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
+      load_row<T, WPR, PER, ACC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
 #pragma unroll
       for (int i = 0; i < PER; ++i) gt[i] *= a[i];
     }
@@ -260,20 +278,20 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
     float mt = 0.f, rt = 1.f, my = 0.f, ry = 1.f;
     if (Tt) {
       if (g.w1) {
-        row_stats<T, WPR, LAYER>(t, cols, inv_cols, g.eps, sum, mt, rt);
+        row_stats<T, WPR, PER, LAYER>(t, cols, inv_cols, g.eps, sum, mt, rt);
 #pragma unroll
         for (int i = 0; i < PER; ++i) t[i] = (t[i] - mt) * rt * w1[i] + b1[i];
       }
 #pragma unroll
       for (int i = 0; i < PER; ++i) x[i] += gt[i] * t[i];
-      if (on) store_row<T, WPR, VEC>((T*)g.y + (size_t)row * cols, cols, x, g.stream);
+      if (on) store_row<T, WPR, PER, ACC>((T*)g.y + (size_t)row * cols, cols, x, g.stream);
     }
     if (g.w2) {
       // from the sum in fp32, not from the stored y: one rounding less in h
-      row_stats<T, WPR, LAYER>(x, cols, inv_cols, g.eps, sum, my, ry);
+      row_stats<T, WPR, PER, LAYER>(x, cols, inv_cols, g.eps, sum, my, ry);
 #pragma unroll
       for (int i = 0; i < PER; ++i) x[i] = (x[i] - my) * ry * w2[i] + b2[i];
-      if (on) store_row<T, WPR, VEC>((T*)g.h + (size_t)row * cols, cols, x, g.stream);
+      if (on) store_row<T, WPR, PER, ACC>((T*)g.h + (size_t)row * cols, cols, x, g.stream);
     }
     if (g.stats && on && threadIdx.x % L == 0) {
       const f32x4 s = {mt, rt, my, ry};
@@ -283,8 +301,8 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
 }
 
 // BIAS: with biases (b1, or a bias' gradient is wanted)
-template <typename T, int WPR, bool LAYER, bool VEC, bool BIAS>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void gated_norm_bwd_kernel(const GatedArgs g) {
+template <typename T, int WPR, int PER, bool LAYER, int ACC, bool BIAS>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_kernel(const GatedArgs g) {
   constexpr int L = 64 * WPR, THREADS = WPR > 4 ? L : 256, RPB = THREADS / L;
   __shared__ float red[2 * 2 * (THREADS / 64)];
   __shared__ float join[RPB > 1 ? RPB * L * PER : 1];
@@ -298,24 +316,42 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void g
   const T* __restrict__ Tt = (const T*)g.t;
   const T* __restrict__ DY = (const T*)g.dy;
   const T* __restrict__ DH = (const T*)g.dh;
-  // 16 waves leave 128 registers a lane: the column vectors are then read for every row (they stay in the caches) and the
-  // next row's loads do not run ahead; with both kept the kernel would spill 150 registers
-  constexpr bool WIDE = WPR == 16;
+  // 16 values a lane: with the column vectors in registers too the kernel would spill, so these lie in LDS, where every lane reads what
+  // it put there itself; and where the next row's loads do not fit either, they do not run ahead
+  constexpr bool WIDE = PER > 8, AHEAD = !WIDE || (sizeof(T) == 2 && !BIAS);
+  extern __shared__ __attribute__((aligned(16))) float wide[];           // [4][PER / 4][L][4]: w1 a, w2, gate, b1 a
   float w1[PER], b1[PER], w2[PER], gt[PER];              // w1 a, b1 a, w2, the gate
-  auto columns = [&]() {
+  {
     float a[PER];
-    load_cols<T, WPR>(g.a, cols, 1.f, a);
-    load_cols<T, WPR>(g.w1, cols, 1.f, w1);
-    if constexpr (BIAS) load_cols<T, WPR>(g.b1, cols, 0.f, b1);
-    load_cols<T, WPR>(g.w2, cols, 1.f, w2);
+    load_cols<T, WPR, PER>(g.a, cols, 1.f, a);
+    load_cols<T, WPR, PER>(g.w1, cols, 1.f, w1);
+    if constexpr (BIAS) load_cols<T, WPR, PER>(g.b1, cols, 0.f, b1);
+    load_cols<T, WPR, PER>(g.w2, cols, 1.f, w2);
 #pragma unroll
     for (int i = 0; i < PER; ++i) { w1[i] *= a[i]; b1[i] = BIAS ? b1[i] * a[i] : 0.f; }
+  }
+  auto wide_at = [&](int q, int i) { return wide + ((q * (PER / 4) + i / 4) * L + threadIdx.x % L) * 4 + i % 4; };
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      *wide_at(0, i) = w1[i];
+      *wide_at(1, i) = w2[i];
+      *wide_at(2, i) = 1.f;
+      if constexpr (BIAS) *wide_at(3, i) = b1[i];
+    }
+  }
+  // a column vector for the next use, from where it is held
+  auto again = [&](int q, float (&v)[PER]) {
+    if constexpr (WIDE) {
+      asm volatile("" ::: "memory");                       // a read of its own, not one kept in registers
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = *wide_at(q, i);
+    }
   };
-  if constexpr (!WIDE) columns();
   float aw[PER], ab[PER], bw[PER], bb[PER], dg[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) { gt[i] = 1.f; aw[i] = ab[i] = bw[i] = bb[i] = dg[i] = 0.f; }
-  Raw<T, WPR, VEC> nx, nt, ny, nh;
+  Raw<T, WPR, PER, ACC> nx, nt, ny, nh;
   f32x4 ns = {0.f, 0.f, 0.f, 0.f};
   auto fetch = [&](int row) {                            // what is left out: x in its place, not used
     row = min(row, g.rows - 1);
@@ -326,22 +362,18 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void g
     nh.load(DH ? DH + (size_t)row * cols : x, cols);
     ns = *reinterpret_cast<const f32x4*>(g.stats + (size_t)row * 4);
   };
-  if (!WIDE) fetch(r0);
+  if (AHEAD) fetch(r0);
   int left = 0, clip = 0;
   for (int k = 0; k < g.run; ++k) {
     const int row = r0 + k;
     const bool on = row < r1;
-    if constexpr (WIDE) {
-      asm volatile("" ::: "memory");                       // keeps the reads in the loop
-      columns();
-      fetch(row);
-    }
+    if (!AHEAD) fetch(row);
     float x[PER], t[PER], dy[PER], dh[PER];
     const f32x4 st = ns;
-    nx.get(x);
-    nt.get(t);
-    ny.get(dy);
-    nh.get(dh);
+    nx.get(x, cols);
+    nt.get(t, cols);
+    ny.get(dy, cols);
+    nh.get(dh, cols);
     if (!on || !DY)
 #pragma unroll
       for (int i = 0; i < PER; ++i) dy[i] = 0.f;
@@ -351,13 +383,20 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void g
     if (!on)                                               // a row that is another's: finite or not, it adds nothing
 #pragma unroll
       for (int i = 0; i < PER; ++i) x[i] = dh[i] = 0.f;
-    if (!WIDE) fetch(row + 1);
+    if (AHEAD) fetch(row + 1);
     if (g.gate && on && left == 0) {
       clip = row / g.clip;
       left = (clip + 1) * g.clip - row;
-      load_row<T, WPR, VEC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
+      load_row<T, WPR, PER, ACC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
+      if constexpr (WIDE)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) *wide_at(2, i) = gt[i];
     }
     --left;
+    again(0, w1);
+    again(2, gt);
+    if constexpr (BIAS) again(3, b1);
+    again(1, w2);
     // t: t^, x: y^
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -365,12 +404,13 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void g
       t[i] = g.w1 ? (t[i] - st[0]) * st[1] : t[i];
       x[i] += gt[i] * (t[i] * w1[i] + (BIAS ? b1[i] : 0.f));
       x[i] = (x[i] - st[2]) * st[3];
-      const float dn = column<T, WPR>(i) < cols ? dh[i] * w2[i] : 0.f;
+      const float dn = column<T, WPR, PER>(i) < cols ? dh[i] * w2[i] : 0.f;
       s1 += dn;
       s2 += dn * x[i];
     }
     if (DH) {
       sum(s1, s2);
+      again(1, w2);
       const float m1 = LAYER ? s1 * inv_cols : 0.f, m2 = s2 * inv_cols;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -379,12 +419,15 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void g
         dy[i] += st[3] * (dh[i] * w2[i] - m1 - x[i] * m2);
       }
     }
-    if (on) store_row<T, WPR, VEC>((T*)g.dx + (size_t)row * cols, cols, dy, g.stream);
+    if (on) store_row<T, WPR, PER, ACC>((T*)g.dx + (size_t)row * cols, cols, dy, g.stream);
     if (Tt) {
       float s3 = 0.f, s4 = 0.f;
+      again(0, w1);
+      again(2, gt);
+      if constexpr (BIAS) again(3, b1);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const float d = on && column<T, WPR>(i) < cols ? dy[i] : 0.f, gd = gt[i] * d;
+        const float d = on && column<T, WPR, PER>(i) < cols ? dy[i] : 0.f, gd = gt[i] * d;
         aw[i] += gd * t[i];
         if constexpr (BIAS) ab[i] += gd;
         dg[i] += d * (t[i] * w1[i] + (BIAS ? b1[i] : 0.f));
@@ -398,14 +441,14 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void g
 #pragma unroll
         for (int i = 0; i < PER; ++i) dy[i] = st[1] * (dy[i] - m3 - t[i] * m4);
       }
-      if (on && g.dt) store_row<T, WPR, VEC>((T*)g.dt + (size_t)row * cols, cols, dy, g.stream);
+      if (on && g.dt) store_row<T, WPR, PER, ACC>((T*)g.dt + (size_t)row * cols, cols, dy, g.stream);
     }
     if (g.dgate && on && (left == 0 || row + 1 == r1)) {
       if (g.gpart) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) if (column<T, WPR>(i) < cols) g.gpart[(size_t)worker * cols + column<T, WPR>(i)] = dg[i];
+        for (int i = 0; i < PER; ++i) if (column<T, WPR, PER>(i) < cols) g.gpart[(size_t)worker * cols + column<T, WPR, PER>(i)] = dg[i];
       } else {
-        store_row<T, WPR, VEC>((T*)g.dgate + (size_t)clip * cols, cols, dg);
+        store_row<T, WPR, PER, ACC>((T*)g.dgate + (size_t)clip * cols, cols, dg);
       }
 #pragma unroll
       for (int i = 0; i < PER; ++i) dg[i] = 0.f;
@@ -434,7 +477,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, WPR == 16 ? 4 : 2) void g
       if (who) continue;
     }
 #pragma unroll
-    for (int i = 0; i < PER; ++i) if (column<T, WPR>(i) < cols) out[(size_t)q * cols + column<T, WPR>(i)] = v[i];
+    for (int i = 0; i < PER; ++i) if (column<T, WPR, PER>(i) < cols) out[(size_t)q * cols + column<T, WPR, PER>(i)] = v[i];
   }
 }
 
@@ -491,13 +534,14 @@ __global__ __launch_bounds__(1024) void gated_norm_finish_kernel(const GatedFini
 }
 
 // ---------------------------------------------------------------------------
-struct GatedPlan { int wpr, rpb, run, spc, workers, blocks; };
+struct GatedPlan { int wpr, per, rpb, run, spc, workers, blocks; };
 // As many waves as a CU holds (backward: half of that, for the registers), each with rows of its own to walk: enough loads in flight (a
 // wave holds two rows' worth), and few partial sums
 constexpr int FWD_WAVES = 16, BWD_WAVES = 8;
 static GatedPlan gated_plan(int rows, int cols, int clip, bool gate, int waves) {
   GatedPlan p;
-  p.wpr = cols <= 512 ? 1 : cols <= 1024 ? 2 : cols <= 2048 ? 4 : cols <= 4096 ? 8 : 16;
+  p.wpr = cols <= 512 ? 1 : cols <= 1024 ? 2 : cols <= 2048 ? 4 : 8;
+  p.per = cols <= 4096 ? 8 : 16;
   p.rpb = p.wpr >= 4 ? 1 : 4 / p.wpr;
   const int64_t want = (int64_t)device_cus() * waves / p.wpr;
   const int64_t run = std::max<int64_t>(1, (rows + want - 1) / want);
@@ -523,27 +567,37 @@ size_t gated_norm_workspace(int rows, int cols, int clip) {
   return ((size_t)p.blocks * 4 + (p.spc ? p.workers : 0)) * cols * sizeof(float);
 }
 
-template <typename T, int WPR, bool LAYER, bool VEC>
+template <typename T, int WPR, int PER, bool LAYER, int ACC>
 static int run_gated(const GatedArgs& g, const GatedPlan& p, int back, hipStream_t s) {
   constexpr int threads = WPR > 4 ? 64 * WPR : 256;
-  if (back == 2) PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, LAYER, VEC, true>), dim3(p.blocks), dim3(threads), 0, s, g);
-  else if (back) PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, LAYER, VEC, false>), dim3(p.blocks), dim3(threads), 0, s, g);
-  else PT_LAUNCH((gated_norm_fwd_kernel<T, WPR, LAYER, VEC>), dim3(p.blocks), dim3(threads), 0, s, g);
+  constexpr int lds = PER > 8 ? 64 * WPR * PER * (int)sizeof(float) : 0;         // a column vector
+  if (back == 2) {
+    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, WPR, PER, LAYER, ACC, true>), 4 * lds);
+    PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, PER, LAYER, ACC, true>), dim3(p.blocks), dim3(threads), 4 * lds, s, g);
+  } else if (back) {
+    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, WPR, PER, LAYER, ACC, false>), 3 * lds);
+    PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, PER, LAYER, ACC, false>), dim3(p.blocks), dim3(threads), 3 * lds, s, g);
+  } else PT_LAUNCH((gated_norm_fwd_kernel<T, WPR, PER, LAYER, ACC>), dim3(p.blocks), dim3(threads), 0, s, g);
   return 0;
 }
-template <typename T, int WPR>
-static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, bool vec, int back, hipStream_t s) {
-  return layer ? (vec ? run_gated<T, WPR, true, true>(g, p, back, s) : run_gated<T, WPR, true, false>(g, p, back, s))
-               : (vec ? run_gated<T, WPR, false, true>(g, p, back, s) : run_gated<T, WPR, false, false>(g, p, back, s));
+template <typename T, int WPR, int PER, bool LAYER>
+static int run_gated(const GatedArgs& g, const GatedPlan& p, Access acc, int back, hipStream_t s) {
+  if (acc == ALIGNED) return run_gated<T, WPR, PER, LAYER, ALIGNED>(g, p, back, s);
+  if constexpr (WPR == 1)
+    if (acc == SCALAR) return run_gated<T, WPR, PER, LAYER, SCALAR>(g, p, back, s);
+  return run_gated<T, WPR, PER, LAYER, ANY>(g, p, back, s);
+}
+template <typename T, int WPR, int PER>
+static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, Access acc, int back, hipStream_t s) {
+  return layer ? run_gated<T, WPR, PER, true>(g, p, acc, back, s) : run_gated<T, WPR, PER, false>(g, p, acc, back, s);
 }
 template <typename T>
-static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, bool vec, int back, hipStream_t s) {
+static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, Access acc, int back, hipStream_t s) {
   switch (p.wpr) {
-    case 1: return run_gated<T, 1>(g, p, layer, vec, back, s);
-    case 2: return run_gated<T, 2>(g, p, layer, vec, back, s);
-    case 4: return run_gated<T, 4>(g, p, layer, vec, back, s);
-    case 8: return run_gated<T, 8>(g, p, layer, vec, back, s);
-    default: return run_gated<T, 16>(g, p, layer, vec, back, s);
+    case 1: return run_gated<T, 1, 8>(g, p, layer, acc, back, s);
+    case 2: return run_gated<T, 2, 8>(g, p, layer, acc, back, s);
+    case 4: return run_gated<T, 4, 8>(g, p, layer, acc, back, s);
+    default: return p.per == 8 ? run_gated<T, 8, 8>(g, p, layer, acc, back, s) : run_gated<T, 8, 16>(g, p, layer, acc, back, s);
   }
 }
 
@@ -558,11 +612,12 @@ static int check_gated(const char* who, const void* x, int64_t ldx, const void* 
 // Two outputs of 64 MB or more together leave the 256 MB of Infinity Cache to x and t, which the backward pass reads again (512 x 88 rows of
 // 512 fp32, both passes: 208 -> 192 us; 16,384 x 4096 bf16: 297 -> 287); smaller ones stay in the caches for the next operator
 static int gated_stream(const GatedArgs& g, int dtype) { return (int64_t)g.rows * g.cols * (dtype ? 2 : 4) * 2 >= ((int64_t)64 << 20); }
-static bool gated_vec(const GatedArgs& g, int dtype) {
+static Access gated_access(const GatedArgs& g, int dtype) {
   const size_t v = dtype ? 8 : 4;
   const uintptr_t p = (uintptr_t)g.x | (uintptr_t)g.t | (uintptr_t)g.gate | (uintptr_t)g.dy | (uintptr_t)g.dh | (uintptr_t)g.y | (uintptr_t)g.h |
                       (uintptr_t)g.dx | (uintptr_t)g.dt | (uintptr_t)g.dgate;
-  return !(p & 15) && g.cols % v == 0 && g.ldx % v == 0 && (!g.t || g.ldt % v == 0);
+  if ((size_t)g.cols < v) return SCALAR;
+  return !(p & 15) && g.cols % v == 0 && g.ldx % v == 0 && (!g.t || g.ldt % v == 0) ? ALIGNED : ANY;
 }
 
 int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1,
@@ -576,8 +631,8 @@ int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   const GatedPlan p = gated_plan(g.rows, cols, g.clip, gate != nullptr, FWD_WAVES);
   g.run = p.run; g.spc = p.spc;
   g.stream = gated_stream(g, dtype);
-  const bool vec = gated_vec(g, dtype);
-  return dtype ? run_gated<unsigned short>(g, p, kind == 0, vec, 0, s) : run_gated<float>(g, p, kind == 0, vec, 0, s);
+  const Access acc = gated_access(g, dtype);
+  return dtype ? run_gated<unsigned short>(g, p, kind == 0, acc, 0, s) : run_gated<float>(g, p, kind == 0, acc, 0, s);
 }
 
 int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1,
@@ -597,9 +652,9 @@ int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   g.part = (float*)ws;
   g.gpart = p.spc && dgate ? g.part + (size_t)p.blocks * 4 * cols : nullptr;
   g.stream = gated_stream(g, dtype);
-  const bool vec = gated_vec(g, dtype);
+  const Access acc = gated_access(g, dtype);
   const int bias = b1 || db1 || db2 ? 1 : 0;
-  if (dtype ? run_gated<unsigned short>(g, p, kind == 0, vec, 1 + bias, s) : run_gated<float>(g, p, kind == 0, vec, 1 + bias, s)) return 1;
+  if (dtype ? run_gated<unsigned short>(g, p, kind == 0, acc, 1 + bias, s) : run_gated<float>(g, p, kind == 0, acc, 1 + bias, s)) return 1;
   GatedFinish f = {};
   f.part = g.part; f.gpart = g.gpart; f.a = a; f.w1 = w1; f.b1 = b1;
   f.da = t ? da : nullptr; f.dw1 = t ? dw1 : nullptr; f.db1 = t ? db1 : nullptr; f.dw2 = dw2; f.db2 = db2;
