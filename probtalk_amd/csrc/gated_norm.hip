@@ -12,10 +12,14 @@
 // Bound by HBM: forward 2 rows in and 2 out, backward 4 in and 2 out.  y and the statistics' arguments are recomputed from x and t
 // (the same bytes as reading a stored y, and exact where y is held in bf16); only 4 floats a row are kept from the forward pass.
 //
-// A row is held by WPR waves, PER values a lane; a worker (these waves) walks a run of rows, so the column vectors stay in registers
+// A row is held by L lanes (8 to 512), PER values each; a worker (these lanes) walks a run of rows, so the column vectors stay in registers
 // and the column sums of the backward pass are register adds.  A worker's rows lie in one clip, or are whole clips, so the gate's
-// gradient is a register sum too, stored once per clip (or once per worker, and added up in order by the second kernel with the
-// other column sums).  No atomics: the same inputs give the same bits.
+// gradient is a register sum too, stored once per clip (or joined within the block, and added up in order by the second kernel with
+// the other column sums).  No atomics: the same inputs give the same bits.
+//
+// Measured: 49,152 x 2048 bf16 forward 180 us (4.5 TB/s; a copy of this size runs at 4.9); 45,056 x 512 fp32 forward 64 us (5.7 TB/s), with all
+// gradients 192; 16,384 x 4096 bf16 with gradients 287; lanes to the row's length: 200,000 x 64 bf16 forward 107 -> 27 us, with
+// gradients 349 -> 189
 #include <algorithm>
 #include <cstdint>
 
@@ -33,10 +37,11 @@ struct GatedArgs {
   void* y; void* h; float* stats;      // stats [rows][4]: mean t, 1/std t, mean y, 1/std y
   void* dx; void* dt; void* dgate;
   float* part;                         // [blocks][4][cols]: sum g D t^ | sum g D | sum dh y^ | sum dh
-  float* gpart;                        // [workers][cols]: a worker's share of its clip's gate gradient, or null (whole clips)
+  float* gpart;                        // [workers][cols] (joined: [blocks][cols]): shares of a clip's gate gradient, or null (whole clips)
   size_t ldx, ldt;
   int rows, cols, clip;                // rows per clip (of the gate)
   int run, spc;                        // rows per worker; workers per clip, or 0: a worker takes run / clip whole clips
+  int joined;                          // a block's workers are all of one clip: they share one row of gpart
   float eps;
   int stream;                          // see store_row
 };
@@ -45,22 +50,31 @@ template <int CTRL>
 __device__ __forceinline__ float dpp_sum(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
 }
-// sum over the wave, the same in every lane, without the LDS crossbar
-__device__ __forceinline__ float wave_sum(float v) {
+// sum over L lanes (64: the wave), the same in every one, without the LDS crossbar
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
   v = dpp_sum<0xB1>(v);        // quad_perm [1,0,3,2]
   v = dpp_sum<0x4E>(v);        // quad_perm [2,3,0,1]
   v = dpp_sum<0x141>(v);       // row_half_mirror
-  v = dpp_sum<0x140>(v);       // row_mirror
-  return row_lanes_sum(v);
+  if constexpr (L >= 16) v = dpp_sum<0x140>(v);        // row_mirror
+  if constexpr (L == 32) {
+    const unsigned u = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned a0 = a[0], a1 = a[1];
+    v = __uint_as_float(a0) + __uint_as_float(a1);
+  }
+  if constexpr (L >= 64) v = row_lanes_sum(v);
+  return v;
 }
 
-template <int WPR>
+template <int L>
 struct RowSum {
+  static constexpr int WPR = L / 64;    // waves of a row
   float* slot;                         // LDS [2][RPB][WPR][2]
   int flip = 0;
   __device__ __forceinline__ void operator()(float& a, float& b) {
-    a = wave_sum(a);
-    b = wave_sum(b);
+    a = lanes_sum<L>(a);
+    b = lanes_sum<L>(b);
     if constexpr (WPR > 1) {
       // two slots in turn: a slot is written again only behind the barrier of the other one, which every reader has passed
       float* s = slot + flip * 2 * (blockDim.x >> 6);
@@ -76,9 +90,9 @@ struct RowSum {
 };
 
 // columns of a lane: chunks of 16 bytes, neighbouring lanes next to each other
-template <typename T, int WPR, int PER>
+template <typename T, int L, int PER>
 __device__ __forceinline__ int column(int i) {
-  constexpr int V = 16 / sizeof(T), L = 64 * WPR;
+  constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x % L;
   return (i / V * L + lane) * V + i % V;
 }
@@ -94,14 +108,14 @@ template <> struct Chunk<float> { typedef u32x4 any __attribute__((aligned(4)));
 template <> struct Chunk<unsigned short> { typedef u32x4 any __attribute__((aligned(2))); static constexpr int V = 8; };
 
 // a lane's values of a row as they lie in memory: what is loaded ahead waits in half the registers where it is bf16
-template <typename T, int WPR, int PER, int ACC>
+template <typename T, int L, int PER, int ACC>
 struct Raw {
   static constexpr int V = Chunk<T>::V, N = PER / V;
   u32x4 x[N];
   __device__ __forceinline__ void load(const T* __restrict__ p, int cols) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int c0 = column<T, WPR, PER>(c * V);
+      const int c0 = column<T, L, PER>(c * V);
       // lanes behind the last column read the last ones again: nothing they compute is summed up or stored, and a load without
       // a branch is one that nobody waits for before its value is needed
       if constexpr (ACC == ALIGNED) x[c] = *reinterpret_cast<const u32x4*>(p + min(c0, cols - V));
@@ -123,7 +137,7 @@ struct Raw {
       u32x4 y = x[c];
       if constexpr (ACC == ANY) {
         // the lane across the row's end read from cols - V on: down by what that is too early
-        const int early = column<T, WPR, PER>(c * V) + V - cols, by = early > 0 && early < V ? early : 0;
+        const int early = column<T, L, PER>(c * V) + V - cols, by = early > 0 && early < V ? early : 0;
         if constexpr (V == 8) {
           const u32x4 s = {y[0] >> 16 | y[1] << 16, y[1] >> 16 | y[2] << 16, y[2] >> 16 | y[3] << 16, y[3] >> 16};
           y = by & 1 ? s : y;
@@ -139,9 +153,9 @@ struct Raw {
     }
   }
 };
-template <typename T, int WPR, int PER, int ACC>
+template <typename T, int L, int PER, int ACC>
 __device__ __forceinline__ void load_row(const T* __restrict__ p, int cols, float (&v)[PER]) {
-  Raw<T, WPR, PER, ACC> r;
+  Raw<T, L, PER, ACC> r;
   r.load(p, cols);
   r.get(v, cols);
 }
@@ -156,12 +170,12 @@ __device__ __forceinline__ void put(Q* p, const Q& q, bool stream) {
   }
 }
 // stream: outputs larger than the caches, which would only push out what is read again
-template <typename T, int WPR, int PER, int ACC>
+template <typename T, int L, int PER, int ACC>
 __device__ __forceinline__ void store_row(T* __restrict__ p, int cols, const float (&v)[PER], bool stream = false) {
   constexpr int V = Chunk<T>::V;
 #pragma unroll
   for (int c = 0; c < PER / V; ++c) {
-    const int c0 = column<T, WPR, PER>(c * V);
+    const int c0 = column<T, L, PER>(c * V);
     unsigned short b[V];
     if constexpr (V == 8)
 #pragma unroll
@@ -186,11 +200,11 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, int cols, const flo
   }
 }
 // a column vector in fp32 at the columns of T's chunks; `fill` where there is none
-template <typename T, int WPR, int PER>
+template <typename T, int L, int PER>
 __device__ __forceinline__ void load_cols(const float* __restrict__ p, int cols, float fill, float (&v)[PER]) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int c = column<T, WPR, PER>(i);
+    const int c = column<T, L, PER>(i);
     v[i] = p ? (c < cols ? p[c] : 0.f) : fill;
   }
 }
@@ -209,31 +223,31 @@ __device__ __forceinline__ void worker_rows(const GatedArgs& g, int worker, int&
 }
 
 // mean and 1/std of the values; what lies behind the last column is kept out of the sums
-template <typename T, int WPR, int PER, bool LAYER>
-__device__ __forceinline__ void row_stats(const float (&v)[PER], int cols, float inv_cols, float eps, RowSum<WPR>& sum, float& mean, float& rstd) {
+template <typename T, int L, int PER, bool LAYER>
+__device__ __forceinline__ void row_stats(const float (&v)[PER], int cols, float inv_cols, float eps, RowSum<L>& sum, float& mean, float& rstd) {
   mean = 0.f;
   if constexpr (LAYER) {
     float s = 0.f, z = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s += column<T, WPR, PER>(i) < cols ? v[i] : 0.f;
+    for (int i = 0; i < PER; ++i) s += column<T, L, PER>(i) < cols ? v[i] : 0.f;
     sum(s, z);
     mean = s * inv_cols;
   }
   float q = 0.f, z = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const float d = column<T, WPR, PER>(i) < cols ? v[i] - mean : 0.f;
+    const float d = column<T, L, PER>(i) < cols ? v[i] - mean : 0.f;
     q += d * d;
   }
   sum(q, z);
   rstd = 1.f / sqrtf(q * inv_cols + eps);
 }
 
-template <typename T, int WPR, int PER, bool LAYER, int ACC>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kernel(const GatedArgs g) {
-  constexpr int L = 64 * WPR, THREADS = WPR > 4 ? L : 256, RPB = THREADS / L;
+template <typename T, int L, int PER, bool LAYER, int ACC>
+__global__ __launch_bounds__(L > 256 ? L : 256) void gated_norm_fwd_kernel(const GatedArgs g) {
+  constexpr int THREADS = L > 256 ? L : 256, RPB = THREADS / L;
   __shared__ float red[2 * 2 * (THREADS / 64)];
-  RowSum<WPR> sum{red};
+  RowSum<L> sum{red};
   int r0, r1;
   worker_rows(g, blockIdx.x * RPB + threadIdx.x / L, r0, r1);
   const int cols = g.cols;
@@ -241,14 +255,14 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
   const T* __restrict__ X = (const T*)g.x;
   const T* __restrict__ Tt = (const T*)g.t;
   float a[PER], w1[PER], b1[PER], w2[PER], b2[PER], gt[PER];
-  load_cols<T, WPR, PER>(g.a, cols, 1.f, a);
-  load_cols<T, WPR, PER>(g.w1, cols, 1.f, w1);
-  load_cols<T, WPR, PER>(g.b1, cols, 0.f, b1);
-  load_cols<T, WPR, PER>(g.w2, cols, 1.f, w2);
-  load_cols<T, WPR, PER>(g.b2, cols, 0.f, b2);
+  load_cols<T, L, PER>(g.a, cols, 1.f, a);
+  load_cols<T, L, PER>(g.w1, cols, 1.f, w1);
+  load_cols<T, L, PER>(g.b1, cols, 0.f, b1);
+  load_cols<T, L, PER>(g.w2, cols, 1.f, w2);
+  load_cols<T, L, PER>(g.b2, cols, 0.f, b2);
 #pragma unroll
   for (int i = 0; i < PER; ++i) gt[i] = a[i];
-  Raw<T, WPR, PER, ACC> nx, nt;                               // without t: x in its place, not used
+  Raw<T, L, PER, ACC> nx, nt;                               // without t: x in its place, not used
   auto fetch = [&](int row) {
     row = min(row, g.rows - 1);
     nx.load(X + (size_t)row * g.ldx, cols);
@@ -266,7 +280,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
     if (g.gate && on && left == 0) {
       const int clip = row / g.clip;
       left = (clip + 1) * g.clip - row;
-      load_row<T, WPR, PER, ACC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
+      load_row<T, L, PER, ACC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
 #pragma unroll
       for (int i = 0; i < PER; ++i) gt[i] *= a[i];
     }
@@ -278,20 +292,20 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
     float mt = 0.f, rt = 1.f, my = 0.f, ry = 1.f;
     if (Tt) {
       if (g.w1) {
-        row_stats<T, WPR, PER, LAYER>(t, cols, inv_cols, g.eps, sum, mt, rt);
+        row_stats<T, L, PER, LAYER>(t, cols, inv_cols, g.eps, sum, mt, rt);
 #pragma unroll
         for (int i = 0; i < PER; ++i) t[i] = (t[i] - mt) * rt * w1[i] + b1[i];
       }
 #pragma unroll
       for (int i = 0; i < PER; ++i) x[i] += gt[i] * t[i];
-      if (on) store_row<T, WPR, PER, ACC>((T*)g.y + (size_t)row * cols, cols, x, g.stream);
+      if (on) store_row<T, L, PER, ACC>((T*)g.y + (size_t)row * cols, cols, x, g.stream);
     }
     if (g.w2) {
       // from the sum in fp32, not from the stored y: one rounding less in h
-      row_stats<T, WPR, PER, LAYER>(x, cols, inv_cols, g.eps, sum, my, ry);
+      row_stats<T, L, PER, LAYER>(x, cols, inv_cols, g.eps, sum, my, ry);
 #pragma unroll
       for (int i = 0; i < PER; ++i) x[i] = (x[i] - my) * ry * w2[i] + b2[i];
-      if (on) store_row<T, WPR, PER, ACC>((T*)g.h + (size_t)row * cols, cols, x, g.stream);
+      if (on) store_row<T, L, PER, ACC>((T*)g.h + (size_t)row * cols, cols, x, g.stream);
     }
     if (g.stats && on && threadIdx.x % L == 0) {
       const f32x4 s = {mt, rt, my, ry};
@@ -301,12 +315,12 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void gated_norm_fwd_kerne
 }
 
 // BIAS: with biases (b1, or a bias' gradient is wanted)
-template <typename T, int WPR, int PER, bool LAYER, int ACC, bool BIAS>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_kernel(const GatedArgs g) {
-  constexpr int L = 64 * WPR, THREADS = WPR > 4 ? L : 256, RPB = THREADS / L;
+template <typename T, int L, int PER, bool LAYER, int ACC, bool BIAS>
+__global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(const GatedArgs g) {
+  constexpr int THREADS = L > 256 ? L : 256, RPB = THREADS / L;
   __shared__ float red[2 * 2 * (THREADS / 64)];
   __shared__ float join[RPB > 1 ? RPB * L * PER : 1];
-  RowSum<WPR> sum{red};
+  RowSum<L> sum{red};
   const int worker = blockIdx.x * RPB + threadIdx.x / L;
   int r0, r1;
   worker_rows(g, worker, r0, r1);
@@ -323,10 +337,10 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
   float w1[PER], b1[PER], w2[PER], gt[PER];              // w1 a, b1 a, w2, the gate
   {
     float a[PER];
-    load_cols<T, WPR, PER>(g.a, cols, 1.f, a);
-    load_cols<T, WPR, PER>(g.w1, cols, 1.f, w1);
-    if constexpr (BIAS) load_cols<T, WPR, PER>(g.b1, cols, 0.f, b1);
-    load_cols<T, WPR, PER>(g.w2, cols, 1.f, w2);
+    load_cols<T, L, PER>(g.a, cols, 1.f, a);
+    load_cols<T, L, PER>(g.w1, cols, 1.f, w1);
+    if constexpr (BIAS) load_cols<T, L, PER>(g.b1, cols, 0.f, b1);
+    load_cols<T, L, PER>(g.w2, cols, 1.f, w2);
 #pragma unroll
     for (int i = 0; i < PER; ++i) { w1[i] *= a[i]; b1[i] = BIAS ? b1[i] * a[i] : 0.f; }
   }
@@ -351,7 +365,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
   float aw[PER], ab[PER], bw[PER], bb[PER], dg[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) { gt[i] = 1.f; aw[i] = ab[i] = bw[i] = bb[i] = dg[i] = 0.f; }
-  Raw<T, WPR, PER, ACC> nx, nt, ny, nh;
+  Raw<T, L, PER, ACC> nx, nt, ny, nh;
   f32x4 ns = {0.f, 0.f, 0.f, 0.f};
   auto fetch = [&](int row) {                            // what is left out: x in its place, not used
     row = min(row, g.rows - 1);
@@ -387,7 +401,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
     if (g.gate && on && left == 0) {
       clip = row / g.clip;
       left = (clip + 1) * g.clip - row;
-      load_row<T, WPR, PER, ACC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
+      load_row<T, L, PER, ACC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
       if constexpr (WIDE)
 #pragma unroll
         for (int i = 0; i < PER; ++i) *wide_at(2, i) = gt[i];
@@ -404,7 +418,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
       t[i] = g.w1 ? (t[i] - st[0]) * st[1] : t[i];
       x[i] += gt[i] * (t[i] * w1[i] + (BIAS ? b1[i] : 0.f));
       x[i] = (x[i] - st[2]) * st[3];
-      const float dn = column<T, WPR, PER>(i) < cols ? dh[i] * w2[i] : 0.f;
+      const float dn = column<T, L, PER>(i) < cols ? dh[i] * w2[i] : 0.f;
       s1 += dn;
       s2 += dn * x[i];
     }
@@ -419,7 +433,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
         dy[i] += st[3] * (dh[i] * w2[i] - m1 - x[i] * m2);
       }
     }
-    if (on) store_row<T, WPR, PER, ACC>((T*)g.dx + (size_t)row * cols, cols, dy, g.stream);
+    if (on) store_row<T, L, PER, ACC>((T*)g.dx + (size_t)row * cols, cols, dy, g.stream);
     if (Tt) {
       float s3 = 0.f, s4 = 0.f;
       again(0, w1);
@@ -427,7 +441,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
       if constexpr (BIAS) again(3, b1);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const float d = on && column<T, WPR, PER>(i) < cols ? dy[i] : 0.f, gd = gt[i] * d;
+        const float d = on && column<T, L, PER>(i) < cols ? dy[i] : 0.f, gd = gt[i] * d;
         aw[i] += gd * t[i];
         if constexpr (BIAS) ab[i] += gd;
         dg[i] += d * (t[i] * w1[i] + (BIAS ? b1[i] : 0.f));
@@ -441,14 +455,14 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
 #pragma unroll
         for (int i = 0; i < PER; ++i) dy[i] = st[1] * (dy[i] - m3 - t[i] * m4);
       }
-      if (on && g.dt) store_row<T, WPR, PER, ACC>((T*)g.dt + (size_t)row * cols, cols, dy, g.stream);
+      if (on && g.dt) store_row<T, L, PER, ACC>((T*)g.dt + (size_t)row * cols, cols, dy, g.stream);
     }
-    if (g.dgate && on && (left == 0 || row + 1 == r1)) {
+    if (g.dgate && on && !g.joined && (left == 0 || row + 1 == r1)) {
       if (g.gpart) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) if (column<T, WPR, PER>(i) < cols) g.gpart[(size_t)worker * cols + column<T, WPR, PER>(i)] = dg[i];
+        for (int i = 0; i < PER; ++i) if (column<T, L, PER>(i) < cols) g.gpart[(size_t)worker * cols + column<T, L, PER>(i)] = dg[i];
       } else {
-        store_row<T, WPR, PER, ACC>((T*)g.dgate + (size_t)clip * cols, cols, dg);
+        store_row<T, L, PER, ACC>((T*)g.dgate + (size_t)clip * cols, cols, dg);
       }
 #pragma unroll
       for (int i = 0; i < PER; ++i) dg[i] = 0.f;
@@ -457,11 +471,12 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
   // this block's column sums
   float* __restrict__ out = g.part + (size_t)blockIdx.x * 4 * cols;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (!BIAS && (q & 1)) continue;
+  for (int q = 0; q < 5; ++q) {
+    if ((!BIAS && (q == 1 || q == 3)) || (q == 4 && !g.joined)) continue;
     float v[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = q == 0 ? aw[i] : q == 1 ? ab[i] : q == 2 ? bw[i] : bb[i];
+    for (int i = 0; i < PER; ++i) v[i] = q == 0 ? aw[i] : q == 1 ? ab[i] : q == 2 ? bw[i] : q == 3 ? bb[i] : dg[i];
+    float* to = q < 4 ? out + (size_t)q * cols : g.gpart + (size_t)blockIdx.x * cols;
     if constexpr (RPB > 1) {
       const int lane = threadIdx.x % L, who = threadIdx.x / L;
       __syncthreads();
@@ -470,19 +485,21 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256, 2) void gated_norm_bwd_ke
         for (int i = 0; i < PER; ++i) join[(who * PER + i) * L + lane] = v[i];
       __syncthreads();
       if (!who)
-#pragma unroll
+#pragma unroll 3
         for (int w = 1; w < RPB; ++w)
 #pragma unroll
           for (int i = 0; i < PER; ++i) v[i] += join[(w * PER + i) * L + lane];
       if (who) continue;
     }
 #pragma unroll
-    for (int i = 0; i < PER; ++i) if (column<T, WPR, PER>(i) < cols) out[(size_t)q * cols + column<T, WPR, PER>(i)] = v[i];
+    for (int i = 0; i < PER; ++i) if (column<T, L, PER>(i) < cols) to[column<T, L, PER>(i)] = v[i];
   }
 }
 
 // Adds the blocks' column sums (grid part 1: 64 columns and one of the two norms per block, 16 waves share the blocks) and the
-// workers' shares of each clip's gate gradient (part 2: 256 columns of one clip per block).
+// shares of each clip's gate gradient (part 2: 1024 columns of one clip per block, or from 32 shares on 64 columns and 16 waves that
+// share them out).
+constexpr int GATE_MANY = 32;
 struct GatedFinish {
   const float* part; const float* gpart;
   const float* a; const float* w1; const float* b1;
@@ -524,28 +541,41 @@ __global__ __launch_bounds__(1024) void gated_norm_finish_kernel(const GatedFini
     }
     return;
   }
-  const int k = blockIdx.x - f.n_first, per = (f.cols + 1023) / 1024, clip = k / per, c = (k - clip * per) * 1024 + threadIdx.x;
-  if (c >= f.cols) return;
+  const int k = blockIdx.x - f.n_first, width = f.spc < GATE_MANY ? 1024 : 64, per = (f.cols + width - 1) / width, clip = k / per;
+  const int c = (k - clip * per) * width + threadIdx.x % width, step = 1024 / width;
   float s = 0.f;
+  if (c < f.cols)
 #pragma unroll 8
-  for (int w = 0; w < f.spc; ++w) s += f.gpart[((size_t)clip * f.spc + w) * f.cols + c];
+    for (int w = threadIdx.x / width; w < f.spc; w += step) s += f.gpart[((size_t)clip * f.spc + w) * f.cols + c];
+  if (step > 1) {
+    __shared__ float share[1024];
+    share[threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += share[w * 64 + threadIdx.x];
+  }
+  if (c >= f.cols) return;
   if constexpr (sizeof(T) == 4) ((float*)f.dgate)[(size_t)clip * f.cols + c] = s;
   else ((unsigned short*)f.dgate)[(size_t)clip * f.cols + c] = to_bf16(s);
 }
 
 // ---------------------------------------------------------------------------
-struct GatedPlan { int wpr, per, rpb, run, spc, workers, blocks; };
+struct GatedPlan { int lanes, per, rpb, run, spc, workers, blocks, joined; };
 // As many waves as a CU holds (backward: half of that, for the registers), each with rows of its own to walk: enough loads in flight (a
-// wave holds two rows' worth), and few partial sums
+// wave holds two rows' worth), and few partial sums.  Above 4096 columns 16 values a lane: with 16 waves of 8 values the backward kernel has half
+// the registers and reads the column vectors for every row (8192 x 8192 bf16, both passes 1025 us against 316).
 constexpr int FWD_WAVES = 16, BWD_WAVES = 8;
 static GatedPlan gated_plan(int rows, int cols, int clip, bool gate, int waves) {
   GatedPlan p;
-  p.wpr = cols <= 512 ? 1 : cols <= 1024 ? 2 : cols <= 2048 ? 4 : 8;
   p.per = cols <= 4096 ? 8 : 16;
-  p.rpb = p.wpr >= 4 ? 1 : 4 / p.wpr;
-  const int64_t want = (int64_t)device_cus() * waves / p.wpr;
+  p.lanes = 8;
+  while (p.lanes * p.per < cols) p.lanes *= 2;
+  p.rpb = p.lanes >= 256 ? 1 : 256 / p.lanes;
+  const int64_t want = (int64_t)device_cus() * waves * 64 / p.lanes;
   const int64_t run = std::max<int64_t>(1, (rows + want - 1) / want);
-  p.spc = 0;
+  p.spc = p.joined = 0;
   if (!gate) {
     p.run = (int)run;
     p.workers = (int)((rows + run - 1) / run);
@@ -554,7 +584,9 @@ static GatedPlan gated_plan(int rows, int cols, int clip, bool gate, int waves) 
     p.workers = (int)(((int64_t)rows + p.run - 1) / p.run);
   } else {
     p.spc = (int)((clip + run - 1) / run);
-    p.run = (clip + p.spc - 1) / p.spc;                    // at most `run`, and none of the spc workers is without rows
+    p.joined = p.spc >= p.rpb;
+    if (p.joined) p.spc = (p.spc + p.rpb - 1) / p.rpb * p.rpb;
+    p.run = (clip + p.spc - 1) / p.spc;                    // at most `run`
     p.workers = (rows + clip - 1) / clip * p.spc;
   }
   p.blocks = (p.workers + p.rpb - 1) / p.rpb;
@@ -564,40 +596,43 @@ static GatedPlan gated_plan(int rows, int cols, int clip, bool gate, int waves) 
 size_t gated_norm_workspace(int rows, int cols, int clip) {
   if (rows < 1 || cols < 1 || cols > 8192 || clip < 0) return 0;
   const GatedPlan p = gated_plan(rows, cols, clip ? clip : rows, clip > 0, BWD_WAVES);
-  return ((size_t)p.blocks * 4 + (p.spc ? p.workers : 0)) * cols * sizeof(float);
+  return ((size_t)p.blocks * 4 + (p.joined ? p.blocks : p.spc ? p.workers : 0)) * cols * sizeof(float);
 }
 
-template <typename T, int WPR, int PER, bool LAYER, int ACC>
+template <typename T, int L, int PER, bool LAYER, int ACC>
 static int run_gated(const GatedArgs& g, const GatedPlan& p, int back, hipStream_t s) {
-  constexpr int threads = WPR > 4 ? 64 * WPR : 256;
-  constexpr int lds = PER > 8 ? 64 * WPR * PER * (int)sizeof(float) : 0;         // a column vector
+  constexpr int threads = L > 256 ? L : 256;
+  constexpr int lds = PER > 8 ? L * PER * (int)sizeof(float) : 0;         // a column vector
   if (back == 2) {
-    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, WPR, PER, LAYER, ACC, true>), 4 * lds);
-    PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, PER, LAYER, ACC, true>), dim3(p.blocks), dim3(threads), 4 * lds, s, g);
+    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, L, PER, LAYER, ACC, true>), 4 * lds);
+    PT_LAUNCH((gated_norm_bwd_kernel<T, L, PER, LAYER, ACC, true>), dim3(p.blocks), dim3(threads), 4 * lds, s, g);
   } else if (back) {
-    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, WPR, PER, LAYER, ACC, false>), 3 * lds);
-    PT_LAUNCH((gated_norm_bwd_kernel<T, WPR, PER, LAYER, ACC, false>), dim3(p.blocks), dim3(threads), 3 * lds, s, g);
-  } else PT_LAUNCH((gated_norm_fwd_kernel<T, WPR, PER, LAYER, ACC>), dim3(p.blocks), dim3(threads), 0, s, g);
+    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, L, PER, LAYER, ACC, false>), 3 * lds);
+    PT_LAUNCH((gated_norm_bwd_kernel<T, L, PER, LAYER, ACC, false>), dim3(p.blocks), dim3(threads), 3 * lds, s, g);
+  } else PT_LAUNCH((gated_norm_fwd_kernel<T, L, PER, LAYER, ACC>), dim3(p.blocks), dim3(threads), 0, s, g);
   return 0;
 }
-template <typename T, int WPR, int PER, bool LAYER>
+template <typename T, int L, int PER, bool LAYER>
 static int run_gated(const GatedArgs& g, const GatedPlan& p, Access acc, int back, hipStream_t s) {
-  if (acc == ALIGNED) return run_gated<T, WPR, PER, LAYER, ALIGNED>(g, p, back, s);
-  if constexpr (WPR == 1)
-    if (acc == SCALAR) return run_gated<T, WPR, PER, LAYER, SCALAR>(g, p, back, s);
-  return run_gated<T, WPR, PER, LAYER, ANY>(g, p, back, s);
+  if (acc == ALIGNED) return run_gated<T, L, PER, LAYER, ALIGNED>(g, p, back, s);
+  if constexpr (L == 8)
+    if (acc == SCALAR) return run_gated<T, L, PER, LAYER, SCALAR>(g, p, back, s);
+  return run_gated<T, L, PER, LAYER, ANY>(g, p, back, s);
 }
-template <typename T, int WPR, int PER>
+template <typename T, int L, int PER>
 static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, Access acc, int back, hipStream_t s) {
-  return layer ? run_gated<T, WPR, PER, true>(g, p, acc, back, s) : run_gated<T, WPR, PER, false>(g, p, acc, back, s);
+  return layer ? run_gated<T, L, PER, true>(g, p, acc, back, s) : run_gated<T, L, PER, false>(g, p, acc, back, s);
 }
 template <typename T>
 static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, Access acc, int back, hipStream_t s) {
-  switch (p.wpr) {
-    case 1: return run_gated<T, 1, 8>(g, p, layer, acc, back, s);
-    case 2: return run_gated<T, 2, 8>(g, p, layer, acc, back, s);
-    case 4: return run_gated<T, 4, 8>(g, p, layer, acc, back, s);
-    default: return p.per == 8 ? run_gated<T, 8, 8>(g, p, layer, acc, back, s) : run_gated<T, 8, 16>(g, p, layer, acc, back, s);
+  switch (p.lanes) {
+    case 8: return run_gated<T, 8, 8>(g, p, layer, acc, back, s);
+    case 16: return run_gated<T, 16, 8>(g, p, layer, acc, back, s);
+    case 32: return run_gated<T, 32, 8>(g, p, layer, acc, back, s);
+    case 64: return run_gated<T, 64, 8>(g, p, layer, acc, back, s);
+    case 128: return run_gated<T, 128, 8>(g, p, layer, acc, back, s);
+    case 256: return run_gated<T, 256, 8>(g, p, layer, acc, back, s);
+    default: return p.per == 8 ? run_gated<T, 512, 8>(g, p, layer, acc, back, s) : run_gated<T, 512, 16>(g, p, layer, acc, back, s);
   }
 }
 
@@ -651,6 +686,7 @@ int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   g.run = p.run; g.spc = p.spc;
   g.part = (float*)ws;
   g.gpart = p.spc && dgate ? g.part + (size_t)p.blocks * 4 * cols : nullptr;
+  g.joined = p.joined && dgate;
   g.stream = gated_stream(g, dtype);
   const Access acc = gated_access(g, dtype);
   const int bias = b1 || db1 || db2 ? 1 : 0;
@@ -658,10 +694,11 @@ int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   GatedFinish f = {};
   f.part = g.part; f.gpart = g.gpart; f.a = a; f.w1 = w1; f.b1 = b1;
   f.da = t ? da : nullptr; f.dw1 = t ? dw1 : nullptr; f.db1 = t ? db1 : nullptr; f.dw2 = dw2; f.db2 = db2;
-  f.dgate = dgate; f.blocks = p.blocks; f.cols = cols; f.spc = p.spc;
+  f.dgate = dgate; f.blocks = p.blocks; f.cols = cols; f.spc = p.joined ? p.spc / p.rpb : p.spc;
   f.col_blocks = (cols + 63) / 64;
   f.n_first = 2 * f.col_blocks;
-  const int64_t gate_blocks = g.gpart ? (int64_t)(rows / clip) * ((cols + 1023) / 1024) : 0;
+  const int width = f.spc < GATE_MANY ? 1024 : 64;
+  const int64_t gate_blocks = g.gpart ? (int64_t)(rows / clip) * ((cols + width - 1) / width) : 0;
   PT_CHECK(f.n_first + gate_blocks < 0x7FFFFFFF, "gated_norm_bwd: too many clips");
   if (dtype) PT_LAUNCH(gated_norm_finish_kernel<unsigned short>, dim3((unsigned)(f.n_first + gate_blocks)), dim3(1024), 0, s, f);
   else PT_LAUNCH(gated_norm_finish_kernel<float>, dim3((unsigned)(f.n_first + gate_blocks)), dim3(1024), 0, s, f);
