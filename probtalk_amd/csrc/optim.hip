@@ -25,7 +25,7 @@ typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 // exponent bits and M mantissa bits over the quantum `scale`: code c < 2^M stands for c, else for (2^M + (c mod 2^M)) 2^(c / 2^M - 1).
 // First moment: sign bit + M = 3 (TOP = 15 * 2^14).  Second moment, never negative: M = 4 (TOP = 31 * 2^14).
 // The parameters and moments pass through the step once: streaming loads and stores keep the gradients, which the norm has just read,
-// in the caches (norm and step over 40 M fp32 values: 281 -> 217 us, with 8-bit moments 266 -> 217 including the reading of them).
+// in the caches (norm and step over 40 M fp32 values: 281 -> 218 us, with 8-bit moments 266 -> 219 including the reading of them).
 // Codes are rounded stochastically: with b2 = 0.999 a second moment moves by a thousandth per step, far less than half a code
 // step (1/32 to 1/16 of the value), so rounding to nearest would leave it where it is for ever; a rounding whose MEAN is the
 // value follows.  A positive second moment never becomes code 0 (its square root divides).  The 32 random bits of a value are a
@@ -79,7 +79,9 @@ __device__ __forceinline__ unsigned wave_umax(unsigned v) {
 // The list
 // ---------------------------------------------------------------------------
 constexpr int AT = 60;                 // tensors per launch: 60 * 60 bytes of table
-constexpr int UNIT = 4096;             // values per workgroup of the step: 4 waves x 4 blocks of 256
+// Values per workgroup of the step: 4 waves x 2 blocks of 256, in registers that let 8 waves run on a SIMD (4 blocks, 5 waves: 40 M fp32 values
+// 222.5 -> 218.3 us, 160 M bf16 with 8-bit moments 705 -> 697)
+constexpr int UNIT = 2048;
 constexpr int NORM_UNIT = 16384;       // values per workgroup of the norm
 
 struct AdamTab {
@@ -197,7 +199,7 @@ __device__ __forceinline__ float adamw32(float p, float g, float gs, float b1, f
   return p * decay - step_size * (m / denom);
 }
 
-// One wave's 1024 values of tensor i from e0 on.  T: float or bf16 bits (unsigned short); S8: 8-bit moments; FULL: all of them are there and
+// One wave's 512 values of tensor i from e0 on.  T: float or bf16 bits (unsigned short); S8: 8-bit moments; FULL: all of them are there and
 // aligned, so the loads are plain vectors and all of them go out before the first is waited for.
 template <typename T, bool S8, bool FULL>
 __device__ __forceinline__ void adamw_wave(const AdamTab& tab, const AdamHyper& h, const int i, const size_t e0, const size_t n) {
@@ -211,7 +213,7 @@ __device__ __forceinline__ void adamw_wave(const AdamTab& tab, const AdamHyper& 
   if (h.dyn) { bc1 = h.dyn[0]; bc2_sqrt = h.dyn[1]; key = __float_as_uint(h.dyn[2]); }
   const float c1 = 1.f - h.b1, c2 = 1.f - h.b2;
   const float decay = fmaf(-h.lr, h.wd, 1.f), step_size = h.lr / bc1;
-  constexpr int NB = UNIT / 4 / QBLOCK;                  // 4 independent blocks per wave: their loads are in flight together
+  constexpr int NB = UNIT / 4 / QBLOCK;                  // independent blocks of a wave: their loads are in flight together
   float p[NB][4], g[NB][4], m[NB][4], v[NB][4];
   unsigned cm[NB], cv[NB];
   float sm[NB], sv[NB];
@@ -233,7 +235,7 @@ __device__ __forceinline__ void adamw_wave(const AdamTab& tab, const AdamHyper& 
       load4<true>((const float*)tab.v[i], e, n, vec, v[k]);
     }
   }
-  // 8-bit moments: the new moments of all four blocks, then the scales of these eight (block, moment) pairs in eight lanes at once:
+  // 8-bit moments: the new moments of all blocks, then the scales of the (block, moment) pairs in as many lanes at once:
   // a division and a reciprocal cost ten instructions each, and every lane of the wave would compute the same
   float inv_m[NB], inv_v[NB];
   if constexpr (S8) {
