@@ -104,6 +104,34 @@ def test_forward_and_gradients(shape, kind, dtype):
     assert all(torch.equal(again[2][k], grads[k]) for k in NAMES)
 
 
+# each number of lanes a row, one clip that all workers share, rows that are no multiples of 16 bytes, and 16 values a lane
+MORE = [(3000, 33, 3000), (700, 64, 1), (900, 100, 450), (1000, 250, 1000), (2, 7, 1), (400, 3, 100), (50, 4097, 50), (64, 6812, 32), (40, 7354, 20), (300, 8191, 300)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("shape", MORE, ids=str)
+def test_row_lengths(shape, bias, dtype):
+    rows, cols, clip = shape
+    v, dy, dh = make(rows, cols, clip, dtype, () if bias else ("post_bias", "pre_bias"), seed=1)
+    kind = "layer" if bias else "rms"
+    y, h, grads = run(v, clip, kind, dy, dh)
+    out, want, size = oracle(v, clip, kind, 1e-5, dy, dh)
+    check(y, out["y"], size["y"], dtype, 100, "y")
+    check(h, out["h"], size["h"], dtype, 200, "h")
+    for k in grads:
+        check(grads[k], want[k], size[k], v[k].dtype, 600 + rows / 512, k)
+    again = run(v, clip, kind, dy, dh)
+    assert all(torch.equal(again[2][k], grads[k]) for k in grads)
+    # rows of a wider tensor, at odd addresses: the same bits, and what lies beside them is not touched
+    wide = torch.full((rows + 1, cols + 5), float("nan"), device="cuda", dtype=dtype)
+    shifted = wide.flatten()[1:1 + rows * (cols + 5)].view(rows, cols + 5)[:, 2:2 + cols]
+    shifted.copy_(v["x"].detach())
+    same = run({**v, "x": shifted.requires_grad_()}, clip, kind, dy, dh)
+    assert torch.equal(same[0], y) and torch.equal(same[1], h) and all(torch.equal(same[2][k], grads[k]) for k in grads)
+    assert int(torch.isnan(wide).sum()) == wide.numel() - rows * cols
+
+
 PARTS = [("gate",), ("res_scale",), ("gate", "res_scale"), ("post_weight", "post_bias"), ("post_bias", "pre_bias"), ("pre_weight", "pre_bias"),
          ("gate", "res_scale", "post_weight", "post_bias", "pre_weight", "pre_bias"), ("t", "gate", "res_scale", "post_weight", "post_bias"),
          ("t", "gate", "res_scale", "post_weight", "post_bias", "pre_bias")]

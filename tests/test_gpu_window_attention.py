@@ -32,6 +32,15 @@ CASES = {
 }
 
 
+# sinks in two blocks of keys and rows far behind them; key heads that share out over the chip evenly, sequences of all lengths
+MORE = {
+    "many sinks, far rows": (1, 900, 900, 2, 1, 64, 70, 0, 100, None),
+    "sinks beyond a block, a new part": (2, 700, 1000, 4, 2, 48, 30, 5, 65, [1000, 333]),
+    "eight key heads, padded": (4, 300, 300, 4, 2, 64, 90, 90, 0, [300, 1, 170, 64]),
+    "a whole sequence in view": (1, 800, 800, 8, 8, 32, None, 0, 0, None),
+}
+
+
 def make(case, dtype, seed=0):
     B, Nq, Nk, H, Hk, D, left, right, sinks, lengths = case
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -100,9 +109,9 @@ def check(got, want, tol):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("name", sorted(CASES))
+@pytest.mark.parametrize("name", sorted(CASES | MORE))
 def test_forward_and_gradients(name, dtype):
-    case = CASES[name]
+    case = (CASES | MORE)[name]
     q, k, v, do, lengths = make(case, dtype)
     want, tol, see = oracle(q, k, v, do, *case[6:9], lengths)
     got = grads(q, k, v, do, case, lengths)
@@ -283,6 +292,33 @@ def test_step(name, dtype):
         err = (o[b].double() - want["o"][0, 0]).abs()
         assert bool((err <= tol["o"][0, 0]).all()), (b, float((err / tol["o"][0, 0]).max()))
     assert torch.equal(T.window_attention_step(q, k, v, lengths, left, sinks=sinks), o)
+
+
+# two to eight slices, more heads of a group than a tile has columns, and caches that are read past the caches
+MORE_STEPS = {
+    "few slices": (40, 300, 16, 4, 64, None, 0, [300 - 7 * b for b in range(40)]),
+    "group of 40": (2, 200, 80, 2, 40, 150, 2, [200, 33]),
+    "a large cache": (8, 4096, 16, 8, 128, None, 0, [4096, 1, 4095, 31, 2048, 0, 33, 4000]),
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", sorted(MORE_STEPS))
+def test_step_cuts(name, dtype):
+    B, N, H, Hk, D, left, sinks, lens = MORE_STEPS[name]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g).to(dtype)  # noqa: E731
+    q, k, v = n(B, H, D), n(B, N, Hk, D), n(B, N, Hk, D)
+    for b, size in enumerate(lens):
+        k[b, size:], v[b, size:] = math.nan, math.inf
+    o = T.window_attention_step(q, k, v, torch.tensor(lens, dtype=torch.int32, device="cuda"), left, sinks=sinks)
+    for b, size in enumerate(lens):
+        if size == 0:
+            assert bool((o[b] == 0).all())
+            continue
+        want, tol, _ = oracle(q[b:b + 1, None], k[b:b + 1, :size], v[b:b + 1, :size], q[b:b + 1, None], left, 0, sinks, None)
+        err = (o[b].double() - want["o"][0, 0]).abs()
+        assert bool((err <= tol["o"][0, 0]).all()), (b, float((err / tol["o"][0, 0]).max()))
 
 
 def test_step_strides_and_growing_cache_in_a_graph():
