@@ -354,14 +354,13 @@ def attention_cross(q, kv, B, Nq, Nk, p=0.0, seeds=None):
 
 def _strides(*tensors):
     """Strides of all but the last dimension, as the C entries take them (a dimension of one value has none)."""
-    out = []
-    for t in tensors:
-        out += [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
-    return array.array("q", out)
+    return array.array("q", [s if n > 1 else 0 for t in tensors for s, n in zip(t.stride()[:-1], t.shape)])
 
 
 def _has_vectors(t):
     """Whether rows of channels can be read in 16-byte vectors."""
+    if t.is_contiguous() and t.shape[-1] % 8 == 0:
+        return t.data_ptr() % 16 == 0
     strides, per = t.stride(), 16 // t.element_size()
     return strides[-1] == 1 and t.data_ptr() % 16 == 0 and all([n == 1 or s % per == 0 for s, n in zip(strides[:-1], t.shape)])
 
@@ -381,7 +380,8 @@ def _window_attention(q, k, v, lengths, meta, grad):
     if grad:
         stats = torch.empty(L.pt_attention_window_stats_bytes(B, Nq, H, D, meta[10]), device=q.device, dtype=torch.uint8)
     with _on(q.device):
-        check(L.pt_attention_window_fwd(_at(q), _at(k), _at(v), _at(o), _at(stats), _address(_strides(q, k, v)), _at(lengths), *meta, stream()))
+        check(L.pt_attention_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _at(stats), _address(_strides(q, k, v)), _at(lengths),
+                                        *meta, stream()))
     return o, stats
 
 
@@ -409,19 +409,19 @@ class WindowAttention(torch.autograd.Function):
 
 
 def _check_window(what, q, k, v, heads, batch, lengths, left, right, sinks, scale):
-    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != batch or k.shape[3] != q.shape[-1] or k.shape[1] < 1:
-        raise RuntimeError(f"{what}: shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} do not go together")
+    shape, d, dtype = k.shape, q.shape[-1], q.dtype
+    if len(shape) != 4 or v.shape != shape or shape[0] != batch or shape[3] != d or shape[1] < 1:
+        raise RuntimeError(f"{what}: shapes {tuple(q.shape)}, {tuple(shape)} and {tuple(v.shape)} do not go together")
     gpu = q.get_device()
     if gpu < 0 or k.get_device() != gpu or v.get_device() != gpu:
         raise RuntimeError(f"{what}: tensors must be on one GPU, got {q.device}, {k.device} and {v.device}")
-    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype is not q.dtype or v.dtype is not q.dtype:
-        raise RuntimeError(f"{what}: fp32 or bf16, one type for all, got {q.dtype}, {k.dtype} and {v.dtype}")
-    d = q.shape[-1]
-    if d % 8 or not 8 <= d <= 128 or k.shape[2] < 1 or heads < 1 or heads % k.shape[2]:
-        raise RuntimeError(f"{what}: {heads} query heads over {k.shape[2]} key heads of {d} channels (a multiple of 8 up to 128)")
-    if lengths is not None and (lengths.shape != (batch,) or lengths.dtype is not torch.int32 or lengths.get_device() != gpu or not lengths.is_contiguous()):
+    if (dtype is not torch.bfloat16 and dtype is not torch.float32) or k.dtype is not dtype or v.dtype is not dtype:
+        raise RuntimeError(f"{what}: fp32 or bf16, one type for all, got {dtype}, {k.dtype} and {v.dtype}")
+    if d % 8 or not 8 <= d <= 128 or shape[2] < 1 or heads < 1 or heads % shape[2]:
+        raise RuntimeError(f"{what}: {heads} query heads over {shape[2]} key heads of {d} channels (a multiple of 8 up to 128)")
+    if lengths is not None and (lengths.dtype is not torch.int32 or lengths.shape != (batch,) or lengths.get_device() != gpu or not lengths.is_contiguous()):
         raise RuntimeError(f"{what}: lengths must be ({batch},) torch.int32 on {q.device}")
-    left, right = (-1 if n is None else int(n) for n in (left, right))
+    left, right = -1 if left is None else int(left), -1 if right is None else int(right)
     if left < -1 or right < -1 or not 0 <= sinks <= 128:
         raise RuntimeError(f"{what}: a window of {left} to the left and {right} to the right with {sinks} first keys (up to 128)")
     scale = d ** -0.5 if scale is None else float(scale)
@@ -443,14 +443,16 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
     leaves inside the capture (q.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if q.dim() != 4 or q.shape[0] < 1 or q.shape[1] < 1:
         raise RuntimeError(f"window_attention: q is (B, Nq, H, D), got {tuple(q.shape)}")
-    left, right, sinks, scale = _check_window("window_attention", q, k, v, q.shape[2], q.shape[0], lengths, left, right, sinks, scale)
-    if k.shape[1] < q.shape[1]:
-        raise RuntimeError(f"window_attention: {q.shape[1]} rows for {k.shape[1]} keys")
-    meta = (*q.shape[:2], k.shape[1], q.shape[2], k.shape[2], q.shape[3], left, right, sinks, scale, int(q.dtype is torch.bfloat16))
-    q, k, v = (_vectors(t if t.shape[1] == 1 or 0 <= t.stride(1) <= 1 << 20 else t.contiguous()) for t in (q, k, v))
+    B, Nq, H, D = q.shape
+    left, right, sinks, scale = _check_window("window_attention", q, k, v, H, B, lengths, left, right, sinks, scale)
+    _, Nk, Hk, _ = k.shape
+    if Nk < Nq:
+        raise RuntimeError(f"window_attention: {Nq} rows for {Nk} keys")
+    meta = (B, Nq, Nk, H, Hk, D, left, right, sinks, scale, int(q.dtype is torch.bfloat16))
+    q, k, v = [_vectors(t if t.shape[1] == 1 or 0 <= t.stride(1) <= 1 << 20 else t.contiguous()) for t in (q, k, v)]
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return WindowAttention.apply(q, k, v, lengths, meta)
-    return _window_attention(q.detach(), k.detach(), v.detach(), lengths, meta, False)[0]
+    return _window_attention(q, k, v, lengths, meta, False)[0]
 
 
 def window_attention_step(q, k, v, lengths, left=None, sinks=0, scale=None):
@@ -461,17 +463,20 @@ def window_attention_step(q, k, v, lengths, left=None, sinks=0, scale=None):
         raise RuntimeError(f"window_attention_step: q is (B, H, D), got {tuple(q.shape)}")
     if lengths is None:
         raise RuntimeError("window_attention_step: lengths are needed")
-    left, _, sinks, scale = _check_window("window_attention_step", q, k, v, q.shape[1], q.shape[0], lengths, left, 0, sinks, scale)
+    B, H, D = q.shape
+    left, _, sinks, scale = _check_window("window_attention_step", q, k, v, H, B, lengths, left, 0, sinks, scale)
     if not _has_vectors(k) or not _has_vectors(v):
         raise RuntimeError("window_attention_step: a cache's channels must be neighbours, its address and strides multiples of 16 bytes")
     q = _vectors(q)
-    (B, H, D), (N, Hk) = q.shape, k.shape[1:3]
-    o = torch.empty(B, H, D, device=q.device, dtype=q.dtype)
+    _, N, Hk, _ = k.shape
+    device, dtype = q.device, q.dtype
+    o = torch.empty(B, H, D, device=device, dtype=dtype)
     L = _lib.lib()
-    with _on(q.device):
-        ws = torch.empty(L.pt_attention_window_step_workspace_bytes(B, N, H, Hk, D, left, sinks), dtype=torch.uint8, device=q.device)
-        check(L.pt_attention_window_step(_at(q), _at(k), _at(v), _at(o), _address(_strides(q, k, v)), _at(lengths), B, N, H, Hk, D, left, sinks, scale,
-                                         int(q.dtype is torch.bfloat16), _at(ws), ws.numel(), stream()))
+    with _on(device):
+        size = L.pt_attention_window_step_workspace_bytes(B, N, H, Hk, D, left, sinks)
+        ws = o if size <= 16 else torch.empty(size, dtype=torch.uint8, device=device)         # up to 16 bytes: nothing is kept there
+        check(L.pt_attention_window_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _address(_strides(q, k, v)), lengths.data_ptr(), B, N,
+                                         H, Hk, D, left, sinks, scale, int(dtype is torch.bfloat16), ws.data_ptr(), size, stream()))
     return o
 
 
