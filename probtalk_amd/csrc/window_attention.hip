@@ -41,8 +41,8 @@ typedef const __attribute__((address_space(1))) void* glb_ptr_t;
 constexpr float LOG2E = 1.4426950408889634f, SLACK = 8.f;
 
 template <typename T> struct Types;
-template <> struct Types<__bf16> { typedef bf16x8 frag; typedef bf16x4 quad; };
-template <> struct Types<float> { typedef f32x8 frag; typedef f32x4 quad; };
+template <> struct Types<__bf16> { typedef bf16x8 frag; };
+template <> struct Types<float> { typedef f32x8 frag; };
 
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {

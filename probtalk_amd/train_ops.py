@@ -439,8 +439,9 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
     left, right: None for no limit (right = 0 is causal); sinks: first keys that stay visible, up to 128; lengths: int32 (B,), the
     keys of each sequence of a padded batch (what lies behind is not read; all of them by default).  A row that sees nothing gives
     zeros and no gradient.  Softmax and sums are fp32; scale is 1 / sqrt(D) by default.  Keys and values inside a sequence must be
-    finite.  The backward pass is free of atomics: the same inputs give the same bits.  To capture it into a HIP graph, make the
-    leaves inside the capture (q.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
+    finite.  With gradients, bf16 keeps a byte more of every output value for them.  The backward pass is free of
+    atomics: the same inputs give the same bits.  To capture it into a HIP graph, make the leaves inside the capture
+    (q.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if q.dim() != 4 or q.shape[0] < 1 or q.shape[1] < 1:
         raise RuntimeError(f"window_attention: q is (B, Nq, H, D), got {tuple(q.shape)}")
     B, Nq, H, D = q.shape
