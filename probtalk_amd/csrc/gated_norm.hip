@@ -43,6 +43,7 @@ struct GatedArgs {
   int run, spc;                        // rows per worker; workers per clip, or 0: a worker takes run / clip whole clips
   int joined;                          // a block's workers are all of one clip: they share one row of gpart
   float eps;
+  int layer;                           // LayerNorm, else RMSNorm
   int stream;                          // see store_row
 };
 
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void gated_norm_fwd_kernel(const
 }
 
 // BIAS: with biases (b1, or a bias' gradient is wanted)
-template <typename T, int L, int PER, bool LAYER, int ACC, bool BIAS>
+template <typename T, int L, int PER, int ACC, bool BIAS>
 __global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(const GatedArgs g) {
   constexpr int THREADS = L > 256 ? L : 256, RPB = THREADS / L;
   __shared__ float red[2 * 2 * (THREADS / 64)];
@@ -425,7 +426,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(co
     if (DH) {
       sum(s1, s2);
       again(1, w2);
-      const float m1 = LAYER ? s1 * inv_cols : 0.f, m2 = s2 * inv_cols;
+      const float m1 = g.layer ? s1 * inv_cols : 0.f, m2 = s2 * inv_cols;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         bw[i] += dh[i] * x[i];
@@ -451,7 +452,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(co
       }
       if (g.w1) {
         sum(s3, s4);
-        const float m3 = LAYER ? s3 * inv_cols : 0.f, m4 = s4 * inv_cols;
+        const float m3 = g.layer ? s3 * inv_cols : 0.f, m4 = s4 * inv_cols;
 #pragma unroll
         for (int i = 0; i < PER; ++i) dy[i] = st[1] * (dy[i] - m3 - t[i] * m4);
       }
@@ -599,40 +600,37 @@ size_t gated_norm_workspace(int rows, int cols, int clip) {
   return ((size_t)p.blocks * 4 + (p.joined ? p.blocks : p.spc ? p.workers : 0)) * cols * sizeof(float);
 }
 
-template <typename T, int L, int PER, bool LAYER, int ACC>
+template <typename T, int L, int PER, int ACC>
 static int run_gated(const GatedArgs& g, const GatedPlan& p, int back, hipStream_t s) {
   constexpr int threads = L > 256 ? L : 256;
   constexpr int lds = PER > 8 ? L * PER * (int)sizeof(float) : 0;         // a column vector
   if (back == 2) {
-    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, L, PER, LAYER, ACC, true>), 4 * lds);
-    PT_LAUNCH((gated_norm_bwd_kernel<T, L, PER, LAYER, ACC, true>), dim3(p.blocks), dim3(threads), 4 * lds, s, g);
+    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, L, PER, ACC, true>), 4 * lds);
+    PT_LAUNCH((gated_norm_bwd_kernel<T, L, PER, ACC, true>), dim3(p.blocks), dim3(threads), 4 * lds, s, g);
   } else if (back) {
-    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, L, PER, LAYER, ACC, false>), 3 * lds);
-    PT_LAUNCH((gated_norm_bwd_kernel<T, L, PER, LAYER, ACC, false>), dim3(p.blocks), dim3(threads), 3 * lds, s, g);
-  } else PT_LAUNCH((gated_norm_fwd_kernel<T, L, PER, LAYER, ACC>), dim3(p.blocks), dim3(threads), 0, s, g);
+    if (lds) PT_ENSURE_LDS((gated_norm_bwd_kernel<T, L, PER, ACC, false>), 3 * lds);
+    PT_LAUNCH((gated_norm_bwd_kernel<T, L, PER, ACC, false>), dim3(p.blocks), dim3(threads), 3 * lds, s, g);
+  } else if (g.layer) PT_LAUNCH((gated_norm_fwd_kernel<T, L, PER, true, ACC>), dim3(p.blocks), dim3(threads), 0, s, g);
+  else PT_LAUNCH((gated_norm_fwd_kernel<T, L, PER, false, ACC>), dim3(p.blocks), dim3(threads), 0, s, g);
   return 0;
 }
-template <typename T, int L, int PER, bool LAYER>
-static int run_gated(const GatedArgs& g, const GatedPlan& p, Access acc, int back, hipStream_t s) {
-  if (acc == ALIGNED) return run_gated<T, L, PER, LAYER, ALIGNED>(g, p, back, s);
-  if constexpr (L == 8)
-    if (acc == SCALAR) return run_gated<T, L, PER, LAYER, SCALAR>(g, p, back, s);
-  return run_gated<T, L, PER, LAYER, ANY>(g, p, back, s);
-}
 template <typename T, int L, int PER>
-static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, Access acc, int back, hipStream_t s) {
-  return layer ? run_gated<T, L, PER, true>(g, p, acc, back, s) : run_gated<T, L, PER, false>(g, p, acc, back, s);
+static int run_gated(const GatedArgs& g, const GatedPlan& p, Access acc, int back, hipStream_t s) {
+  if (acc == ALIGNED) return run_gated<T, L, PER, ALIGNED>(g, p, back, s);
+  if constexpr (L == 8)
+    if (acc == SCALAR) return run_gated<T, L, PER, SCALAR>(g, p, back, s);
+  return run_gated<T, L, PER, ANY>(g, p, back, s);
 }
 template <typename T>
-static int run_gated(const GatedArgs& g, const GatedPlan& p, bool layer, Access acc, int back, hipStream_t s) {
+static int run_gated(const GatedArgs& g, const GatedPlan& p, Access acc, int back, hipStream_t s) {
   switch (p.lanes) {
-    case 8: return run_gated<T, 8, 8>(g, p, layer, acc, back, s);
-    case 16: return run_gated<T, 16, 8>(g, p, layer, acc, back, s);
-    case 32: return run_gated<T, 32, 8>(g, p, layer, acc, back, s);
-    case 64: return run_gated<T, 64, 8>(g, p, layer, acc, back, s);
-    case 128: return run_gated<T, 128, 8>(g, p, layer, acc, back, s);
-    case 256: return run_gated<T, 256, 8>(g, p, layer, acc, back, s);
-    default: return p.per == 8 ? run_gated<T, 512, 8>(g, p, layer, acc, back, s) : run_gated<T, 512, 16>(g, p, layer, acc, back, s);
+    case 8: return run_gated<T, 8, 8>(g, p, acc, back, s);
+    case 16: return run_gated<T, 16, 8>(g, p, acc, back, s);
+    case 32: return run_gated<T, 32, 8>(g, p, acc, back, s);
+    case 64: return run_gated<T, 64, 8>(g, p, acc, back, s);
+    case 128: return run_gated<T, 128, 8>(g, p, acc, back, s);
+    case 256: return run_gated<T, 256, 8>(g, p, acc, back, s);
+    default: return p.per == 8 ? run_gated<T, 512, 8>(g, p, acc, back, s) : run_gated<T, 512, 16>(g, p, acc, back, s);
   }
 }
 
@@ -665,9 +663,10 @@ int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   g.ldx = (size_t)ldx; g.ldt = (size_t)ldt; g.rows = (int)rows; g.cols = cols; g.clip = gate ? clip : (int)rows; g.eps = eps;
   const GatedPlan p = gated_plan(g.rows, cols, g.clip, gate != nullptr, FWD_WAVES);
   g.run = p.run; g.spc = p.spc;
+  g.layer = kind == 0;
   g.stream = gated_stream(g, dtype);
   const Access acc = gated_access(g, dtype);
-  return dtype ? run_gated<unsigned short>(g, p, kind == 0, acc, 0, s) : run_gated<float>(g, p, kind == 0, acc, 0, s);
+  return dtype ? run_gated<unsigned short>(g, p, acc, 0, s) : run_gated<float>(g, p, acc, 0, s);
 }
 
 int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1,
@@ -687,10 +686,11 @@ int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   g.part = (float*)ws;
   g.gpart = p.spc && dgate ? g.part + (size_t)p.blocks * 4 * cols : nullptr;
   g.joined = p.joined && dgate;
+  g.layer = kind == 0;
   g.stream = gated_stream(g, dtype);
   const Access acc = gated_access(g, dtype);
   const int bias = b1 || db1 || db2 ? 1 : 0;
-  if (dtype ? run_gated<unsigned short>(g, p, kind == 0, acc, 1 + bias, s) : run_gated<float>(g, p, kind == 0, acc, 1 + bias, s)) return 1;
+  if (dtype ? run_gated<unsigned short>(g, p, acc, 1 + bias, s) : run_gated<float>(g, p, acc, 1 + bias, s)) return 1;
   GatedFinish f = {};
   f.part = g.part; f.gpart = g.gpart; f.a = a; f.w1 = w1; f.b1 = b1;
   f.da = t ? da : nullptr; f.dw1 = t ? dw1 : nullptr; f.db1 = t ? db1 : nullptr; f.dw2 = dw2; f.db2 = db2;
