@@ -75,6 +75,7 @@ struct WinArgs {
   const int* lengths;
   int B, Nq, Nk, H, Hk, D, left, right, sinks;
   float sc, scale;                                       // scale * log2(e), scale
+  int tiny;                                              // keys of one tile: see few_keys
   int far, far_chunks, far_rows;                         // first row index that sees the first keys only as sinks, its chunks, rows of one
 };
 
@@ -346,7 +347,8 @@ __device__ __forceinline__ void key_tiles(const WinArgs& a, int len, int t0, int
 // Whether rows at positions [t0, t1] see so few keys (512 each, 640 together) that in bf16 the rounding of their probabilities does not
 // average out: dQ and dK feel it, and that of o, through delta.  There the probabilities enter o's product as sums of two bf16 values, and
 // o keeps a byte more for delta: error of dQ and dK for 3 / 129 visible keys 2.2 / 1.53 -> 1.42 times that of rounding the exact
-// result (what is left is dS in bf16).  8192 rows, 16 heads over 4, D = 128: a window of 256 keys forward 43 -> 53 us, with gradients 183 -> 205;
+// result (what is left is dS in bf16, whose rounding averages out over the rows; sequences of at most 32 keys, where it would not, hold dS and
+// the probabilities of dV in two values too).  8192 rows, 16 heads over 4, D = 128: a window of 256 keys forward 43 -> 53 us, with gradients 183 -> 205;
 // 1024 keys, where only the first rows see few, 86 -> 87 and 375 -> 377
 __device__ __forceinline__ bool few_keys(const WinArgs& a, int len, int t0, int t1) {
   const int hi = min(t1 + a.right, len - 1), lo = max(t0 - a.left, 0);
@@ -654,10 +656,10 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -lse)) * (dp[x][r] - delta);
-      add_product<T, DP>(dq, kf[0], st[0]);                              // dS to bf16: 2^-9 of each
+      add_product<T, DP>(dq, kf[0], st[0], BF && a.tiny);                // dS to bf16: 2^-9 of each
       if constexpr (NB > 1) {
         if constexpr (!BF) kc.template read<32 * tile::RB>(kf[NB - 1]);
-        add_product<T, DP>(dq, kf[NB - 1], st[NB - 1]);
+        add_product<T, DP>(dq, kf[NB - 1], st[NB - 1], BF && a.tiny);
       }
     }
     dma_wait();
@@ -700,7 +702,7 @@ struct KvPlan {
   static constexpr int LDS = VB + BUF * ONE > JOIN ? VB + BUF * ONE : JOIN;
   static_assert(LDS <= 160 * 1024 && BUF * ONE <= 128 * 1024, "LDS, and what LDS-DMA reaches of it");
 };
-template <typename T, int DP, bool SINK>
+template <typename T, int DP, bool SINK, bool TINY>
 __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bwd_kv_kernel(const WinArgs a) {
   typedef KvPlan<T, DP, SINK> plan;
   constexpr bool BF = sizeof(T) == 2;
@@ -826,9 +828,9 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
         add_product<T, DP>(dv, f, st);
         add_product<T, DP>(dk, f2, dp);
       } else {
-        add_product<T, DP>(dv, f, st);
+        add_product<T, DP>(dv, f, st, TINY);
         Cols<T, DP>(Qs, cb).template read<0>(f);
-        add_product<T, DP>(dk, f, dp);
+        add_product<T, DP>(dk, f, dp, TINY);
       }
     }
     if constexpr (SINK) __syncthreads();
@@ -1250,6 +1252,7 @@ static WinArgs win_args(const void* q, const void* k, const void* v, const int64
   a.right = right < 0 || right > WIN_FAR ? WIN_FAR : right;
   a.sinks = std::min(sinks, Nk);
   a.scale = scale; a.sc = scale * LOG2E;
+  a.tiny = Nk <= 32;
   // rows behind the window of the first 128 keys, which see the sinks among those as sinks only
   const int64_t far = std::max<int64_t>((int64_t)128 + a.left - (Nk - Nq), 0);
   if (a.sinks > 0 && far < Nq) {
@@ -1281,12 +1284,19 @@ static int run_win_bwd(const WinArgs& a, hipStream_t s) {
   typedef RowPlan<T, DP> plan;
   constexpr int lds = plan::SETS * 4 * key_tile_q<T, DP>() * Tile<T, DP>::RB, lds_kv = KvPlan<T, DP, false>::LDS, lds_sink = KvPlan<T, DP, true>::LDS;
   PT_ENSURE_LDS((win_bwd_q_kernel<T, DP>), lds);
-  PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false>), lds_kv);
   PT_LAUNCH((win_bwd_q_kernel<T, DP>), dim3((unsigned)win_blocks(a, plan::ROWS)), dim3(plan::TH), lds, s, a);
-  PT_LAUNCH((win_bwd_kv_kernel<T, DP, false>), dim3((unsigned)((a.Nk + KvPlan<T, DP, false>::KEYS - 1) / KvPlan<T, DP, false>::KEYS) * a.Hk * a.B), dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
+  const dim3 keys((unsigned)((a.Nk + KvPlan<T, DP, false>::KEYS - 1) / KvPlan<T, DP, false>::KEYS) * a.Hk * a.B);
+  constexpr bool BF = sizeof(T) == 2;
+  if (BF && a.tiny) {                                    // a kernel of its own: the wide products cost the other one its registers (413 -> 462 us)
+    PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false, BF>), lds_kv);
+    PT_LAUNCH((win_bwd_kv_kernel<T, DP, false, BF>), keys, dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
+  } else {
+    PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false, false>), lds_kv);
+    PT_LAUNCH((win_bwd_kv_kernel<T, DP, false, false>), keys, dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
+  }
   if (a.far_chunks) {
-    PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, true>), lds_sink);
-    PT_LAUNCH((win_bwd_kv_kernel<T, DP, true>), dim3((unsigned)((a.sinks + 31) / 32 * a.far_chunks) * a.H * a.B), dim3(KvPlan<T, DP, true>::TH), lds_sink, s, a);
+    PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, true, false>), lds_sink);
+    PT_LAUNCH((win_bwd_kv_kernel<T, DP, true, false>), dim3((unsigned)((a.sinks + 31) / 32 * a.far_chunks) * a.H * a.B), dim3(KvPlan<T, DP, true>::TH), lds_sink, s, a);
     const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sinks * a.D;
     PT_LAUNCH(win_bwd_join_kernel<T>, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, a, 1 + a.far_chunks * (a.H / a.Hk));
   }

@@ -148,6 +148,19 @@ def test_gradients_of_few_keys_do_not_feel_the_rounding_of_the_output(left):
         assert float(err) <= 1.1 * e * float(square.sum() + want.square().sum()), (n, float(err / (e * (square.sum() + want.square().sum()))))
 
 
+@pytest.mark.parametrize("D", [32, 128])
+def test_gradients_of_short_sequences_are_rounded_once(D):
+    """bf16, at most 32 keys: the factors of the second products are held in 16 bits, so that only the results' rounding is left; its mean
+    square is at most (2^-8)^2 / 3 of the value's, and what comes before is 2^-8 of it."""
+    case = (5, 29, 29, 4, 2, D, 6, 0, 2, None)
+    q, k, v, do, _ = make(case, torch.bfloat16)
+    want = oracle(q, k, v, do, *case[6:9], None)[0]
+    got = grads(q, k, v, do, case, None)
+    for n in "oqkv":
+        err, size = (got[n].double() - want[n]).square().sum(), want[n].square().sum()
+        assert float(err) <= 1.02 * (2.0 ** -8) ** 2 / 3 * float(size), (n, float(err / size) ** 0.5)
+
+
 def test_gradients_against_differences():
     case = CASES["a new part of a sequence"]
     q, k, v, do, _ = make(case, torch.float32)
