@@ -924,7 +924,7 @@ __global__ __launch_bounds__(256) void win_bwd_join_kernel(const WinArgs a, int 
 // keys side by side, each with its own running maximum and sum, joined at the end.  fp32, and few short sequences of either type.
 // win_step_group_kernel: bf16 on the matrix cores.
 // Read rates over all visible keys and values: 64 sequences of some 3100 keys, 64 heads over 8, D = 128: 140 us, 6.0 TB/s (vector unit: 303);
-// 32 heads over 8: 157 us for 986 MB, 6.3 TB/s (183); 8 over 8, D = 64, 393 MB: 75 us; one sequence of 18,000 keys, 74 MB: 18 us;
+// 32 heads over 8: 159 us for 986 MB, 6.2 TB/s (183); 8 over 8, D = 64, 393 MB: 75 us; one sequence of 18,000 keys, 74 MB: 18 us;
 // fp32, 214 MB: 40 us
 // ---------------------------------------------------------------------------
 struct StepArgs {
@@ -1060,8 +1060,8 @@ __global__ __launch_bounds__(W * 64) void win_step_kernel(const StepArgs a) {
 // The same in bf16: up to 32 heads of a group are the columns of a 32 x 32 tile, 32 keys its rows, as in the forward kernel.  Columns
 // without a head cost matrix time that the loads leave over: with one head in use it is as fast as the vector unit, with eight, where
 // the vector unit is the bound, more than twice.  Every wave walks tiles of its own through LDS-DMA into two buffers, without
-// barriers; probabilities are rounded to bf16 for the second product (an output in bf16 is rounded as much), their sum is of the
-// unrounded ones.
+// barriers.  Probabilities enter the second product as sums of two bf16 values: the matrix cores have the time (64 sequences, 986 MB: 156.9 us
+// with one, 159.1 with two), and the result is rounded once.
 constexpr int STEP_WAVES = 4;
 template <int DP, bool STREAM>
 __global__ __launch_bounds__(STEP_WAVES * 64) void win_step_group_kernel(const StepArgs a) {
@@ -1127,7 +1127,7 @@ __global__ __launch_bounds__(STEP_WAVES * 64) void win_step_group_kernel(const S
     }
     bf16x8 f[2][ND];
     Cols<T, DP>(now + TB, vb).template read<0>(f);
-    add_product<T, DP>(acc, f, st);
+    add_product<T, DP>(acc, f, st, true);
   }
   l += half_other(l);
   // join the waves
