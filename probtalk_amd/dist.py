@@ -99,10 +99,6 @@ class OutputGatherer:
         return self.bufs[(self.i - 1) % 2]
 
 
-# tools/micro/dist_train_debug.py sets this to hand gloo the device tensors themselves (the configuration that hung)
-GLOO_DEVICE_TENSORS = False
-
-
 class GradientReducer:
     """Data-parallel training: averages the gradients of `params` over all ranks in flat buckets.
 
@@ -160,7 +156,7 @@ class GradientReducer:
         # rank (profiles/r2/gloo_device_tensor_hang.txt; three 64 K-float all_reduce launched the same way complete,
         # profiles/r2/gloo_cuda_probe_small.txt).  RCCL reduces the device buffer in place; a stuck collective there ends
         # the job through init_process_group's timeout (bench.py)
-        msg = flat.cpu() if flat.is_cuda and dist.get_backend() == "gloo" and not GLOO_DEVICE_TENSORS else flat
+        msg = flat.cpu() if flat.is_cuda and dist.get_backend() == "gloo" else flat
         self._pending[i] = (dist.all_reduce(msg, op=dist.ReduceOp.SUM, async_op=True), flat, live, msg)
 
     def _on_grad(self, p):
