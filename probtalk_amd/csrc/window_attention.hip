@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "pt_common.h"
 
@@ -69,13 +70,12 @@ struct WinArgs {
   void* o; float* lse;                                   // lse [B][H][Nq], in powers of two; +inf for a row that sees nothing
   const void* od; const void* dod;                       // backward: o and its gradient, (B, Nq, H, D)
   void* dq; void* dk; void* dv; float* delta;            // delta [B][H][Nq]
-  signed char* rest;                                     // bf16: what o lost when it was rounded, a byte a value, where few_keys says so; or null
+  signed char* rest;                                     // bf16: what o lost when it was rounded, a byte a value; or null
   float* part;                                           // shares of the first keys' gradients (see win_bwd_sink_kernel)
   int64_t sq[3], sk[3], sv[3];                           // strides of batch, row, head in values
   const int* lengths;
   int B, Nq, Nk, H, Hk, D, left, right, sinks;
   float sc, scale;                                       // scale * log2(e), scale
-  int tiny;                                              // keys of one tile: see few_keys
   int far, far_chunks, far_rows;                         // first row index that sees the first keys only as sinks, its chunks, rows of one
 };
 
@@ -136,10 +136,34 @@ struct Cols<__bf16, DP> {
       y[db] = x[db] ^ (tile::swz(8) << 4);
     }
   }
+  // columns 64 HALF .. 64 HALF + 63
+  template <int OFF, int HALF>
+  __device__ __forceinline__ void read_half(bf16x8 (&f)[2][2]) const {
+    s16x4 r[4][2];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %1, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %8 offset:%14\n\tds_read_b64_tr_b16 %6, %10 offset:%15\n\t"
+        "ds_read_b64_tr_b16 %5, %9 offset:%14\n\tds_read_b64_tr_b16 %7, %11 offset:%15\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[3][0]), "=&v"(r[3][1])
+        : "v"(x[2 * HALF]), "v"(x[2 * HALF + 1]), "v"(y[2 * HALF]), "v"(y[2 * HALF + 1]), "i"(OFF), "i"(OFF + 8 * RB), "i"(OFF + 16 * RB), "i"(OFF + 24 * RB));
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        const s16x4 p = r[2 * s2][db], q = r[2 * s2 + 1][db];
+        const s16x8 v = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
+        f[s2][db] = __builtin_bit_cast(bf16x8, v);
+      }
+  }
   template <int OFF>
   __device__ __forceinline__ void read(bf16x8 (&f)[2][ND]) const {
-    s16x4 r[4][ND];
-    if constexpr (ND == 4) {
+    if constexpr (ND == 2) {
+      read_half<OFF, 0>(f);
+    } else {
+      static_assert(ND == 4, "64 or 128 columns");
+      s16x4 r[4][ND];
       asm volatile(
           "ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %4, %20 offset:%25\n\t"
           "ds_read_b64_tr_b16 %1, %17 offset:%24\n\tds_read_b64_tr_b16 %5, %21 offset:%25\n\t"
@@ -154,25 +178,15 @@ struct Cols<__bf16, DP> {
             "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[2][2]), "=&v"(r[2][3]), "=&v"(r[3][0]), "=&v"(r[3][1]), "=&v"(r[3][2]), "=&v"(r[3][3])
           : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]), "i"(OFF), "i"(OFF + 8 * RB), "i"(OFF + 16 * RB),
             "i"(OFF + 24 * RB));
-    } else {
-      static_assert(ND == 2, "64 or 128 columns");
-      asm volatile(
-          "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %10 offset:%13\n\t"
-          "ds_read_b64_tr_b16 %1, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%13\n\t"
-          "ds_read_b64_tr_b16 %4, %8 offset:%14\n\tds_read_b64_tr_b16 %6, %10 offset:%15\n\t"
-          "ds_read_b64_tr_b16 %5, %9 offset:%14\n\tds_read_b64_tr_b16 %7, %11 offset:%15\n\t"
-          "s_waitcnt lgkmcnt(0)"
-          : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[3][0]), "=&v"(r[3][1])
-          : "v"(x[0]), "v"(x[1]), "v"(y[0]), "v"(y[1]), "i"(OFF), "i"(OFF + 8 * RB), "i"(OFF + 16 * RB), "i"(OFF + 24 * RB));
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int db = 0; db < ND; ++db) {
+          const s16x4 p = r[2 * s2][db], q = r[2 * s2 + 1][db];
+          const s16x8 v = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
+          f[s2][db] = __builtin_bit_cast(bf16x8, v);
+        }
     }
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-      for (int db = 0; db < ND; ++db) {
-        const s16x4 p = r[2 * s2][db], q = r[2 * s2 + 1][db];
-        const s16x8 v = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
-        f[s2][db] = __builtin_bit_cast(bf16x8, v);
-      }
   }
 };
 template <int DP>
@@ -195,26 +209,51 @@ struct Cols<float, DP> {
         }
   }
 };
-// acc[db] += (columns of 32 rows)^T . p, p the registers of a score tile over these rows.  wide (bf16): p as the sum of two bf16 values
+// The registers of a score tile as the second operand of a product.  bf16: as the sum of two bf16 values, 2^-17 off.  One alone is 2^-8 off, and so is
+// the result, however many keys share a row's weight: 1.44 times the error of rounding the exact result, and more where few rows add up.
+// 8192 rows, 1028 keys, 16 heads over 4, D = 128, one value and two: forward 113 and 137 us, dQ 166 and 191, dK / dV 183 and 233
+template <typename T>
+__device__ __forceinline__ void split(const f32x16& p, int s2, typename Types<T>::frag& hi, typename Types<T>::frag& lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) hi[e] = (T)p[8 * s2 + e];
+  if constexpr (sizeof(T) == 2)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[e] = (T)(p[8 * s2 + e] - (float)hi[e]);
+}
+// acc[db] += (columns of 32 rows)^T . p, p the registers of a score tile over these rows
 template <typename T, int DP>
-__device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const typename Types<T>::frag (&f)[2][DP / 32], const f32x16& p, bool wide = false) {
+__device__ __forceinline__ void add_product(f32x16 (&acc)[DP / 32], const typename Types<T>::frag (&f)[2][DP / 32], const f32x16& p) {
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
-    typename Types<T>::frag x;
+    typename Types<T>::frag hi, lo;
+    split<T>(p, s2, hi, lo);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (T)p[8 * s2 + e];
+    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], hi, acc[db]);
+    if constexpr (sizeof(T) == 2)
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], x, acc[db]);
+      for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], lo, acc[db]);
   }
-  if (sizeof(T) == 2 && wide)
+}
+// The same with the columns read 64 at a time, for a kernel that has no registers for all of them (dK / dV at D = 128: a tenth less)
+template <int DP>
+__device__ __forceinline__ void add_columns(f32x16 (&acc)[DP / 32], const Cols<__bf16, DP>& c, const f32x16& p) {
+  bf16x8 hi[2], lo[2];
+#pragma unroll
+  for (int s2 = 0; s2 < 2; ++s2) split<__bf16>(p, s2, hi[s2], lo[s2]);
+  auto half = [&](auto h) {
+    constexpr int H = decltype(h)::value;
+    bf16x8 f[2][2];
+    c.template read_half<0, H>(f);
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
-      typename Types<T>::frag x;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (T)(p[8 * s2 + e] - (float)(T)p[8 * s2 + e]);
+      for (int d = 0; d < 2; ++d) acc[2 * H + d] = mma(f[s2][d], hi[s2], acc[2 * H + d]);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) acc[db] = mma(f[s2][db], x, acc[db]);
+      for (int d = 0; d < 2; ++d) acc[2 * H + d] = mma(f[s2][d], lo[s2], acc[2 * H + d]);
     }
+  };
+  half(std::integral_constant<int, 0>{});
+  if constexpr (DP > 64) half(std::integral_constant<int, 1>{});
 }
 // What a value lost when it was rounded to bf16, in steps of its 24-bit pattern (-128 to 128, of which 128 is taken for 127), and the value
 // that both stand for, off by a step and a half of 2^-15 at most
@@ -238,8 +277,8 @@ struct Dma {
   int row, col[2];                                       // row and first byte of this lane in the first turn (and in odd turns of 8 rows)
   unsigned off[2];
   int64_t stride;                                        // bytes of a row
-  __device__ __forceinline__ Dma(int D, int64_t stride_) : stride(stride_ * (int64_t)sizeof(T)) {
-    const int byte = threadIdx.x % TH * 16;
+  __device__ __forceinline__ Dma(int D, int64_t stride_, int thread = threadIdx.x) : stride(stride_ * (int64_t)sizeof(T)) {
+    const int byte = thread % TH * 16;
     row = byte / RB;
     const int chunk = (byte % RB / 16) ^ tile::swz(row), odd = chunk ^ tile::swz(ROWS);
     col[0] = chunk * tile::EPC < D ? chunk * 16 : 0;
@@ -344,16 +383,6 @@ __device__ __forceinline__ void key_tiles(const WinArgs& a, int len, int t0, int
   from = max(lo / KT, first);
   to = hi < lo ? from : max(hi / KT + 1, from);
 }
-// Whether rows at positions [t0, t1] see so few keys (512 each, 640 together) that in bf16 the rounding of their probabilities does not
-// average out: dQ and dK feel it, and that of o, through delta.  There the probabilities enter o's product as sums of two bf16 values, and
-// o keeps a byte more for delta: error of dQ and dK for 3 / 129 visible keys 2.2 / 1.53 -> 1.42 times that of rounding the exact
-// result (what is left is dS in bf16, whose rounding averages out over the rows; sequences of at most 32 keys, where it would not, hold dS and
-// the probabilities of dV in two values too).  8192 rows, 16 heads over 4, D = 128: a window of 256 keys forward 43 -> 53 us, with gradients 183 -> 205;
-// 1024 keys, where only the first rows see few, 86 -> 87 and 375 -> 377
-__device__ __forceinline__ bool few_keys(const WinArgs& a, int len, int t0, int t1) {
-  const int hi = min(t1 + a.right, len - 1), lo = max(t0 - a.left, 0);
-  return hi - lo + 1 + min(a.sinks, lo) <= 640;
-}
 // Scores of invisible pairs to -infinity: keys along the registers of a transposed tile (KEYS) or along the lanes
 template <bool KEYS>
 __device__ __forceinline__ void mask_tile(const WinArgs& a, int len, int t, int key, int h, f32x16& st, int last = 0x7FFFFFFF) {
@@ -418,9 +447,9 @@ struct RowPlan {                                         // WAVES: per SIMD
 };
 
 // ---------------------------------------------------------------------------
-// Forward: waves of 32 rows each over common key tiles (RowPlan).  bf16, 8192 rows that see 1028 keys, 16 heads over 4, D = 128: 105 us,
-// 615 TFLOP/s of visible pairs; its products alone take 66 us, the rate of a large matrix product on this card, the rest is softmax, the window's
-// edges and loads that they do not cover.  fp32: see RowPlan
+// Forward: waves of 32 rows each over common key tiles (RowPlan).  bf16, 8192 rows that see 1028 keys, 16 heads over 4, D = 128: 137 us,
+// 470 TFLOP/s of visible pairs; its products (three for the formula's two) alone would take 99 us at the rate of a large matrix product on this card, the
+// rest is softmax, the window's edges and loads that they do not cover.  fp32: see RowPlan
 // ---------------------------------------------------------------------------
 template <typename T, int DP>
 __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void win_fwd_kernel(const WinArgs a) {
@@ -443,7 +472,6 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
   int first, from, to;
   key_tiles<KT>(a, len, i00 + shift, min(i00 + ROWS - 1, a.Nq - 1) + shift, first, from, to);
   const int tiles = first + (to - from);
-  const bool wide = BF && few_keys(a, len, i00 + shift, min(i00 + ROWS - 1, a.Nq - 1) + shift);
   auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
   const Dma<T, DP, KT, plan::TS> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
   if (set < tiles) {
@@ -521,8 +549,8 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
         vc.template read<32 * tile::RB>(vf[1]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      add_product<T, DP>(o, vf[0], st[0], wide);                         // probabilities in [0, 1] to bf16: 2^-9 of each; wide: 2^-17
-      if constexpr (NB > 1) add_product<T, DP>(o, vf[1], st[1], wide);
+      add_product<T, DP>(o, vf[0], st[0]);
+      if constexpr (NB > 1) add_product<T, DP>(o, vf[1], st[1]);
     }
     dma_wait();
   }
@@ -550,12 +578,12 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
   if (row >= a.Nq) return;
   l += half_other(l);
   const int64_t out = (((int64_t)b * a.Nq + row) * a.H + head) * a.D;
-  store_transposed<T, DP>((T*)a.o + out, o, h, a.D, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), wide && a.rest ? a.rest + out : nullptr);
+  store_transposed<T, DP>((T*)a.o + out, o, h, a.D, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), a.rest ? a.rest + out : nullptr);
   if (a.lse && h == 0) a.lse[((int64_t)b * a.H + head) * a.Nq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // ---------------------------------------------------------------------------
-// Backward, dQ (and delta): rows and key tiles as forward.  The case above: 145 us for three products (668 TFLOP/s of visible pairs)
+// Backward, dQ (and delta): rows and key tiles as forward.  The case above: 191 us for four products of the formula's three (507 TFLOP/s of visible pairs)
 // ---------------------------------------------------------------------------
 template <typename T, int DP> constexpr int key_tile_q() { return sizeof(T) * DP <= 128 ? 64 : 32; }   // 256 registers hold no more
 template <typename T, int DP>
@@ -580,7 +608,6 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
   int first, from, to;
   key_tiles<KT>(a, len, i00 + shift, min(i00 + ROWS - 1, a.Nq - 1) + shift, first, from, to);
   const int tiles = first + (to - from);
-  const bool wide = BF && few_keys(a, len, i00 + shift, min(i00 + ROWS - 1, a.Nq - 1) + shift);
   auto key_of = [&](int n) { return (n < first ? n : from + n - first) * KT; };
   const Dma<T, DP, KT, plan::TS> dma_k(a.D, a.sk[1]), dma_v(a.D, a.sv[1]);
   if (set < tiles) {
@@ -595,7 +622,7 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
     gf[s] = global_frag((const T*)a.dod + ob, so, row, a.Nq, 16 * s + 8 * h, a.D);
     const auto of = global_frag((const T*)a.od + ob, so, row, a.Nq, 16 * s + 8 * h, a.D);
     if constexpr (BF)
-      if (wide && row < a.Nq && 16 * s + 8 * h < a.D) {
+      if (row < a.Nq && 16 * s + 8 * h < a.D) {
         const uint2 w = *reinterpret_cast<const uint2*>(a.rest + ob + row * so + 16 * s + 8 * h);
 #pragma unroll
         for (int e = 0; e < 8; ++e) delta += (float)gf[s][e] * with_rest(of[e], (signed char)((e < 4 ? w.x : w.y) >> 8 * (e & 3)));
@@ -656,10 +683,10 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           st[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][r], a.sc, -lse)) * (dp[x][r] - delta);
-      add_product<T, DP>(dq, kf[0], st[0], BF && a.tiny);                // dS to bf16: 2^-9 of each
+      add_product<T, DP>(dq, kf[0], st[0]);
       if constexpr (NB > 1) {
         if constexpr (!BF) kc.template read<32 * tile::RB>(kf[NB - 1]);
-        add_product<T, DP>(dq, kf[NB - 1], st[NB - 1], BF && a.tiny);
+        add_product<T, DP>(dq, kf[NB - 1], st[NB - 1]);
       }
     }
     dma_wait();
@@ -680,7 +707,7 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
 // on the tile's first 32 rows and one on the others, added up at the end (there are too few blocks of keys to fill the chip with
 // 4 waves each).  The keys stay in registers as operands; in bf16, rows of more than 128 bytes leave no room for the values beside them (two
 // waves a SIMD have 256 registers each, half of them hold the results), so these are read from LDS, where they stay too.
-// The case above: 170 us for four products (760 TFLOP/s of visible pairs).  fp32 with D up to 64: 2 blocks of keys, values in registers, two
+// The case above: 233 us for six products of the formula's four (554 TFLOP/s of visible pairs).  fp32 with D up to 64: 2 blocks of keys, values in registers, two
 // workgroups on a CU (105 -> 57 us where the row kernels gain as RowPlan says).
 // SINK: the rows far behind the window, which see the first 32-key blocks as sinks only.  There are as many of these rows as the
 // sequence is long and only a few keys, so the waves take the SAME keys and 32 rows of a tile each, the rows are cut into
@@ -702,7 +729,7 @@ struct KvPlan {
   static constexpr int LDS = VB + BUF * ONE > JOIN ? VB + BUF * ONE : JOIN;
   static_assert(LDS <= 160 * 1024 && BUF * ONE <= 128 * 1024, "LDS, and what LDS-DMA reaches of it");
 };
-template <typename T, int DP, bool SINK, bool TINY>
+template <typename T, int DP, bool SINK>
 __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 256 ? 1 : 2) void win_bwd_kv_kernel(const WinArgs a) {
   typedef KvPlan<T, DP, SINK> plan;
   constexpr bool BF = sizeof(T) == 2;
@@ -746,16 +773,18 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
   }
   const int per = r1 > r0 ? (r1 - r0 + QT - 1) / QT : 0, total = SINK ? per : per * group;
   const int64_t so = (int64_t)a.H * a.D;
-  const Dma<T, DP, QT, TH> dma_q(a.D, a.sq[1]), dma_g(a.D, so);
   int fh = SINK ? item : kvh * group, fr = r0;                           // head and first row of the next tile
   auto fetch = [&](unsigned char* m) {
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));                                     // made anew for every tile, these offsets take no registers in between
+    const Dma<T, DP, QT, TH> dma_q(a.D, a.sq[1], thread), dma_g(a.D, so, thread);
     dma_q((const T*)a.q + b * a.sq[0] + fh * a.sq[2], fr, a.Nq, m);
     dma_g((const T*)a.dod + ((int64_t)b * a.Nq * a.H + fh) * a.D, fr, a.Nq, m + TB);
     // lse by the first wave(s), delta by the next; rows behind the last one are masked
     if (wave < 2 * LB / 256) {
       const int part = wave % (LB / 256);
       const float* from = (wave < LB / 256 ? a.lse : a.delta) + ((int64_t)b * a.H + fh) * a.Nq;
-      __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + min(fr + part * 64 + lane, a.Nq - 1)), (lds_ptr_t)(m + 2 * TB + wave * 256), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_ptr_t)(from + min(fr + part * 64 + (thread & 63), a.Nq - 1)), (lds_ptr_t)(m + 2 * TB + wave * 256), 4, 0, 0);
     }
     fr += QT;
     if (fr >= r1) { fr = r0; ++fh; }
@@ -798,18 +827,22 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
     if (!SINK && n + 1 < total) fetch(bufs + ((n + 1) & 1) * ONE);
     if (sub < QT && k0 <= t1 + a.right && (k0 + 31 >= t0 - a.left || k0 < a.sinks) && k0 < len) {
       const bool all = k0 + 31 <= t0 + a.right && k0 + 31 < len && (k0 >= t1 - a.left || k0 + 31 < a.sinks) && t1 - shift < r1;
+      int rl = rb, cl = cb;                                              // made here, the addresses of a block's operands do not take the registers of all blocks
+      asm volatile("" : "+v"(rl), "+v"(cl));
       f32x16 st = zero16(), dp = zero16();
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
-        st = mma(tile::row_frag(Qs, rb, s), kf[s], st);
-        if constexpr (plan::V_LDS) dp = mma(tile::row_frag(Gs, rb, s), tile::row_frag(Vw, rb, s), dp);
-        else dp = mma(tile::row_frag(Gs, rb, s), vf[s], dp);
+        st = mma(tile::row_frag(Qs, rl, s), kf[s], st);
+        if constexpr (plan::V_LDS) dp = mma(tile::row_frag(Gs, rl, s), tile::row_frag(Vw, rl, s), dp);
+        else dp = mma(tile::row_frag(Gs, rl, s), vf[s], dp);
       }
       constexpr int READS = plan::V_LDS ? 3 : 2;                         // for two products
       if constexpr (BF) reads_ahead<2 * READS, READS, 2, DP / 8>(); else reads_ahead<2 * READS, READS * 2, 16, DP>();
       typename Types<T>::frag f[2][DP / 32];
-      Cols<T, DP>(Gs, cb).template read<0>(f);
-      if constexpr (!BF) __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!BF) {
+        Cols<T, DP>(Gs, cl).template read<0>(f);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if (!all) mask_tile<false>(a, len, t0, key, h, st, r1 - 1 + shift);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -821,16 +854,19 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
           dp[r] = st[r] * (dp[r] - D4[e]);
         }
       }
-      if constexpr (!BF && plan::V_LDS) {
+      if constexpr (BF) {
+        add_columns<DP>(dv, Cols<T, DP>(Gs, cl), st);
+        add_columns<DP>(dk, Cols<T, DP>(Qs, cl), dp);
+      } else if constexpr (plan::V_LDS) {
         typename Types<T>::frag f2[2][DP / 32];
-        Cols<T, DP>(Qs, cb).template read<0>(f2);
+        Cols<T, DP>(Qs, cl).template read<0>(f2);
         __builtin_amdgcn_sched_barrier(0);
         add_product<T, DP>(dv, f, st);
         add_product<T, DP>(dk, f2, dp);
       } else {
-        add_product<T, DP>(dv, f, st, TINY);
-        Cols<T, DP>(Qs, cb).template read<0>(f);
-        add_product<T, DP>(dk, f, dp, TINY);
+        add_product<T, DP>(dv, f, st);
+        Cols<T, DP>(Qs, cl).template read<0>(f);
+        add_product<T, DP>(dk, f, dp);
       }
     }
     if constexpr (SINK) __syncthreads();
@@ -1127,7 +1163,7 @@ __global__ __launch_bounds__(STEP_WAVES * 64) void win_step_group_kernel(const S
     }
     bf16x8 f[2][ND];
     Cols<T, DP>(now + TB, vb).template read<0>(f);
-    add_product<T, DP>(acc, f, st, true);
+    add_product<T, DP>(acc, f, st);
   }
   l += half_other(l);
   // join the waves
@@ -1252,7 +1288,6 @@ static WinArgs win_args(const void* q, const void* k, const void* v, const int64
   a.right = right < 0 || right > WIN_FAR ? WIN_FAR : right;
   a.sinks = std::min(sinks, Nk);
   a.scale = scale; a.sc = scale * LOG2E;
-  a.tiny = Nk <= 32;
   // rows behind the window of the first 128 keys, which see the sinks among those as sinks only
   const int64_t far = std::max<int64_t>((int64_t)128 + a.left - (Nk - Nq), 0);
   if (a.sinks > 0 && far < Nq) {
@@ -1286,17 +1321,11 @@ static int run_win_bwd(const WinArgs& a, hipStream_t s) {
   PT_ENSURE_LDS((win_bwd_q_kernel<T, DP>), lds);
   PT_LAUNCH((win_bwd_q_kernel<T, DP>), dim3((unsigned)win_blocks(a, plan::ROWS)), dim3(plan::TH), lds, s, a);
   const dim3 keys((unsigned)((a.Nk + KvPlan<T, DP, false>::KEYS - 1) / KvPlan<T, DP, false>::KEYS) * a.Hk * a.B);
-  constexpr bool BF = sizeof(T) == 2;
-  if (BF && a.tiny) {                                    // a kernel of its own: the wide products cost the other one its registers (413 -> 462 us)
-    PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false, BF>), lds_kv);
-    PT_LAUNCH((win_bwd_kv_kernel<T, DP, false, BF>), keys, dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
-  } else {
-    PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false, false>), lds_kv);
-    PT_LAUNCH((win_bwd_kv_kernel<T, DP, false, false>), keys, dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
-  }
+  PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false>), lds_kv);
+  PT_LAUNCH((win_bwd_kv_kernel<T, DP, false>), keys, dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
   if (a.far_chunks) {
-    PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, true, false>), lds_sink);
-    PT_LAUNCH((win_bwd_kv_kernel<T, DP, true, false>), dim3((unsigned)((a.sinks + 31) / 32 * a.far_chunks) * a.H * a.B), dim3(KvPlan<T, DP, true>::TH), lds_sink, s, a);
+    PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, true>), lds_sink);
+    PT_LAUNCH((win_bwd_kv_kernel<T, DP, true>), dim3((unsigned)((a.sinks + 31) / 32 * a.far_chunks) * a.H * a.B), dim3(KvPlan<T, DP, true>::TH), lds_sink, s, a);
     const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sinks * a.D;
     PT_LAUNCH(win_bwd_join_kernel<T>, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, a, 1 + a.far_chunks * (a.H / a.Hk));
   }

@@ -161,6 +161,38 @@ def test_gradients_of_short_sequences_are_rounded_once(D):
         assert float(err) <= 1.02 * (2.0 ** -8) ** 2 / 3 * float(size), (n, float(err / size) ** 0.5)
 
 
+def rounded_once(got, want, what):
+    """bf16: results that are off by d before their one rounding are off by |round(x) - x| + 2 |d| at most after it.  d is 2^-14 of the whole:
+    the factors of the second products and the output in delta are held in 16 bits or more (2^-17 and 2^-16 of each), fp32 sums add less."""
+    size, ideal = float(want.norm()), float((want.to(torch.bfloat16).double() - want).norm())
+    err = float((got.double() - want).norm())
+    assert err <= ideal + 2 * 2.0 ** -14 * size, (what, err, ideal, size)
+
+
+ONCE = {
+    "many keys": (1, 1500, 1500, 4, 1, 128, 1023, 0, 4, None),
+    "sinks and far rows": (1, 900, 900, 4, 2, 64, 300, 0, 40, None),
+    "short sequences in a padded batch": (4, 200, 200, 2, 1, 64, None, 0, 0, [20, 200, 3, 32]),
+    "short sequences, wide heads": (3, 130, 130, 4, 2, 128, 40, 40, 0, [7, 130, 31]),
+}
+
+
+@pytest.mark.parametrize("sharp", [1.0, 6.0])
+@pytest.mark.parametrize("name", sorted(ONCE))
+def test_results_are_rounded_once(name, sharp):
+    """bf16: outputs and gradients of every sequence, whatever its length and that of its neighbours, as far from 64 bits as one rounding.
+    sharp: scores that leave most of a row's weight to a few of its many keys, so that roundings of probabilities do not average out."""
+    case = ONCE[name]
+    q, k, v, do, lengths = make(case, torch.bfloat16)
+    with torch.no_grad():
+        q.mul_(sharp)
+    want, _, see = oracle(q, k, v, do, *case[6:9], lengths)
+    got = grads(q, k, v, do, case, lengths)
+    for b in range(case[0]):
+        for n in "oqkv":
+            rounded_once(got[n][b], want[n][b], (name, b, n))
+
+
 def test_gradients_against_differences():
     case = CASES["a new part of a sequence"]
     q, k, v, do, _ = make(case, torch.float32)
@@ -332,6 +364,21 @@ def test_step_cuts(name, dtype):
         want, tol, _ = oracle(q[b:b + 1, None], k[b:b + 1, :size], v[b:b + 1, :size], q[b:b + 1, None], left, 0, sinks, None)
         err = (o[b].double() - want["o"][0, 0]).abs()
         assert bool((err <= tol["o"][0, 0]).all()), (b, float((err / tol["o"][0, 0]).max()))
+
+
+@pytest.mark.parametrize("name", ["few slices", "many slices", "one workgroup", "wide heads"])
+def test_step_results_are_rounded_once(name):
+    """bf16: the probabilities of the single-token form are held in 16 bits or more, in one slice and in many."""
+    B, N, H, Hk, D, left, sinks, lens = {"few slices": MORE_STEPS["few slices"], "many slices": (2, 6000, 16, 2, 64, None, 0, [6000, 3333]),
+                                         "one workgroup": (3, 900, 4, 4, 64, 700, 4, [900, 20, 801]),
+                                         "wide heads": (4, 3000, 32, 4, 128, 2000, 4, [3000, 1, 2100, 300])}[name]
+    g = torch.Generator(device="cuda").manual_seed(6)
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g).to(torch.bfloat16)  # noqa: E731
+    q, k, v = n(B, H, D) * 3, n(B, N, Hk, D), n(B, N, Hk, D)
+    o = T.window_attention_step(q, k, v, torch.tensor(lens, dtype=torch.int32, device="cuda"), left, sinks=sinks)
+    want = torch.stack([oracle(q[b:b + 1, None], k[b:b + 1, :size], v[b:b + 1, :size], q[b:b + 1, None], left, 0, sinks, None)[0]["o"][0, 0]
+                        for b, size in enumerate(lens)])
+    rounded_once(o, want, name)
 
 
 def test_step_strides_and_growing_cache_in_a_graph():
