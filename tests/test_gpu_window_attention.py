@@ -368,17 +368,18 @@ def test_step_cuts(name, dtype):
 
 @pytest.mark.parametrize("name", ["few slices", "many slices", "one workgroup", "wide heads"])
 def test_step_results_are_rounded_once(name):
-    """bf16: the probabilities of the single-token form are held in 16 bits or more, in one slice and in many."""
+    """bf16: the probabilities of the single-token form are held in 16 bits or more, in one slice and in many.  Scores of a few units, so that many
+    keys share a row's weight (a weight next to 1 is held exactly by any type)."""
     B, N, H, Hk, D, left, sinks, lens = {"few slices": MORE_STEPS["few slices"], "many slices": (2, 6000, 16, 2, 64, None, 0, [6000, 3333]),
                                          "one workgroup": (3, 900, 4, 4, 64, 700, 4, [900, 20, 801]),
                                          "wide heads": (4, 3000, 32, 4, 128, 2000, 4, [3000, 1, 2100, 300])}[name]
     g = torch.Generator(device="cuda").manual_seed(6)
     n = lambda *s: torch.randn(*s, device="cuda", generator=g).to(torch.bfloat16)  # noqa: E731
-    q, k, v = n(B, H, D) * 3, n(B, N, Hk, D), n(B, N, Hk, D)
+    q, k, v = n(B, H, D), n(B, N, Hk, D), n(B, N, Hk, D)
     o = T.window_attention_step(q, k, v, torch.tensor(lens, dtype=torch.int32, device="cuda"), left, sinks=sinks)
-    want = torch.stack([oracle(q[b:b + 1, None], k[b:b + 1, :size], v[b:b + 1, :size], q[b:b + 1, None], left, 0, sinks, None)[0]["o"][0, 0]
-                        for b, size in enumerate(lens)])
-    rounded_once(o, want, name)
+    for b, size in enumerate(lens):
+        want = oracle(q[b:b + 1, None], k[b:b + 1, :size], v[b:b + 1, :size], q[b:b + 1, None], left, 0, sinks, None)[0]
+        rounded_once(o[b], want["o"][0, 0], (name, b))
 
 
 def test_step_strides_and_growing_cache_in_a_graph():
