@@ -384,7 +384,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(co
     const bool on = row < r1;
     if (!AHEAD) fetch(row);
     float x[PER], t[PER], dy[PER], dh[PER];
-    const f32x4 st = ns;
+    const f32x4 st = on ? ns : f32x4{0.f, 0.f, 0.f, 0.f};   // another's row: its statistics may be no numbers, and 0 times these none either
     nx.get(x, cols);
     nt.get(t, cols);
     ny.get(dy, cols);

@@ -219,6 +219,22 @@ def test_rows_of_zeros_infinities_and_nan_stay_in_their_rows():
     assert bool(torch.isfinite(grads["gate"][0]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(40_002, 8, 20_001), (6002, 512, 3001), (8190, 4096, 4095)], ids=str)
+@pytest.mark.parametrize("bad", ["x", "t"])
+def test_a_row_that_is_not_finite_reaches_its_own_clip_only(bad, shape, dtype):
+    """Long clips that many workers share, with rows over: the workers behind a clip's end look at the next clip's rows."""
+    rows, cols, clip = shape
+    v, dy, dh = make(rows, cols, clip, dtype)
+    want = run(v, clip, "layer", dy, dh)[2]
+    with torch.no_grad():
+        v[bad][clip, cols // 2] = float("nan")
+    got = run(v, clip, "layer", dy, dh)[2]
+    assert torch.equal(got["gate"][0], want["gate"][0]) and bool(torch.isnan(got["gate"][1]).all())
+    ok = torch.arange(rows, device="cuda") != clip
+    assert all(torch.equal(got[k][ok], want[k][ok]) and bool(torch.isfinite(got[k][ok]).all()) for k in ("x", "t"))
+
+
 def test_captured_forward_and_backward():
     v, dy, dh = make(300, 520, 100, torch.bfloat16)
     base = {k: x.detach() for k, x in v.items()}
