@@ -246,7 +246,8 @@ int pt_train_ln_bwd(const float* dy, const float* x, const float* res, const flo
 /* The norms around a residual sum with its gate and scale, rows of `cols` (1 to 8192) values, dtype 0 fp32 | 1 bf16:
  *   y = x + res_scale * gate[row / rows_per_clip] * u,  u = N(t) * post_w + post_b,  h = N(y) * pre_w + pre_b
  * kind 0 LayerNorm, 1 RMSNorm.  x, t: row strides ldx, ldt; gate [rows / rows_per_clip][cols]; the rest contiguous; vectors fp32.  May
- * be NULL: t (then y is x and not written), gate, res_scale (ones), post_w (u = t), post_b, pre_w (no h), pre_b.  stats [rows][4]
+ * be NULL: t (then y is x and not written), gate, res_scale (ones), post_w (u = t), post_b, pre_w (no h), pre_b; a bias
+ * comes with its weight.  stats [rows][4]
  * (16-byte aligned, may be NULL) is what the backward call needs: mean and 1/std of t and of y.
  * Backward: dy or dh may be NULL (zeros); any gradient but dx may be NULL.  ws: pt_train_gated_norm_workspace_bytes(rows, cols,
  * rows_per_clip or 0 without a gate) bytes, 16-byte aligned.  Gradients are written, not added to, and do not depend on timing. */

@@ -634,11 +634,12 @@ static int run_gated(const GatedArgs& g, const GatedPlan& p, Access acc, int bac
   }
 }
 
-static int check_gated(const char* who, const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, int64_t rows, int cols, int clip,
-                       int kind, int dtype) {
+static int check_gated(const char* who, const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* w1, const float* b1,
+                       const float* w2, const float* b2, int64_t rows, int cols, int clip, int kind, int dtype) {
   PT_CHECK(x && rows >= 1 && rows <= 0x7FFFFFFF && cols >= 1 && cols <= 8192, "%s: %lld rows of %d columns (1 to 8192)", who, (long long)rows, cols);
   PT_CHECK(ldx >= cols && (!t || ldt >= cols), "%s: row strides %lld and %lld for %d columns", who, (long long)ldx, (long long)ldt, cols);
   PT_CHECK(!gate || (t && clip >= 1 && rows % clip == 0), "%s: %lld rows in clips of %d", who, (long long)rows, clip);
+  PT_CHECK((w1 || !b1) && (w2 || !b2), "%s: a bias comes with its weight", who);
   PT_CHECK((kind == 0 || kind == 1) && (dtype == 0 || dtype == 1), "%s: kind %d, dtype %d", who, kind, dtype);
   return 0;
 }
@@ -656,7 +657,7 @@ static Access gated_access(const GatedArgs& g, int dtype) {
 int launch_gated_norm_fwd(const void* x, int64_t ldx, const void* t, int64_t ldt, const void* gate, const float* a, const float* w1,
                           const float* b1, const float* w2, const float* b2, void* y, void* h, float* stats, int64_t rows, int cols, int clip,
                           int kind, float eps, int dtype, hipStream_t s) {
-  if (check_gated("gated_norm_fwd", x, ldx, t, ldt, gate, rows, cols, clip, kind, dtype)) return 1;
+  if (check_gated("gated_norm_fwd", x, ldx, t, ldt, gate, w1, b1, w2, b2, rows, cols, clip, kind, dtype)) return 1;
   PT_CHECK((t || w2) && (!t || y) && (!w2 || h) && ((uintptr_t)stats & 15) == 0, "gated_norm_fwd: null or misaligned argument");
   GatedArgs g = {};
   g.x = x; g.t = t; g.gate = gate; g.a = a; g.w1 = w1; g.b1 = b1; g.w2 = w2; g.b2 = b2; g.y = y; g.h = h; g.stats = stats;
@@ -673,7 +674,7 @@ int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt
                           const float* b1, const float* w2, const float* stats, const void* dy, const void* dh, void* dx, void* dt,
                           void* dgate, float* da, float* dw1, float* db1, float* dw2, float* db2, void* ws, size_t ws_bytes, int64_t rows,
                           int cols, int clip, int kind, int dtype, hipStream_t s) {
-  if (check_gated("gated_norm_bwd", x, ldx, t, ldt, gate, rows, cols, clip, kind, dtype)) return 1;
+  if (check_gated("gated_norm_bwd", x, ldx, t, ldt, gate, w1, b1, w2, nullptr, rows, cols, clip, kind, dtype)) return 1;
   PT_CHECK(stats && dx && (dy || dh) && (!dh || w2) && (!dgate || gate) && (!dt || t), "gated_norm_bwd: null argument");
   PT_CHECK(ws && ws_bytes >= gated_norm_workspace((int)rows, cols, gate ? clip : 0) && (((uintptr_t)ws | (uintptr_t)stats) & 15) == 0,
            "gated_norm_bwd: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, gated_norm_workspace((int)rows, cols, gate ? clip : 0));

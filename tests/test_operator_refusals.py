@@ -101,3 +101,12 @@ def test_window_attention_refuses():
     refused(L.pt_attention_window_step(p, p, p, p, st, p, *(step | dict(N=0)).values(), p, 1 << 20, None), "keys")
     refused(L.pt_attention_window_step(p, p, p, p, st, p, *step.values(), p, 0, None), "workspace")
     refused(L.pt_attention_window_step(p, odd, p, p, st, p, *step.values(), p, 1 << 20, None), "multiples")
+
+
+def test_gated_norm_refuses_a_bias_without_its_weight():
+    """Forward would leave the bias of u out and backward count it in."""
+    L, p, n = _lib.lib(), C.c_void_p(256), None
+    fwd = lambda post_w, post_b, pre_w, pre_b: L.pt_train_gated_norm_fwd(p, 4, p, 4, n, n, post_w, post_b, pre_w, pre_b, p, p, n, 2, 4, 2, 0, 1e-5, 0, None)  # noqa: E731
+    refused(fwd(n, p, p, p), "bias")
+    refused(fwd(p, p, n, p), "bias")
+    refused(L.pt_train_gated_norm_bwd(p, 4, p, 4, n, n, n, p, p, p, p, p, p, p, n, n, n, n, n, n, p, 1 << 20, 2, 4, 2, 0, 0, None), "bias")
