@@ -678,6 +678,7 @@ int launch_gated_norm_bwd(const void* x, int64_t ldx, const void* t, int64_t ldt
   PT_CHECK(stats && dx && (dy || dh) && (!dh || w2) && (!dgate || gate) && (!dt || t), "gated_norm_bwd: null argument");
   PT_CHECK(ws && ws_bytes >= gated_norm_workspace((int)rows, cols, gate ? clip : 0) && (((uintptr_t)ws | (uintptr_t)stats) & 15) == 0,
            "gated_norm_bwd: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, gated_norm_workspace((int)rows, cols, gate ? clip : 0));
+  if (!t) a = w1 = b1 = nullptr;                           // y is x, whatever else is given
   GatedArgs g = {};
   g.x = x; g.t = t; g.gate = gate; g.a = a; g.w1 = w1; g.b1 = b1; g.w2 = w2; g.dy = dy; g.dh = dh; g.stats = const_cast<float*>(stats);
   g.dx = dx; g.dt = dt; g.dgate = dgate;

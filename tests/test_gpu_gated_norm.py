@@ -235,6 +235,28 @@ def test_a_row_that_is_not_finite_reaches_its_own_clip_only(bad, shape, dtype):
     assert all(torch.equal(got[k][ok], want[k][ok]) and bool(torch.isfinite(got[k][ok]).all()) for k in ("x", "t"))
 
 
+def test_without_t_nothing_else_of_the_first_norm_counts():
+    """The C entries take res_scale, post_w and post_b without t: y is x then, in the backward pass too."""
+    from probtalk_amd import _lib
+    L, p, rows, cols = _lib.lib(), _lib.ptr, 30, 72
+    v, _, dh = make(rows, cols, 10, torch.float32)
+    d = {k: x.detach() for k, x in v.items()}
+    got = []
+    for first in ((None, None, None), (d["res_scale"], d["post_weight"], d["post_bias"])):
+        h, stats, dx = torch.empty_like(d["x"]), torch.empty(rows, 4, device="cuda"), torch.empty_like(d["x"])
+        dw, db = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+        ws = torch.empty(L.pt_train_gated_norm_workspace_bytes(rows, cols, 0), dtype=torch.uint8, device="cuda")
+        _lib.check(L.pt_train_gated_norm_fwd(p(d["x"]), cols, None, 0, None, *map(p, first), p(d["pre_weight"]), p(d["pre_bias"]), None, p(h), p(stats), rows, cols,
+                                             rows, 0, 1e-5, 0, _lib.stream()))
+        _lib.check(L.pt_train_gated_norm_bwd(p(d["x"]), cols, None, 0, None, *map(p, first), p(d["pre_weight"]), p(stats), None, p(dh), p(dx), None, None, None, None,
+                                             None, p(dw), p(db), p(ws), ws.numel(), rows, cols, rows, 0, 0, _lib.stream()))
+        got.append((h, dx, dw, db))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    y, h = T.gated_norm(v["x"], pre_weight=v["pre_weight"], pre_bias=v["pre_bias"])
+    assert y is v["x"] and torch.equal(got[0][0], h)
+    assert torch.equal(got[0][1], torch.autograd.grad(h, v["x"], dh)[0])
+
+
 def test_captured_forward_and_backward():
     v, dy, dh = make(300, 520, 100, torch.bfloat16)
     base = {k: x.detach() for k, x in v.items()}
