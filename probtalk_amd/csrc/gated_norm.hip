@@ -264,23 +264,23 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void gated_norm_fwd_kernel(const
 #pragma unroll
   for (int i = 0; i < PER; ++i) gt[i] = a[i];
   Raw<T, L, PER, ACC> nx, nt;                               // without t: x in its place, not used
-  auto fetch = [&](int row) {
-    row = min(row, g.rows - 1);
+  auto fetch = [&](unsigned row) {
+    row = min(row, (unsigned)g.rows - 1u);
     nx.load(X + (size_t)row * g.ldx, cols);
     nt.load(Tt ? Tt + (size_t)row * g.ldt : X + (size_t)row * g.ldx, cols);
   };
   fetch(r0);
   int left = 0;                                          // rows left of the current clip
   for (int k = 0; k < g.run; ++k) {                      // the same count for every worker of the block: barriers inside
-    const int row = r0 + k;
-    const bool on = row < r1;
+    const unsigned row = (unsigned)r0 + k;               // behind the worker's last row it may pass 2^31
+    const bool on = k < r1 - r0;
     float x[PER], t[PER];
     nx.get(x, cols);
     nt.get(t, cols);
     fetch(row + 1);
     if (g.gate && on && left == 0) {
-      const int clip = row / g.clip;
-      left = (clip + 1) * g.clip - row;
+      const int clip = (int)row / g.clip;
+      left = (clip + 1) * g.clip - (int)row;
       load_row<T, L, PER, ACC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
 #pragma unroll
       for (int i = 0; i < PER; ++i) gt[i] *= a[i];
@@ -368,8 +368,8 @@ __global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(co
   for (int i = 0; i < PER; ++i) { gt[i] = 1.f; aw[i] = ab[i] = bw[i] = bb[i] = dg[i] = 0.f; }
   Raw<T, L, PER, ACC> nx, nt, ny, nh;
   f32x4 ns = {0.f, 0.f, 0.f, 0.f};
-  auto fetch = [&](int row) {                            // what is left out: x in its place, not used
-    row = min(row, g.rows - 1);
+  auto fetch = [&](unsigned row) {                       // what is left out: x in its place, not used
+    row = min(row, (unsigned)g.rows - 1u);
     const T* x = X + (size_t)row * g.ldx;
     nx.load(x, cols);
     nt.load(Tt ? Tt + (size_t)row * g.ldt : x, cols);
@@ -380,8 +380,8 @@ __global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(co
   if (AHEAD) fetch(r0);
   int left = 0, clip = 0;
   for (int k = 0; k < g.run; ++k) {
-    const int row = r0 + k;
-    const bool on = row < r1;
+    const unsigned row = (unsigned)r0 + k;               // behind the worker's last row it may pass 2^31
+    const bool on = k < r1 - r0;
     if (!AHEAD) fetch(row);
     float x[PER], t[PER], dy[PER], dh[PER];
     const f32x4 st = on ? ns : f32x4{0.f, 0.f, 0.f, 0.f};   // another's row: its statistics may be no numbers, and 0 times these none either
@@ -400,8 +400,8 @@ __global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(co
       for (int i = 0; i < PER; ++i) x[i] = dh[i] = 0.f;
     if (AHEAD) fetch(row + 1);
     if (g.gate && on && left == 0) {
-      clip = row / g.clip;
-      left = (clip + 1) * g.clip - row;
+      clip = (int)row / g.clip;
+      left = (clip + 1) * g.clip - (int)row;
       load_row<T, L, PER, ACC>((const T*)g.gate + (size_t)clip * cols, cols, gt);
       if constexpr (WIDE)
 #pragma unroll
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, 2) void gated_norm_bwd_kernel(co
       }
       if (on && g.dt) store_row<T, L, PER, ACC>((T*)g.dt + (size_t)row * cols, cols, dy, g.stream);
     }
-    if (g.dgate && on && !g.joined && (left == 0 || row + 1 == r1)) {
+    if (g.dgate && on && !g.joined && (left == 0 || k + 1 == r1 - r0)) {
       if (g.gpart) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) if (column<T, L, PER>(i) < cols) g.gpart[(size_t)worker * cols + column<T, L, PER>(i)] = dg[i];
@@ -575,7 +575,7 @@ static GatedPlan gated_plan(int rows, int cols, int clip, bool gate, int waves) 
   while (p.lanes * p.per < cols) p.lanes *= 2;
   p.rpb = p.lanes >= 256 ? 1 : 256 / p.lanes;
   const int64_t want = (int64_t)device_cus() * waves * 64 / p.lanes;
-  const int64_t run = std::max<int64_t>(1, (rows + want - 1) / want);
+  const int64_t run = std::max<int64_t>(1, (rows + want - 1) / want), clips = ((int64_t)rows + clip - 1) / clip;
   p.spc = p.joined = 0;
   if (!gate) {
     p.run = (int)run;
@@ -587,8 +587,8 @@ static GatedPlan gated_plan(int rows, int cols, int clip, bool gate, int waves) 
     p.spc = (int)((clip + run - 1) / run);
     p.joined = p.spc >= p.rpb;
     if (p.joined) p.spc = (p.spc + p.rpb - 1) / p.rpb * p.rpb;
-    p.run = (clip + p.spc - 1) / p.spc;                    // at most `run`
-    p.workers = (rows + clip - 1) / clip * p.spc;
+    p.run = (int)(((int64_t)clip + p.spc - 1) / p.spc);    // at most `run`
+    p.workers = (int)(clips * p.spc);                      // at most four times `want`: a clip has more than `run` rows
   }
   p.blocks = (p.workers + p.rpb - 1) / p.rpb;
   return p;

@@ -257,6 +257,44 @@ def test_without_t_nothing_else_of_the_first_norm_counts():
     assert torch.equal(got[0][1], torch.autograd.grad(h, v["x"], dh)[0])
 
 
+def test_as_many_rows_as_32_bits_hold():
+    """Rows of one value (RMS): 2^31 - 1 of them forward, where a row's number behind the last one passes 32 bits; and one gate for more than
+    2^30 rows with gradients.  The same rows in a small call give the same bits."""
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 60 GB")
+    g = torch.Generator(device="cuda").manual_seed(7)
+    part, dt = 1 << 20, torch.bfloat16
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g).to(dt)  # noqa: E731
+    w = torch.tensor([0.9], device="cuda")
+    gate = n(1, 1) + 1
+    small = [n(part, 1) for _ in range(4)]
+    f = lambda x, t, q: T.gated_norm(x, t, q, None, w, None, w, kind="rms", rows_per_clip=x.shape[0])  # noqa: E731
+    rows = (1 << 31) - 1
+    big = [x.repeat(1 << 11, 1)[:rows] for x in small[:2]]
+    with torch.no_grad():
+        y, h = f(*big, gate)
+        want = f(*small[:2], gate)
+    for got, e in zip((y, h), want):
+        assert torch.equal(got[:part], e) and torch.equal(got[-part + 1:], e[:-1]) and torch.equal(got[rows // 2 // part * part:][:part], e)
+    del big, y, h, got
+    times = (1 << 10) + 1
+    x, t, dy, dh = (v.repeat(times, 1) for v in small)
+    leaves = [v.requires_grad_() for v in (x, t, gate.clone())]
+    dx, dtt, dg = torch.autograd.grad(f(*leaves), leaves, (dy, dh))
+    same = [v.clone().requires_grad_() for v in (*small[:2], gate)]
+    ex, et, _ = torch.autograd.grad(f(*same), same, small[2:])
+    for got, e in ((dx, ex), (dtt, et)):
+        assert torch.equal(got[:part], e) and torch.equal(got[-part:], e)
+    s = [v.detach().double().requires_grad_() for v in same]
+    norm = lambda v: v / (v.square() + 1e-5).sqrt() * w.double()  # noqa: E731
+    u = norm(s[1])
+    yy = s[0] + s[2] * u
+    d = torch.autograd.grad((yy, norm(yy)), [s[0], s[2]], [v.double() for v in small[2:]])
+    # a worker adds up 65,600 rows one after the other, 16,384 workers are added up after that; a bf16 result
+    size = float((d[0] * u.detach()).abs().sum()) * times
+    assert abs(float(dg) - float(d[1]) * times) <= (65_600 + 16_400) * U * size + 2.0 ** -8 * abs(float(d[1]) * times)
+
+
 def test_captured_forward_and_backward():
     v, dy, dh = make(300, 520, 100, torch.bfloat16)
     base = {k: x.detach() for k, x in v.items()}

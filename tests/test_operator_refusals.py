@@ -110,3 +110,10 @@ def test_gated_norm_refuses_a_bias_without_its_weight():
     refused(fwd(n, p, p, p), "bias")
     refused(fwd(p, p, n, p), "bias")
     refused(L.pt_train_gated_norm_bwd(p, 4, p, 4, n, n, n, p, p, p, p, p, p, p, n, n, n, n, n, n, p, 1 << 20, 2, 4, 2, 0, 0, None), "bias")
+
+
+def test_gated_norm_counts_rows_beyond_2_to_the_30():
+    """A clip of rows that 32 bits hold, but not twice: 512 blocks of 32 workers, five sums of 8 columns each (256 CUs)."""
+    f = _lib.lib().pt_train_gated_norm_workspace_bytes
+    assert [f(n, 8, n) for n in (1 << 30, (1 << 30) + 64, (1 << 31) - 1)] == [512 * 5 * 8 * 4] * 3
+    assert f(1 << 31, 8, 0) == 0
