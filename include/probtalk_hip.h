@@ -294,7 +294,7 @@ int pt_train_embed_bwd(const float* dx, const int32_t* ids, int rows, int vocab,
 /* nn.Dropout: y = x * mask / (1-p), mask = hash(seed, element) (call again on dy with the same seed for the backward) */
 int pt_train_dropout(const float* x, float* y, size_t n, float p, uint64_t seed, void* stream);
 /* torch.nn.utils.clip_grad_norm_ + torch.optim.AdamW (predictor.py:112-118,270-278): *out += sum g^2; coef = min(1,
- * max_norm / (sqrt(sumsq) + 1e-6)); AdamW update with the gradient scaled by *gscale (device scalar, may be NULL) */
+ * max_norm / (sqrt(sumsq) + 1e-6)), NaN where the norm is; AdamW update with the gradient scaled by *gscale (device scalar, may be NULL) */
 int pt_train_sumsq(const float* g, size_t n, float* out, void* stream);
 int pt_train_clip_coef(const float* sumsq, float max_norm, float* coef, float* norm_out, void* stream);
 int pt_train_adamw(float* p, const float* g, float* m, float* v, size_t n, const float* gscale, float lr, float beta1,
@@ -302,7 +302,7 @@ int pt_train_adamw(float* p, const float* g, float* m, float* v, size_t n, const
 int pt_train_add(const float* a, const float* b, float* out, size_t n, void* stream);
 /* The same two over a whole list of tensors (host arrays of `count` device pointers and sizes; entries of size 0 are skipped; a
  * call reads the arrays before it returns).
- * pt_train_grad_norm: *norm = sqrt(sum over the list of g^2), *coef = min(1, max_norm / (*norm + 1e-6)); is_bf16 (may be NULL: all
+ * pt_train_grad_norm: *norm = sqrt(sum over the list of g^2), *coef = min(1, max_norm / (*norm + 1e-6)), NaN where the norm is; is_bf16 (may be NULL: all
  *   fp32) marks tensors held in bf16.  Squares are summed in fp64 in a fixed order: the same gradients give the same bits.  ws:
  *   pt_train_grad_norm_workspace_bytes(n, count) bytes, 8-byte aligned.
  * pt_train_adamw_multi: the update of pt_train_adamw on every tensor.  dtype of p and g: 0 fp32, 1 bf16 (parameters are then rounded

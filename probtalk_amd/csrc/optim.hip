@@ -484,7 +484,7 @@ __device__ __forceinline__ void norm_out(double s, float max_norm, float* __rest
     const float nrm = (float)sqrt(s);
     const float c = max_norm / (nrm + 1e-6f);
     *norm = nrm;
-    *coef = c < 1.f ? c : 1.f;
+    *coef = c > 1.f ? 1.f : c;                           // a norm that is no number gives a coefficient that is none
   }
 }
 __global__ __launch_bounds__(1024) void grad_norm_kernel(const double* __restrict__ part, unsigned units, float max_norm,

@@ -1546,11 +1546,11 @@ int launch_adamw(float* p, const float* g, float* m, float* v, size_t n, const f
   PT_LAUNCH(adamw_kernel, dim3(ew_blocks(n)), dim3(256), 0, s, p, g, m, v, n, gscale, lr, beta1, beta2, eps, wd, bc1, sqrtf(bc2));
   return 0;
 }
-// clip coefficient of torch.nn.utils.clip_grad_norm_: coef = min(1, max_norm / (sqrt(sumsq) + 1e-6)); norm_out = sqrt(sumsq)
+// clip coefficient of torch.nn.utils.clip_grad_norm_: coef = min(1, max_norm / (sqrt(sumsq) + 1e-6)), NaN where that is; norm_out = sqrt(sumsq)
 __global__ void clip_coef_kernel(const float* __restrict__ sumsq, float max_norm, float* __restrict__ coef, float* __restrict__ norm_out) {
   const float nrm = sqrtf(*sumsq);
   const float c = max_norm / (nrm + 1e-6f);
-  *coef = c < 1.f ? c : 1.f;
+  *coef = c > 1.f ? 1.f : c;                             // a norm that is no number gives a coefficient that is none
   if (norm_out) *norm_out = nrm;
 }
 int launch_clip_coef(const float* sumsq, float max_norm, float* coef, float* norm_out, hipStream_t s) {

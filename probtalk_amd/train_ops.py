@@ -854,7 +854,7 @@ def _grad_norm(pointers, sizes, is_bf16, n, max_norm, device, ws_bytes=None):
 
 def grad_norm(grads, max_norm):
     """(norm, coef), two device tensors of one float: the norm over all of `grads` (fp32 or bf16) and the factor
-    min(1, max_norm / (norm + 1e-6)) of torch.nn.utils.clip_grad_norm_.  The sum runs in fp64 in a fixed order."""
+    min(1, max_norm / (norm + 1e-6)) of torch.nn.utils.clip_grad_norm_, NaN where the norm is.  The sum runs in fp64 in a fixed order."""
     grads = [g.contiguous() for g in grads]
     device = _same("grad_norm", grads, (torch.float32, torch.bfloat16)) if grads else torch.device("cuda", torch.cuda.current_device())
     kinds = None

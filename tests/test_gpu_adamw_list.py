@@ -58,6 +58,46 @@ def test_norm_of_nothing_and_of_non_finite():
     assert math.isnan(float(T.grad_norm([g], 1.0)[0]))
 
 
+def pair_of_calls(gs, max_norm):
+    """Norm and coefficient by the entries for one tensor."""
+    from probtalk_amd import _lib
+    L, p, s = _lib.lib(), _lib.ptr, _lib.stream()
+    total, coef, norm = (torch.zeros(1, device="cuda") for _ in range(3))
+    for g in gs:
+        _lib.check(L.pt_train_sumsq(p(g), g.numel(), p(total), s))
+    _lib.check(L.pt_train_clip_coef(p(total), max_norm, p(coef), p(norm), s))
+    return norm, coef
+
+
+@pytest.mark.parametrize("name", ["units", "many", "one"])
+def test_norm_of_a_list_is_that_of_the_entries_for_one_tensor(name):
+    gs = tensors(LISTS[name], 21, 0.3)
+    want, got = pair_of_calls(gs, 0.7), T.grad_norm(gs, 0.7)
+    # fp32 sums of squares: a thread passes n / 262,144 + 1 values, then 6 lanes, 4 waves and as many workgroups as there are, once per tensor; the
+    # root halves what they lose, the quotient keeps it
+    n = sum(1 + 6 + 4 + min(-(-s // 1024), 1024) + s // 262_144 for s in LISTS[name])
+    for a, b in zip(want, got):
+        assert abs(float(a) - float(b)) <= (n / 2 + 8) * E * float(b)
+
+
+@pytest.mark.parametrize("size", [1000, 300_000])                          # one launch, and a launch of partial sums
+def test_a_norm_that_is_no_number_is_not_taken_for_one(size):
+    """As torch.nn.utils.clip_grad_norm_ has it: the factor is NaN, and no tensor takes an unclipped step."""
+    gs = [torch.ones(size, device="cuda"), torch.ones(7, device="cuda")]
+    gs[0][3] = math.nan
+    for norm, coef in (T.grad_norm(gs, 1.0), pair_of_calls(gs, 1.0)):
+        assert math.isnan(float(norm)) and math.isnan(float(coef))
+    ps = [torch.nn.Parameter(torch.ones_like(g)) for g in gs]
+    qs = [torch.nn.Parameter(torch.ones_like(g)) for g in gs]
+    for p, q, g in zip(ps, qs, gs):
+        p.grad, q.grad = g.clone(), g.clone()
+    torch.nn.utils.clip_grad_norm_(ps, 1.0)
+    torch.optim.AdamW(ps).step()
+    norm, coef = T.clip_grad_norm(qs, 1.0)
+    T.AdamW([{"params": qs}]).step({q: coef for q in qs})
+    assert all(torch.equal(torch.isnan(p), torch.isnan(q)) and bool(torch.isnan(q).all()) for p, q in zip(ps, qs))
+
+
 def reference(p, g, m, v, coef, step, lr, betas, eps, weight_decay):
     """64 bits, with the constants that the kernel is given (fp32)."""
     b1, b2, lr, eps, wd = (float(np.float32(x)) for x in (*betas, lr, eps, weight_decay))
