@@ -12,6 +12,7 @@ import contextlib
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, ptr, stream
@@ -172,6 +173,11 @@ def layer_norm(x, gamma, beta, res=None):
     return LayerNormRes.apply(x, res, gamma, beta)
 
 
+def _forward_mode():
+    """Whether tensors may carry tangents, which autograd refuses for its functions without a forward rule: a raw call would drop them."""
+    return forward_ad._current_level >= 0
+
+
 def _row_major(v):
     return v if v.stride(1) == 1 and v.stride(0) >= v.shape[1] else v.contiguous()
 
@@ -240,7 +246,7 @@ def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias
     x, t: rows (R, C) of fp32 or bf16, 1 <= C <= 8192.  gate (R / rows_per_clip, C) of x's type: a row for every rows_per_clip rows
     (by default as many as it has rows for).  Vectors of C values in fp32.  kind: 'layer' (mean and variance) or 'rms'.  Left out:
     t (y is x itself), gate, res_scale, post_weight (u = t), pre_weight (h is None).  Statistics and sums are fp32; h is taken from y
-    before that is rounded to bf16.  To capture the backward pass into a HIP graph, make the leaves inside the capture
+    before that is rounded to bf16.  No forward-mode differentiation.  To capture the backward pass into a HIP graph, make the leaves inside the capture
     (x.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16) or not 1 <= x.shape[1] <= 8192 or x.shape[0] < 1:
         raise RuntimeError(f"gated_norm: rows (R, C) of fp32 or bf16 on the GPU with C up to 8192, got {tuple(x.shape)} {x.dtype} on {x.device}")
@@ -274,7 +280,7 @@ def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias
         t = _row_major(t)
     given = (x, t, gate, *[v if v is None or v.is_contiguous() else v.contiguous() for v in vectors])
     mode = 0 if kind == "layer" else 1
-    if torch.is_grad_enabled() and any([v is not None and v.requires_grad for v in given]):
+    if _forward_mode() or (torch.is_grad_enabled() and any([v is not None and v.requires_grad for v in given])):
         y, h = GatedNorm.apply(*given, clip, mode, eps)
     else:
         y, h, _ = _gated_norm(*given, clip, mode, eps, False)
@@ -440,7 +446,7 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
     keys of each sequence of a padded batch (what lies behind is not read; all of them by default).  A row that sees nothing gives
     zeros and no gradient.  Softmax and sums are fp32; scale is 1 / sqrt(D) by default.  Keys and values inside a sequence must be
     finite.  With gradients, bf16 keeps a byte more of every output value for them.  The backward pass is free of
-    atomics: the same inputs give the same bits.  To capture it into a HIP graph, make the leaves inside the capture
+    atomics: the same inputs give the same bits.  No forward-mode differentiation.  To capture it into a HIP graph, make the leaves inside the capture
     (q.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if q.dim() != 4 or q.shape[0] < 1 or q.shape[1] < 1:
         raise RuntimeError(f"window_attention: q is (B, Nq, H, D), got {tuple(q.shape)}")
@@ -451,7 +457,7 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
         raise RuntimeError(f"window_attention: {Nq} rows for {Nk} keys")
     meta = (B, Nq, Nk, H, Hk, D, left, right, sinks, scale, int(q.dtype is torch.bfloat16))
     q, k, v = [_vectors(t if t.shape[1] == 1 or 0 <= t.stride(1) <= 1 << 20 else t.contiguous()) for t in (q, k, v)]
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _forward_mode() or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         return WindowAttention.apply(q, k, v, lengths, meta)
     return _window_attention(q, k, v, lengths, meta, False)[0]
 
@@ -464,6 +470,8 @@ def window_attention_step(q, k, v, lengths, left=None, sinks=0, scale=None):
         raise RuntimeError(f"window_attention_step: q is (B, H, D), got {tuple(q.shape)}")
     if lengths is None:
         raise RuntimeError("window_attention_step: lengths are needed")
+    if _forward_mode() and any([forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v)]):
+        raise NotImplementedError("window_attention_step: no forward mode differentiation")
     B, H, D = q.shape
     left, _, sinks, scale = _check_window("window_attention_step", q, k, v, H, B, lengths, left, 0, sinks, scale)
     if not _has_vectors(k) or not _has_vectors(v):

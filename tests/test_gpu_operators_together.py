@@ -95,6 +95,23 @@ def test_a_block_its_gradients_and_a_step(B, N, lengths):
         assert bool((err <= 2.0 ** -22 * P[n].abs() + lr * 2.0 ** -12).all()), (n, float(err.max()))
 
 
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused_not_dropped(grad):
+    from torch.autograd import forward_ad
+    x, w = torch.randn(8, 64, device="cuda"), torch.ones(64, device="cuda")
+    q, lengths = torch.randn(1, 4, 2, 32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for f in (lambda: T.gated_norm(dual(x), pre_weight=w), lambda: T.gated_norm(x, x.clone(), post_weight=dual(w), pre_weight=w),
+                  lambda: T.window_attention(dual(q), q, q), lambda: T.window_attention(q, q, dual(q)),
+                  lambda: T.window_attention_step(q[:, 0], q, dual(q), lengths)):
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                f()
+        T.gated_norm(x, pre_weight=w)                      # without tangents they run
+        T.window_attention(q, q, q)
+        T.window_attention_step(q[:, 0], q, q, lengths)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_token_by_token_over_a_cache(dtype):
     """The block's attention for the last token of growing sequences: what window_attention gives for that row."""
