@@ -178,6 +178,19 @@ def _forward_mode():
     return forward_ad._current_level >= 0
 
 
+class _Last(torch.autograd.Function):
+    """Gradients inside a graph of their own (create_graph): a gradient of these is refused, not left out.  `anchor`: a tensor that requires one."""
+
+    @staticmethod
+    def forward(ctx, what, anchor, *grads):
+        ctx.what = what
+        return tuple(None if g is None else g.clone() for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what}: no second derivatives")
+
+
 def _row_major(v):
     return v if v.stride(1) == 1 and v.stride(0) >= v.shape[1] else v.contiguous()
 
@@ -234,6 +247,8 @@ class GatedNorm(torch.autograd.Function):
             ws = torch.empty(size, dtype=torch.uint8, device=device)
             at = [None if v is None else v.data_ptr() for v in (x, t, gate, res_scale, post_w, post_b, pre_w, stats, dy, dh, dx, dt, dgate, *vec, ws)]
             check(L.pt_train_gated_norm_bwd(at[0], _row_stride(x), at[1], _row_stride(t), *at[2:], size, rows, cols, clip, kind, bf, stream()))
+        if torch.is_grad_enabled():
+            dx, dt, dgate, *vec = _Last.apply("gated_norm", torch.zeros((), requires_grad=True), dx, dt, dgate, *vec)
         return dx, dt, dgate, *vec, None, None, None
 
 
@@ -246,7 +261,7 @@ def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias
     x, t: rows (R, C) of fp32 or bf16, 1 <= C <= 8192.  gate (R / rows_per_clip, C) of x's type: a row for every rows_per_clip rows
     (by default as many as it has rows for).  Vectors of C values in fp32.  kind: 'layer' (mean and variance) or 'rms'.  Left out:
     t (y is x itself), gate, res_scale, post_weight (u = t), pre_weight (h is None).  Statistics and sums are fp32; h is taken from y
-    before that is rounded to bf16.  No forward-mode differentiation.  To capture the backward pass into a HIP graph, make the leaves inside the capture
+    before that is rounded to bf16.  No forward-mode and no second derivatives.  To capture the backward pass into a HIP graph, make the leaves inside the capture
     (x.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16) or not 1 <= x.shape[1] <= 8192 or x.shape[0] < 1:
         raise RuntimeError(f"gated_norm: rows (R, C) of fp32 or bf16 on the GPU with C up to 8192, got {tuple(x.shape)} {x.dtype} on {x.device}")
@@ -411,6 +426,8 @@ class WindowAttention(torch.autograd.Function):
             ws = torch.empty(L.pt_attention_window_bwd_workspace_bytes(*ctx.meta[:9]), dtype=torch.uint8, device=q.device)
             check(L.pt_attention_window_bwd(_at(q), _at(k), _at(v), _at(o), _at(do), _at(stats), _at(dq), _at(dk), _at(dv), _address(_strides(q, k, v)),
                                             _at(lengths), *ctx.meta, _at(ws), ws.numel(), stream()))
+        if torch.is_grad_enabled():
+            dq, dk, dv = _Last.apply("window_attention", torch.zeros((), requires_grad=True), dq, dk, dv)
         return dq, dk, dv, None, None
 
 
@@ -446,7 +463,7 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
     keys of each sequence of a padded batch (what lies behind is not read; all of them by default).  A row that sees nothing gives
     zeros and no gradient.  Softmax and sums are fp32; scale is 1 / sqrt(D) by default.  Keys and values inside a sequence must be
     finite.  With gradients, bf16 keeps a byte more of every output value for them.  The backward pass is free of
-    atomics: the same inputs give the same bits.  No forward-mode differentiation.  To capture it into a HIP graph, make the leaves inside the capture
+    atomics: the same inputs give the same bits.  No forward-mode and no second derivatives.  To capture it into a HIP graph, make the leaves inside the capture
     (q.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if q.dim() != 4 or q.shape[0] < 1 or q.shape[1] < 1:
         raise RuntimeError(f"window_attention: q is (B, Nq, H, D), got {tuple(q.shape)}")

@@ -112,6 +112,24 @@ def test_tangents_are_refused_not_dropped(grad):
         T.window_attention_step(q[:, 0], q, q, lengths)
 
 
+def test_second_derivatives_are_refused_not_left_out():
+    x, b = (torch.randn(s, device="cuda", requires_grad=True) for s in ((8, 64), (64,)))
+    q = torch.randn(1, 4, 2, 32, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda")
+    for leaf, f in ((x, lambda: T.gated_norm(x, pre_weight=w)[1]), (b, lambda: T.gated_norm(x.detach(), pre_weight=w, pre_bias=b)[1]),
+                    (q, lambda: T.window_attention(q, q.detach(), q.detach()))):
+        first = torch.autograd.grad(f().square().sum(), leaf)[0]
+        loss = f().square().sum()
+        d, = torch.autograd.grad(loss, leaf, create_graph=True)
+        assert torch.equal(d, first)
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            (loss + d.square().sum()).backward()
+        leaf.grad = None                                   # the part of `loss` may have arrived before
+        f().square().sum().backward(create_graph=True)     # without them nothing is refused
+        assert torch.equal(leaf.grad, first)
+        leaf.grad = None
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_token_by_token_over_a_cache(dtype):
     """The block's attention for the last token of growing sequences: what window_attention gives for that row."""
