@@ -941,6 +941,11 @@ class AdamWList:
         instead: the coefficient of this list's own gradient norm, which is then returned.  step: the count of this step, from
         1; or a CUDA int32 tensor of one value that holds it, read when the step runs (a captured step needs that: the
         caller adds 1 to it inside the capture).  seed: of the random bits of stochastic roundings."""
+        if not torch.is_tensor(step) and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamWList.step: a captured step would repeat one step count: pass `step` as a CUDA int32 tensor")
+        return self._step(grads, step, lr, betas, eps, weight_decay, coef, max_norm, seed)
+
+    def _step(self, grads, step, lr, betas, eps, weight_decay, coef=None, max_norm=None, seed=0):
         if len(grads) != len(self.sizes):
             raise RuntimeError(f"AdamWList.step: {len(grads)} gradients for {len(self.sizes)} parameters")
         if not all(map(torch.Tensor.is_contiguous, grads)):
@@ -965,8 +970,6 @@ class AdamWList:
         norm = dyn = None
         scale = _at(coef)
         with _on(self.device):
-            if not on_device and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdamWList.step: a captured step would repeat one step count: pass `step` as a CUDA int32 tensor")
             g = _address(_addresses(grads))
             if max_norm is not None:
                 out = _grad_norm(g, self._pointers[-1], self._kinds, len(grads), float(max_norm), self.device, self._norm_ws)
@@ -995,7 +998,8 @@ def moment_values(exp_avg, exp_avg_sq, scale):
 class AdamW:
     """torch.optim.AdamW (amsgrad off) on the library's kernel; state_dict()/load_state_dict() use torch's layout.
     state_bits = 8 holds the moments in a byte each (AdamWList), with a third state tensor 'scale'; its stochastic rounding
-    draws from `seed`."""
+    draws from `seed`.  A captured step keeps the step count that it was captured with, in every replay (AdamWList.step takes a
+    count that lives on the device); where it would round stochastically it is refused, for its random bits would repeat."""
 
     def __init__(self, param_groups, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if state_bits not in (8, 32):
@@ -1053,9 +1057,12 @@ class AdamW:
                 part = parts.setdefault((id(c), st["step"], p.dtype, p.device), (c, [], []))
                 part[1].append(p)
                 part[2].append(st)
-            for k, ((_, done, _, _), (c, ps, sts)) in enumerate(parts.items()):
-                self._list(ps, sts).step([p.grad for p in ps], done + 1, g["lr"], g["betas"], g["eps"], g["weight_decay"], coef=c,
-                                         seed=self.seed + 0x10001 * gi + 0x1000003 * k)
+            for k, ((_, done, dtype, device), (c, ps, sts)) in enumerate(parts.items()):
+                with _on(device):
+                    if (self.state_bits == 8 or dtype is torch.bfloat16) and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW.step: a captured step would repeat its random bits: use AdamWList.step with a step count on the device")
+                hyper = (g["lr"], g["betas"], g["eps"], g["weight_decay"], c, None, self.seed + 0x10001 * gi + 0x1000003 * k)
+                self._list(ps, sts)._step([p.grad for p in ps], done + 1, *hyper)
                 for st in sts:
                     st["step"] = done + 1
 

@@ -361,6 +361,49 @@ def test_optimizer_class_follows_exchanged_memory():
     assert bool((p < 4.95).all()) and bool((old > 0.89).all())
 
 
+def one_by_one(ps, grads, states, step, **h):
+    """The entry for one tensor, parameter by parameter."""
+    from probtalk_amd import _lib
+    p = _lib.ptr
+    for x, g, (m, v) in zip(ps, grads, states):
+        _lib.check(_lib.lib().pt_train_adamw(p(x), p(g), p(m), p(v), x.numel(), None, h["lr"], *h["betas"], h["eps"], h["weight_decay"], step, _lib.stream()))
+
+
+def test_optimizer_class_in_a_graph_keeps_its_step_count():
+    """fp32 with 32-bit moments: what a captured step did when it launched a kernel for every tensor."""
+    sizes = [5000, 17]
+    ps, qs = ([torch.nn.Parameter(t) for t in tensors(sizes, 2)] for _ in range(2))
+    gs = tensors(sizes, 3, 0.1)
+    opt = T.AdamW([{"params": ps}], **H)
+    states = [[torch.zeros_like(q) for _ in range(2)] for q in qs]
+    for p, g in zip(ps, gs):
+        p.grad = g
+    opt.step()
+    one_by_one([q.detach() for q in qs], gs, states, 1, **H)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        for g in gs:
+            g.mul_(0.8)
+        graph.replay()
+        torch.cuda.synchronize()
+        one_by_one([q.detach() for q in qs], gs, states, 2, **H)
+        assert all(torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg_sq"], s[1]) for p, q, s in zip(ps, qs, states))
+    low = T.AdamW([{"params": qs}], state_bits=8)
+    for q, g in zip(qs, gs):
+        q.grad = g
+    low.step()
+    torch.cuda.synchronize()
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other):
+        with pytest.raises(RuntimeError, match="random bits"):
+            low.step()
+        gs[0].mul_(1.0)
+    del graph, other
+
+
 def test_refusals():
     p, m, v = (torch.zeros(300, device="cuda") for _ in range(3))
     u, w, s = torch.zeros(300, device="cuda", dtype=torch.uint8), torch.zeros(300, device="cuda", dtype=torch.uint8), torch.zeros(2, 2, device="cuda")
