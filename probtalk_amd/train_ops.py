@@ -896,6 +896,12 @@ def clip_grad_norm(params, max_norm):
     return grad_norm([p.grad for p in params if p.grad is not None], max_norm)
 
 
+def _overlap(tensors):
+    """Whether two of these contiguous tensors share memory."""
+    at = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel())
+    return any([a + n > b for (a, n), (b, _) in zip(at, at[1:])])
+
+
 class AdamWList:
     """AdamW over a fixed list of tensors, a few launches a step whatever their number.
 
@@ -929,6 +935,8 @@ class AdamWList:
             used = [x for x in a or () if x]
             if len(set(used)) != len(used):
                 raise RuntimeError("AdamWList: the same tensor twice")
+        if _overlap([t for x in lists for t in x]):
+            raise RuntimeError("AdamWList: two tensors share memory")
         self.sizes = [p.numel() for p in params]
         self._n = array.array("q", self.sizes)
         self._bf16 = int(self.dtype is torch.bfloat16)
@@ -1035,14 +1043,16 @@ class AdamW:
         return st
 
     def _list(self, ps, sts):
-        """The AdamWList of these parameters: made once, and anew where a parameter's or a moment's memory is another."""
+        """The AdamWList of these parameters: made once, and anew where a parameter's or a moment's memory is another.  None where
+        parameters share memory."""
         key = tuple(map(id, ps))
         held = [x for k in self._names() for x in map(torch.Tensor.data_ptr, [st[k] for st in sts])] + list(map(torch.Tensor.data_ptr, ps))
         made = self._lists.get(key)
         if made is None or made[1] != held:
             if len(self._lists) >= 32:
                 self._lists.clear()
-            made = self._lists[key] = (AdamWList(ps, *([st[k] for st in sts] for k in self._names())), held, ps)
+            apart = len(ps) == 1 or not _overlap(ps)
+            made = self._lists[key] = (AdamWList(ps, *([st[k] for st in sts] for k in self._names())) if apart else None, held, ps)
         return made[0]
 
     def step(self, coefs=None):
@@ -1062,9 +1072,15 @@ class AdamW:
                     if (self.state_bits == 8 or dtype is torch.bfloat16) and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("AdamW.step: a captured step would repeat its random bits: use AdamWList.step with a step count on the device")
                 hyper = (g["lr"], g["betas"], g["eps"], g["weight_decay"], c, None, self.seed + 0x10001 * gi + 0x1000003 * k)
-                self._list(ps, sts)._step([p.grad for p in ps], done + 1, *hyper)
-                for st in sts:
-                    st["step"] = done + 1
+                whole = self._list(ps, sts)
+                if whole is not None:
+                    whole._step([p.grad for p in ps], done + 1, *hyper)
+                    for st in sts:
+                        st["step"] = done + 1
+                    continue
+                for p, st in zip(ps, sts):         # parameters that share memory: one after the other, as they come
+                    self._list([p], [st])._step([p.grad], st["step"] + 1, *hyper)
+                    st["step"] += 1
 
     def state_dict(self):
         idx, packed, groups = {}, {}, []

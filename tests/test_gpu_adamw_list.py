@@ -369,6 +369,42 @@ def one_by_one(ps, grads, states, step, **h):
         _lib.check(_lib.lib().pt_train_adamw(p(x), p(g), p(m), p(v), x.numel(), None, h["lr"], *h["betas"], h["eps"], h["weight_decay"], step, _lib.stream()))
 
 
+@pytest.mark.parametrize("shared", ["same", "part", "twice"])
+def test_optimizer_class_steps_parameters_that_share_memory_in_turn(shared):
+    def model():
+        flat = tensors([3000], 2)[0].clone()
+        if shared == "twice":
+            p = torch.nn.Parameter(flat[:1000])
+            return flat, [p, torch.nn.Parameter(flat[1000:]), p]
+        return flat, [torch.nn.Parameter(x) for x in ((flat, flat, flat[64:128]) if shared == "same" else (flat[:2000], flat[1024:], flat[:512]))]
+    (a, ps), (b, qs) = model(), model()
+    opt = T.AdamW([{"params": ps}], lr=H["lr"], betas=H["betas"], eps=H["eps"], weight_decay=H["weight_decay"])
+    states = {id(q): [torch.zeros_like(q) for _ in range(2)] for q in qs}
+    steps = 0
+    for k in range(2):
+        for i, p in enumerate(ps):
+            p.grad = tensors([p.numel()], 30 + 10 * k + i)[0]
+        opt.step()
+        gs = [p.grad for p in ps]
+        for q, g in zip(qs, gs):
+            steps += 1
+            count = k + 1 if shared != "twice" or q is qs[1] else (2 * k + 1 if steps % 3 == 1 else 2 * k + 2)
+            one_by_one([q.detach()], [g], [states[id(q)]], count, **H)
+        assert torch.equal(a, b), k
+    for p, q in zip(ps, qs):
+        assert torch.equal(opt.state[p]["exp_avg"], states[id(q)][0]) and torch.equal(opt.state[p]["exp_avg_sq"], states[id(q)][1])
+    assert opt.state[ps[0]]["step"] == (4 if shared == "twice" else 2) and opt.state[ps[1]]["step"] == 2
+
+
+def test_list_refuses_tensors_that_share_memory():
+    flat = torch.zeros(4000, device="cuda")
+    t = lambda: torch.zeros(1000, device="cuda")  # noqa: E731
+    for p, m, v in (([flat[:1000], flat[999:1999]], [t(), t()], [t(), t()]), ([flat[:1000]], [flat[500:1500]], [t()]), ([t()], [flat[:1000]], [flat[4:1004]])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            T.AdamWList(p, m, v)
+    T.AdamWList([flat[:1000], flat[3000:]], [flat[1000:2000], t()], [flat[2000:3000], t()])
+
+
 def test_optimizer_class_in_a_graph_keeps_its_step_count():
     """fp32 with 32-bit moments: what a captured step did when it launched a kernel for every tensor."""
     sizes = [5000, 17]
