@@ -1049,7 +1049,7 @@ class AdamW:
         held = [x for k in self._names() for x in map(torch.Tensor.data_ptr, [st[k] for st in sts])] + list(map(torch.Tensor.data_ptr, ps))
         made = self._lists.get(key)
         if made is None or made[1] != held:
-            if len(self._lists) >= 32:
+            if len(self._lists) >= 32 + 4 * len(self.param_groups):      # more than the lists that steps come back to
                 self._lists.clear()
             apart = len(ps) == 1 or not _overlap(ps)
             made = self._lists[key] = (AdamWList(ps, *([st[k] for st in sts] for k in self._names())) if apart else None, held, ps)

@@ -405,6 +405,18 @@ def test_list_refuses_tensors_that_share_memory():
     T.AdamWList([flat[:1000], flat[3000:]], [flat[1000:2000], t()], [flat[2000:3000], t()])
 
 
+def test_optimizer_class_makes_the_lists_of_many_groups_once(monkeypatch):
+    ps = [torch.nn.Parameter(t) for t in tensors([64 + i for i in range(90)], 2)]
+    opt = T.AdamW([{"params": ps[i:i + 2]} for i in range(0, 90, 2)])
+    made = []
+    monkeypatch.setattr(T, "AdamWList", lambda *a, of=T.AdamWList: made.append(1) or of(*a))
+    for k in range(3):
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        assert len(made) == 45, k
+
+
 def test_optimizer_class_in_a_graph_keeps_its_step_count():
     """fp32 with 32-bit moments: what a captured step did when it launched a kernel for every tensor."""
     sizes = [5000, 17]
