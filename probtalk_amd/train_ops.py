@@ -944,6 +944,9 @@ class AdamWList:
         self._pointers = [*map(_address, self._arrays), _address(self._n)]
         self._norm_ws = _lib.lib().pt_train_grad_norm_workspace_bytes(self._pointers[-1], len(params))
 
+    def __reduce__(self):                    # a copy has memory, and so addresses, of its own
+        return type(self), tuple(self._lists)
+
     def step(self, grads, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, coef=None, max_norm=None, seed=0):
         """One step with `grads` (of the parameters' type and sizes).  coef: device scalar that scales the gradients; max_norm
         instead: the coefficient of this list's own gradient norm, which is then returned.  step: the count of this step, from
@@ -1017,6 +1020,12 @@ class AdamW:
         self.state = {}
         self.state_bits, self.seed = state_bits, int(seed)
         self._lists = {}
+
+    def __getstate__(self):                  # lists are made anew where they are needed
+        return self.__dict__ | {"_lists": {}}
+
+    def __setstate__(self, state):
+        self.__dict__.update({"state_bits": 32, "seed": 0, "_lists": {}} | state)
 
     def zero_grad(self):
         for g in self.param_groups:
@@ -1096,6 +1105,7 @@ class AdamW:
 
     def load_state_dict(self, sd):
         flat = [p for g in self.param_groups for p in g["params"]]
+        self._lists.clear()                        # they hold the moments that are replaced
         for i, st in sd.get("state", {}).items():
             p = flat[int(i)]
             if self.state_bits == 8:

@@ -417,6 +417,37 @@ def test_optimizer_class_makes_the_lists_of_many_groups_once(monkeypatch):
         assert len(made) == 45, k
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_of_an_optimizer_are_apart(bits):
+    """copy.deepcopy and pickle after steps, as a sweep or a whole-object checkpoint makes them."""
+    import copy
+    import io
+    ps = [torch.nn.Parameter(t) for t in tensors([300, 17], 2)]
+    opt = T.AdamW([{"params": ps}], state_bits=bits, seed=4)
+
+    def step(o):
+        for i, p in enumerate(o.param_groups[0]["params"]):
+            p.grad = tensors([p.numel()], 40 + i)[0]
+        o.step()
+
+    step(opt)
+    held, file = [p.detach().clone() for p in ps], io.BytesIO()
+    torch.save(opt, file)
+    file.seek(0)
+    others = [copy.deepcopy(opt), torch.load(file, weights_only=False)]
+    for o in others:
+        step(o)
+    assert all(torch.equal(p, h) for p, h in zip(ps, held))
+    step(opt)
+    for o in others:
+        for p, q in zip(ps, o.param_groups[0]["params"]):
+            assert torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg"], o.state[q]["exp_avg"])
+    lists = T.AdamWList([torch.zeros(300, device="cuda")], [torch.zeros(300, device="cuda")], [torch.zeros(300, device="cuda")])
+    twin = copy.deepcopy(lists)
+    twin.step([torch.ones(300, device="cuda")], 1)
+    assert all(bool((t[0] == 0).all()) for t in lists._lists) and bool((twin._lists[0][0] != 0).all())
+
+
 def test_optimizer_class_in_a_graph_keeps_its_step_count():
     """fp32 with 32-bit moments: what a captured step did when it launched a kernel for every tensor."""
     sizes = [5000, 17]
