@@ -241,6 +241,34 @@ def test_step_with_8_bit_moments(name, odd, dtype):
         assert np.array_equal(got[0].cpu().numpy(), np.where(cm >= 128, -mm, mm)) and np.array_equal(got[1].cpu().numpy(), values(cv, 4, ws[:, 1]))
 
 
+@pytest.mark.parametrize("name", sorted(LISTS))
+@pytest.mark.parametrize("odd", [False, True])
+def test_step_of_bf16_parameters_with_32_bit_moments(name, odd):
+    """numpy's fp32, one operation at a time: the same bits of moments and of parameters, whose rounding takes 16 bits of the value's hash."""
+    sizes = LISTS[name]
+    bf = torch.bfloat16
+    p, g = tensors(sizes, 2, 1.0, bf, odd), tensors(sizes, 3, 0.1, bf, odd)
+    m, v = tensors(sizes, 4, 0.05, odd=odd), [t.square_() for t in tensors(sizes, 5, 0.05, odd=odd)]
+    before = [[t.float().cpu().numpy() for t in x] for x in (p, g, m, v)]
+    T.AdamWList(p, m, v).step(g, 3, coef=torch.tensor([0.37], device="cuda"), seed=11, **H)
+    b1, b2, lr, eps, wd = F(0.9), F(0.99), F(1e-3), F(1e-8), F(1e-2)
+    bc1, bc2 = F(1) - F(float(b1) ** 3), F(1) - F(float(b2) ** 3)
+    decay, size, root = F(1 - float(lr) * float(wd)), lr / bc1, np.sqrt(bc2)
+    block = 0
+    for i, n in enumerate(sizes):
+        P, G, M, V = (b[i] for b in before)
+        gr = G * F(0.37)
+        M = b1 * M + (F(1) - b1) * gr
+        V = b2 * V + ((F(1) - b2) * gr) * gr
+        want = P * decay - size * (M / (np.sqrt(V) / root + eps))
+        assert np.array_equal(m[i].cpu().numpy(), M) and np.array_equal(v[i].cpu().numpy(), V), (i, n)
+        with np.errstate(over="ignore"):
+            r = (hashed(np.arange(n) + block * 256, 11, 3) * U32(0xBB67AE85)) >> U32(16)
+        block += -(-n // 256)
+        codes16 = (want.view(U32) + r) >> U32(16)
+        assert np.array_equal(p[i].view(torch.int16).cpu().numpy().view(np.uint16), codes16.astype(np.uint16)), (i, n)
+
+
 def test_stochastic_roundings_have_no_bias():
     """Zero gradients and no decay: m and v only shrink, by less than a code step.  Over many values the mean of what is stored is
     the mean of what was to be stored: a rounding has a standard deviation of at most half a step, 1/16 and 1/32 of the value.
