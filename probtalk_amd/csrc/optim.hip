@@ -362,8 +362,8 @@ int launch_adamw_multi(void* const* p, const void* const* g, void* const* m, voi
     for (; i < count && k < AT; ++i) {
       if (n[i] == 0) continue;
       const uint64_t u = ((uint64_t)n[i] + UNIT - 1) / UNIT;
-      PT_CHECK(u < (1u << 30), "adamw_multi: tensor %d has too many values", i);
-      if (k && units + u >= (1u << 30)) break;
+      PT_CHECK(u < (1u << 24), "adamw_multi: tensor %d has too many values", i);       // a launch holds less than 2^32 threads
+      if (k && units + u >= (1u << 24)) break;
       t.p[k] = p[i]; t.g[k] = g[i]; t.m[k] = m[i]; t.v[k] = v[i]; t.s[k] = scales ? scales[i] : nullptr;
       const bool vec = !((((uintptr_t)p[i] | (uintptr_t)g[i]) & pmask) | (((uintptr_t)m[i] | (uintptr_t)v[i]) & smask));
       t.n[k] = (uint64_t)n[i] * 2 + (vec ? 1 : 0);
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void moment_values_kernel(const unsigned char*
 }
 int launch_moment_values(const unsigned char* m, const unsigned char* v, const float* scales, int64_t n, float* m_out, float* v_out,
                          hipStream_t s) {
-  PT_CHECK(n >= 0 && n < ((int64_t)1 << 41) && (n == 0 || (m && v && scales && m_out && v_out)), "moment_values: bad argument");
+  PT_CHECK(n >= 0 && n < ((int64_t)1 << 34) && (n == 0 || (m && v && scales && m_out && v_out)), "moment_values: bad argument");
   if (n == 0) return 0;
   const int vec = !(((uintptr_t)m | (uintptr_t)v) & 3) && !(((uintptr_t)m_out | (uintptr_t)v_out) & 15);
   PT_LAUNCH(moment_values_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, m, v, scales, (size_t)n, vec, m_out, v_out);

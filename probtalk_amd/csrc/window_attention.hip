@@ -928,28 +928,33 @@ __global__ __launch_bounds__((KvPlan<T, DP, SINK>::TH), DP * (int)sizeof(T) > 25
   }
 }
 
-// the first keys' gradients: 16 values a workgroup, each the sum of 16 runs of the shares
+// the first keys' gradients: 16 values a workgroup at a time, each the sum of 16 runs of the shares
 template <typename T>
 __global__ __launch_bounds__(256) void win_bwd_join_kernel(const WinArgs a, int slots) {
-  const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sinks * a.D, i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+  const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sinks * a.D;
   __shared__ float red[16][16];
-  float s = 0.f;
-  if (i < n) {
+  for (int64_t first = (int64_t)blockIdx.x * 16; first < n; first += (int64_t)gridDim.x * 16) {
+    const int64_t i = first + (threadIdx.x & 15);
+    float s = 0.f;
+    if (i < n) {
 #pragma unroll 8
-    for (int k = threadIdx.x >> 4; k < slots; k += 16) s += a.part[k * n + i];
-  }
-  red[threadIdx.x >> 4][threadIdx.x & 15] = s;
-  __syncthreads();
-  if (threadIdx.x >= 16 || i >= n) return;
-  s = 0.f;
+      for (int k = threadIdx.x >> 4; k < slots; k += 16) s += a.part[k * n + i];
+    }
+    red[threadIdx.x >> 4][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (threadIdx.x < 16 && i < n) {
+      s = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) s += red[k][threadIdx.x];
-  int64_t r = i;
-  const int d = (int)(r % a.D); r /= a.D;
-  const int key = (int)(r % a.sinks); r /= a.sinks;
-  const int which = (int)(r & 1); r >>= 1;
-  const int kvh = (int)(r % a.Hk), b = (int)(r / a.Hk);
-  ((T*)(which ? a.dv : a.dk))[(((int64_t)b * a.Nk + key) * a.Hk + kvh) * a.D + d] = (T)s;
+      for (int k = 0; k < 16; ++k) s += red[k][threadIdx.x];
+      int64_t r = i;
+      const int d = (int)(r % a.D); r /= a.D;
+      const int key = (int)(r % a.sinks); r /= a.sinks;
+      const int which = (int)(r & 1); r >>= 1;
+      const int kvh = (int)(r % a.Hk), b = (int)(r / a.Hk);
+      ((T*)(which ? a.dv : a.dk))[(((int64_t)b * a.Nk + key) * a.Hk + kvh) * a.D + d] = (T)s;
+    }
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1299,12 +1304,15 @@ static WinArgs win_args(const void* q, const void* k, const void* v, const int64
   return a;
 }
 
+// a launch holds less than 2^32 threads
+static bool one_launch(int64_t blocks, int threads) { return blocks * threads < ((int64_t)1 << 32); }
 static int64_t win_blocks(const WinArgs& a, int rows) { return (int64_t)((a.Nq + rows - 1) / rows) * a.H * a.B; }
 
 template <typename T, int DP>
 static int run_win_fwd(const WinArgs& a, hipStream_t s) {
   typedef RowPlan<T, DP> plan;
   constexpr int lds = plan::SETS * 4 * key_tile<T, DP>() * Tile<T, DP>::RB;
+  PT_CHECK(one_launch(win_blocks(a, plan::ROWS), plan::TH), "attention_window_fwd: too many rows and heads");
   PT_ENSURE_LDS((win_fwd_kernel<T, DP>), lds);
   PT_LAUNCH((win_fwd_kernel<T, DP>), dim3((unsigned)win_blocks(a, plan::ROWS)), dim3(plan::TH), lds, s, a);
   return 0;
@@ -1318,16 +1326,19 @@ template <typename T, int DP>
 static int run_win_bwd(const WinArgs& a, hipStream_t s) {
   typedef RowPlan<T, DP> plan;
   constexpr int lds = plan::SETS * 4 * key_tile_q<T, DP>() * Tile<T, DP>::RB, lds_kv = KvPlan<T, DP, false>::LDS, lds_sink = KvPlan<T, DP, true>::LDS;
+  typedef KvPlan<T, DP, false> kv;
+  const int64_t key_blocks = (int64_t)((a.Nk + kv::KEYS - 1) / kv::KEYS) * a.Hk * a.B, sink_blocks = (int64_t)((a.sinks + 31) / 32) * a.far_chunks * a.H * a.B;
+  PT_CHECK(one_launch(win_blocks(a, plan::ROWS), plan::TH) && one_launch(key_blocks, kv::TH) && one_launch(sink_blocks, KvPlan<T, DP, true>::TH),
+           "attention_window_bwd: too many rows and heads");
   PT_ENSURE_LDS((win_bwd_q_kernel<T, DP>), lds);
   PT_LAUNCH((win_bwd_q_kernel<T, DP>), dim3((unsigned)win_blocks(a, plan::ROWS)), dim3(plan::TH), lds, s, a);
-  const dim3 keys((unsigned)((a.Nk + KvPlan<T, DP, false>::KEYS - 1) / KvPlan<T, DP, false>::KEYS) * a.Hk * a.B);
   PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, false>), lds_kv);
-  PT_LAUNCH((win_bwd_kv_kernel<T, DP, false>), keys, dim3(KvPlan<T, DP, false>::TH), lds_kv, s, a);
+  PT_LAUNCH((win_bwd_kv_kernel<T, DP, false>), dim3((unsigned)key_blocks), dim3(kv::TH), lds_kv, s, a);
   if (a.far_chunks) {
     PT_ENSURE_LDS((win_bwd_kv_kernel<T, DP, true>), lds_sink);
-    PT_LAUNCH((win_bwd_kv_kernel<T, DP, true>), dim3((unsigned)((a.sinks + 31) / 32 * a.far_chunks) * a.H * a.B), dim3(KvPlan<T, DP, true>::TH), lds_sink, s, a);
+    PT_LAUNCH((win_bwd_kv_kernel<T, DP, true>), dim3((unsigned)sink_blocks), dim3(KvPlan<T, DP, true>::TH), lds_sink, s, a);
     const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sinks * a.D;
-    PT_LAUNCH(win_bwd_join_kernel<T>, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, a, 1 + a.far_chunks * (a.H / a.Hk));
+    PT_LAUNCH(win_bwd_join_kernel<T>, dim3((unsigned)std::min<int64_t>((n + 15) / 16, 1 << 20)), dim3(256), 0, s, a, 1 + a.far_chunks * (a.H / a.Hk));
   }
   return 0;
 }

@@ -247,6 +247,17 @@ def test_strides_and_scale(dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, same))
 
 
+def test_more_shares_of_first_keys_than_a_grid_has_threads():
+    """2^28 values of first keys' gradients to add up: the same bits as of a few sequences alone."""
+    case = (1024, 131, 131, 8, 8, 128, 0, 0, 128, None)
+    q, k, v, do, _ = make(case, torch.bfloat16)
+    got = grads(q, k, v, do, case, None)
+    for b in (0, 511, 1022):
+        few = [x.detach()[b:b + 2].clone().requires_grad_() for x in (q, k, v)]
+        want = grads(*few, do[b:b + 2], case, None)
+        assert all(torch.equal(got[n][b:b + 2], want[n]) for n in want), b
+
+
 def test_no_gradient_wanted_and_scores_of_any_size():
     q, k, v, do, _ = make(CASES["two row tiles"], torch.float32)
     o = T.window_attention(q, k, v, 40)

@@ -112,6 +112,23 @@ def test_gated_norm_refuses_a_bias_without_its_weight():
     refused(L.pt_train_gated_norm_bwd(p, 4, p, 4, n, n, n, p, p, p, p, p, p, p, n, n, n, n, n, n, p, 1 << 20, 2, 4, 2, 0, 0, None), "bias")
 
 
+def test_launches_of_more_threads_than_32_bits_count():
+    """The largest sizes are refused before anything is launched (a grid holds less than 2^32 threads)."""
+    L, p, n = _lib.lib(), C.c_void_p(256), None
+    st = (C.c_int64 * 9)(*([64] * 9))
+    for dtype in (0, 1):
+        big = (65535, 1, 1, 512, 1, 8, 0, 0, 0, 1.0, dtype)
+        refused(L.pt_attention_window_fwd(p, p, p, p, n, st, n, *big, None), "too many rows and heads")
+        refused(L.pt_attention_window_bwd(p, p, p, p, p, p, p, p, p, st, n, *big, p, 1 << 40, None), "too many rows and heads")
+        # the far rows of the first keys: four blocks of 32 keys for every head
+        far = (65535, 129, 129, 96, 96, 8, 0, 0, 128, 1.0, dtype)
+        refused(L.pt_attention_window_bwd(p, p, p, p, p, p, p, p, p, st, n, *far, p, 1 << 60, None), "too many rows and heads")
+    one = (C.c_void_p * 1)(256)
+    h = (None, 1e-3, 0.9, 0.99, 1e-8, 0.0)
+    refused(L.pt_train_adamw_multi(one, one, one, one, one, (C.c_int64 * 1)(1 << 35), 1, 1, *h, 1, None, None, 0, None), "too many values")
+    refused(L.pt_train_moment_values(p, p, p, 1 << 34, p, p, None), "bad argument")
+
+
 def test_gated_norm_counts_rows_beyond_2_to_the_30():
     """A clip of rows that 32 bits hold, but not twice: 512 blocks of 32 workers, five sums of 8 columns each (256 CUs)."""
     f = _lib.lib().pt_train_gated_norm_workspace_bytes
