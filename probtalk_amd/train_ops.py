@@ -1111,12 +1111,12 @@ class AdamW:
             if self.state_bits == 8:
                 if "scale" not in st:
                     raise RuntimeError("AdamW: a state with moments in 32 bits cannot be loaded with state_bits=8")
-                new = {k: st[k].to(p.device).clone() for k in self._names()}
+                new = {k: st[k].to(p.device).clone(memory_format=torch.contiguous_format) for k in self._names()}
             elif "scale" in st:                    # moments saved in 8 bits: what they stand for
                 m, v = moment_values(*(st[k].to("cuda") for k in ("exp_avg", "exp_avg_sq", "scale")))
                 new = {"exp_avg": m.to(p.device), "exp_avg_sq": v.to(p.device)}
             else:
-                new = {k: st[k].to(p.device).float().clone() for k in self._names()}
+                new = {k: st[k].to(p.device).float().clone(memory_format=torch.contiguous_format) for k in self._names()}
             self.state[p] = {"step": int(float(st["step"]))} | new
         for g, sg in zip(self.param_groups, sd.get("param_groups", [])):
             for k in ("lr", "betas", "eps", "weight_decay"):

@@ -378,6 +378,26 @@ def test_optimizer_class_in_8_bits_resumes_bit_for_bit():
         assert torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg"], opt2.state[q]["exp_avg"])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_class_loads_moments_in_any_order_of_memory(bits):
+    """A checkpoint's tensors keep the strides that they were saved with."""
+    def model():
+        return torch.nn.Parameter(tensors([30 * 40], 2)[0].view(30, 40))
+    p, q = model(), model()
+    opt, other = (T.AdamW([{"params": [x]}], state_bits=bits) for x in (p, q))
+    p.grad, q.grad = (tensors([1200], 3)[0].view(30, 40) for _ in range(2))
+    opt.step()
+    with torch.no_grad():
+        q.copy_(p)
+    sd = opt.state_dict()
+    for k in ("exp_avg", "exp_avg_sq"):
+        sd["state"][0][k] = sd["state"][0][k].t().contiguous().t()
+    other.load_state_dict(sd)
+    opt.step()
+    other.step()
+    assert torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg_sq"], other.state[q]["exp_avg_sq"])
+
+
 def test_optimizer_class_follows_exchanged_memory():
     p = torch.nn.Parameter(torch.ones(100, device="cuda"))
     opt = T.AdamW([{"params": [p]}], lr=0.1, weight_decay=0.0)
