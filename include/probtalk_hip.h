@@ -194,7 +194,7 @@ int pt_attention_bf16(const void* Q, int ldq, const void* K, int ldk, const void
  * left, right: -1 = no limit; sinks <= 128; lengths: B device int32 (NULL: Nk), taken into [0, Nk]; keys behind are not read.  A row
  * that sees nothing gives zeros.  o, dout, dq (B, Nq, H, D) and dk, dv (B, Nk, Hk, D) are contiguous; stats (16-byte aligned, of
  * stats_bytes; NULL: not wanted) is what the backward call needs.  Inside lengths[b] keys and values must be finite: one that is not may reach rows
- * within 128 positions of those that see it. */
+ * within 128 positions of those that see it; and in the backward pass so must q and dout, which may reach keys that near. */
 size_t pt_attention_window_stats_bytes(int B, int Nq, int H, int D, int dtype);
 int pt_attention_window_fwd(const void* q, const void* k, const void* v, void* o, void* stats, const int64_t* strides, const int32_t* lengths, int B,
                             int Nq, int Nk, int H, int Hk, int D, int left, int right, int sinks, float scale, int dtype, void* stream);

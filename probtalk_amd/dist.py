@@ -194,8 +194,8 @@ class GradientReducer:
 
     def agree(self, *scalars):
         """Rank 0's values of small device tensors (gradient norms, clip coefficients) replace everyone's, in place.
-        The norm kernels sum with floating-point atomics, so two ranks holding the same averaged gradient can differ in
-        the last bit of the norm; a clip coefficient that differs between ranks would let the replicas drift apart."""
+        A clip coefficient that differs between ranks would let the replicas drift apart.  The norm's sum has a fixed order, so ranks
+        that hold the same averaged gradient agree by themselves; this holds them together whatever the gradients came through."""
         if dist.get_world_size() == 1 or not scalars:
             return
         flat = torch.cat([t.detach().reshape(-1).float() for t in scalars])

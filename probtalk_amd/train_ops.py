@@ -261,8 +261,8 @@ def gated_norm(x, t=None, gate=None, res_scale=None, post_weight=None, post_bias
     x, t: rows (R, C) of fp32 or bf16, 1 <= C <= 8192.  gate (R / rows_per_clip, C) of x's type: a row for every rows_per_clip rows
     (by default as many as it has rows for).  Vectors of C values in fp32.  kind: 'layer' (mean and variance) or 'rms'.  Left out:
     t (y is x itself), gate, res_scale, post_weight (u = t), pre_weight (h is None).  Statistics and sums are fp32; h is taken from y
-    before that is rounded to bf16.  No forward-mode and no second derivatives.  To capture the backward pass into a HIP graph, make the leaves inside the capture
-    (x.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
+    before that is rounded to bf16.  No forward-mode and no second derivatives.  To capture the backward pass into a HIP graph, make
+    the leaves inside the capture (x.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16) or not 1 <= x.shape[1] <= 8192 or x.shape[0] < 1:
         raise RuntimeError(f"gated_norm: rows (R, C) of fp32 or bf16 on the GPU with C up to 8192, got {tuple(x.shape)} {x.dtype} on {x.device}")
     if kind != "layer" and kind != "rms":
@@ -461,9 +461,10 @@ def window_attention(q, k, v, left=None, right=0, sinks=0, lengths=None, scale=N
 
     left, right: None for no limit (right = 0 is causal); sinks: first keys that stay visible, up to 128; lengths: int32 (B,), the
     keys of each sequence of a padded batch (what lies behind is not read; all of them by default).  A row that sees nothing gives
-    zeros and no gradient.  Softmax and sums are fp32; scale is 1 / sqrt(D) by default.  Keys and values inside a sequence must be
-    finite.  With gradients, bf16 keeps a byte more of every output value for them.  The backward pass is free of
-    atomics: the same inputs give the same bits.  No forward-mode and no second derivatives.  To capture it into a HIP graph, make the leaves inside the capture
+    zeros and no gradient.  Softmax and sums are fp32, probabilities and their gradients 16 bits or more, results are rounded once;
+    scale is 1 / sqrt(D) by default.  Keys and values inside a sequence must be finite, with gradients q and the output's gradient too.
+    With gradients, bf16 keeps a byte more of every output value for them.  The backward pass is free of atomics: the same inputs give
+    the same bits.  No forward-mode and no second derivatives.  To capture it into a HIP graph, make the leaves inside the capture
     (q.detach().requires_grad_()): an eager graph of the same leaves must not be alive."""
     if q.dim() != 4 or q.shape[0] < 1 or q.shape[1] < 1:
         raise RuntimeError(f"window_attention: q is (B, Nq, H, D), got {tuple(q.shape)}")
