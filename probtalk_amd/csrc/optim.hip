@@ -9,8 +9,8 @@
 // The list travels as kernel arguments (pointers, sizes and the first work unit of each tensor; AT tensors a launch, below the
 // 4 KB that a launch is sure to take), so nothing is uploaded, nothing is kept between calls and a captured step owns its
 // table.  A workgroup takes one unit of one tensor and finds the tensor by bisection over the scalar table.
-// The step alone: 160 tensors of 40 M fp32 values 180 us, 6.2 TB/s (most gradients come from the Infinity Cache); with 8-bit moments 117 us,
-// 5.5 TB/s; 310 tensors of 160 M bf16 values with 8-bit moments 380 to 430 us, about 4 TB/s
+// The step alone: 226 tensors of 40 M fp32 values 180 us, 6.2 TB/s (most gradients come from the Infinity Cache); with 8-bit moments 119 us,
+// 5.4 TB/s; 310 tensors of 160 M bf16 values with 8-bit moments 370 us in a row, 4.3 TB/s (450 when traced launch by launch)
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

@@ -7,7 +7,7 @@
 //     dV = P^T dO,  dS = P (dO V^T - delta) scale,  dQ = dS K,  dK = dS^T Q      (dK, dV summed over the query heads of a group)
 //
 // Bound by the matrix cores (4 D flops a visible pair forward, 14 D backward: S and dP are computed in both of its kernels, which
-// costs 4 D and saves the atomics or the round trip of dQ) and, next to them, by the exponentials on the vector unit.
+// costs 4 D and saves the atomics or the round trip of dQ; bf16 6 D and 20 D, see split) and, next to them, by the exponentials on the vector unit.
 //
 // Layout.  All products are 32 x 32 tiles with 16 contraction steps: bf16 one v_mfma_f32_32x32x16_bf16, fp32 eight
 // v_mfma_f32_32x32x2_f32 on the same lanes (element e of a lane's eight is contraction step 8 (lane / 32) + e in both, so one code
@@ -211,7 +211,7 @@ struct Cols<float, DP> {
 };
 // The registers of a score tile as the second operand of a product.  bf16: as the sum of two bf16 values, 2^-17 off.  One alone is 2^-8 off, and so is
 // the result, however many keys share a row's weight: 1.44 times the error of rounding the exact result, and more where few rows add up.
-// 8192 rows, 1028 keys, 16 heads over 4, D = 128, one value and two: forward 113 and 137 us, dQ 166 and 191, dK / dV 183 and 233
+// 8192 rows, 1028 keys, 16 heads over 4, D = 128, one value and two: forward 106 and 133 us, dQ 155 and 189, dK / dV 169 and 230
 template <typename T>
 __device__ __forceinline__ void split(const f32x16& p, int s2, typename Types<T>::frag& hi, typename Types<T>::frag& lo) {
 #pragma unroll
@@ -447,8 +447,8 @@ struct RowPlan {                                         // WAVES: per SIMD
 };
 
 // ---------------------------------------------------------------------------
-// Forward: waves of 32 rows each over common key tiles (RowPlan).  bf16, 8192 rows that see 1028 keys, 16 heads over 4, D = 128: 137 us,
-// 470 TFLOP/s of visible pairs; its products (three for the formula's two) alone would take 99 us at the rate of a large matrix product on this card, the
+// Forward: waves of 32 rows each over common key tiles (RowPlan).  bf16, 8192 rows that see 1028 keys, 16 heads over 4, D = 128: 133 us,
+// 486 TFLOP/s of visible pairs; its products (three for the formula's two) alone would take 99 us at the rate of a large matrix product on this card, the
 // rest is softmax, the window's edges and loads that they do not cover.  fp32: see RowPlan
 // ---------------------------------------------------------------------------
 template <typename T, int DP>
@@ -583,7 +583,7 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
 }
 
 // ---------------------------------------------------------------------------
-// Backward, dQ (and delta): rows and key tiles as forward.  The case above: 191 us for four products of the formula's three (507 TFLOP/s of visible pairs)
+// Backward, dQ (and delta): rows and key tiles as forward.  The case above: 189 us for four products of the formula's three (513 TFLOP/s of visible pairs)
 // ---------------------------------------------------------------------------
 template <typename T, int DP> constexpr int key_tile_q() { return sizeof(T) * DP <= 128 ? 64 : 32; }   // 256 registers hold no more
 template <typename T, int DP>
@@ -707,7 +707,7 @@ __global__ __launch_bounds__((RowPlan<T, DP>::TH), (RowPlan<T, DP>::WAVES)) void
 // on the tile's first 32 rows and one on the others, added up at the end (there are too few blocks of keys to fill the chip with
 // 4 waves each).  The keys stay in registers as operands; in bf16, rows of more than 128 bytes leave no room for the values beside them (two
 // waves a SIMD have 256 registers each, half of them hold the results), so these are read from LDS, where they stay too.
-// The case above: 233 us for six products of the formula's four (554 TFLOP/s of visible pairs).  fp32 with D up to 64: 2 blocks of keys, values in registers, two
+// The case above: 230 us for six products of the formula's four (562 TFLOP/s of visible pairs).  fp32 with D up to 64: 2 blocks of keys, values in registers, two
 // workgroups on a CU (105 -> 57 us where the row kernels gain as RowPlan says).
 // SINK: the rows far behind the window, which see the first 32-key blocks as sinks only.  There are as many of these rows as the
 // sequence is long and only a few keys, so the waves take the SAME keys and 32 rows of a tile each, the rows are cut into
