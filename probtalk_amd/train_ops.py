@@ -953,8 +953,10 @@ class AdamWList:
         instead: the coefficient of this list's own gradient norm, which is then returned.  step: the count of this step, from
         1; or a CUDA int32 tensor of one value that holds it, read when the step runs (a captured step needs that: the
         caller adds 1 to it inside the capture).  seed: of the random bits of stochastic roundings."""
-        if not torch.is_tensor(step) and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamWList.step: a captured step would repeat one step count: pass `step` as a CUDA int32 tensor")
+        if not torch.is_tensor(step):
+            with _on(self.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamWList.step: a captured step would repeat one step count: pass `step` as a CUDA int32 tensor")
         return self._step(grads, step, lr, betas, eps, weight_decay, coef, max_norm, seed)
 
     def _step(self, grads, step, lr, betas, eps, weight_decay, coef=None, max_norm=None, seed=0):
