@@ -17,9 +17,9 @@
 // gradient is a register sum too, stored once per clip (or joined within the block, and added up in order by the second kernel with
 // the other column sums).  No atomics: the same inputs give the same bits.
 //
-// Measured: 49,152 x 2048 bf16 forward 180 us (4.5 TB/s; a copy of this size runs at 4.9); 45,056 x 512 fp32 forward 80 us (4.6 TB/s; 64
-// where its inputs lie in the caches), with all gradients 195; 16,384 x 4096 bf16 with gradients 287; lanes to the row's length: 200,000 x 64 bf16 forward 107 -> 27 us, with
-// gradients 349 -> 189
+// Measured: 49,152 x 2048 bf16 forward 180 us (4.5 TB/s; a copy of this size runs at 4.9); 45,056 x 512 fp32 forward 80 us (4.6 TB/s;
+// 64 where its inputs lie in the caches), with all gradients 195; 16,384 x 4096 bf16 with gradients 290; lanes to the row's length:
+// 200,000 x 64 bf16 forward 107 -> 27 us, with gradients 349 -> 189
 #include <algorithm>
 #include <cstdint>
 
